@@ -299,6 +299,73 @@ typedef struct q3_sampler {
 } q3_sampler;
 int q3_sample_topk(const q3_sampler* sampler, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * An 8-bit paged K/V cache, and attention over it. No reference counterpart (the reference keeps its cache in bf16).
+ * Each head of a token row (128 values) is stored as 128 e4m3 bytes and one E8M0 scale byte s: value = e4m3 * 2^(s-127).
+ * Writing takes the least exponent e in [-96, 119] with max |x| <= 448 * 2^e over the head's finite values and rounds
+ * x * 2^-e to e4m3 once, half to even (beyond 448 * 2^119 it saturates); infinities and NaN become NaN. Reading back
+ * is exact in bf16. 2064 bytes per token (K and V) where bf16 takes 4096. */
+typedef struct q3_quant_cache {
+  void* k;                     /* [num_pages, page_size, 8, 128] e4m3, contiguous, 16-byte aligned */
+  void* v;
+  void* k_scale;               /* [num_pages, page_size, 8] E8M0 bytes, contiguous, 8-byte aligned */
+  void* v_scale;
+  int32_t num_pages;
+  int32_t page_size;
+} q3_quant_cache;
+
+/* q3_kv_append_slots / q3_kv_append_paged for an 8-bit cache: row i of k/v (bf16 [8, 128], row_stride elements apart)
+ * is quantised into pool row slots[i], or into token positions[i] of seat seat_of_row[i] (NULL: seat i) of the
+ * num_seats block-table rows. A row whose slot, seat, position or page is out of range is skipped and raises its
+ * status bit. The destinations of one call must differ; which row's bytes a repeated one ends up with is unspecified. */
+int q3_kv_quant_append_slots(const void* k, const void* v, int64_t row_stride, const q3_quant_cache* cache,
+                             int32_t num_kv_heads, int32_t head_dim, const int64_t* slots, int32_t n_rows, void* stream);
+int q3_kv_quant_append_paged(const void* k, const void* v, int64_t row_stride, const q3_quant_cache* cache,
+                             int32_t num_kv_heads, int32_t head_dim, const int32_t* positions,
+                             const int32_t* seat_of_row, const int32_t* block_table, int64_t block_table_stride,
+                             int32_t num_seats, int32_t max_pages_per_seat, int32_t n_rows, void* stream);
+/* Rows read back as bf16 [8, 128] (out_row_stride elements apart), addressed as in q3_kv_quant_append_paged. A row out
+ * of range is written as zeros and raises its status bit. */
+int q3_kv_dequant_paged(const q3_quant_cache* cache, int32_t num_kv_heads, int32_t head_dim, const int32_t* positions,
+                        const int32_t* seat_of_row, const int32_t* block_table, int64_t block_table_stride,
+                        int32_t num_seats, int32_t max_pages_per_seat, void* k_out, void* v_out,
+                        int64_t out_row_stride, int32_t n_rows, void* stream);
+
+/* Attention of each seat's drafted tokens (speculative decoding), or of its one next token over an 8-bit cache.
+ * Token i < draft_lens[b] (NULL: tokens) of seat b attends over the seat's cache_seqlens[b] cached rows and over the
+ * drafted rows j < draft_lens[b] with bit j of tree_mask[b, i] set (a token that sees itself has its own bit set). The
+ * drafted rows are read where they are and not written to the cache: after verification the accepted ones are appended.
+ * A token with nothing to see, and one at or past draft_lens[b], gets a zero row. Values that a token does not see do
+ * not reach its output, whatever they are. k_new == NULL: no drafted rows (tree_mask and draft_lens are not read).
+ * The cache is bf16 (k_scale == v_scale == NULL) or the 8-bit format above. Sums and softmax statistics are fp32.
+ * 1 <= tokens <= 64; the workspace (q3_paged_tree_workspace_bytes, 256-byte aligned) needs no initialisation and may
+ * not be shared by calls that overlap. Entries of the block table outside the pool read page 0 and raise a status bit. */
+typedef struct q3_tree_attn {
+  const void* q;               /* bf16 [batch, tokens, 16, 128], heads contiguous; strides in elements */
+  int64_t q_seat_stride, q_token_stride;
+  const void* k_new;           /* bf16 [batch, tokens, 8, 128] drafted rows, or NULL */
+  const void* v_new;
+  int64_t kv_new_seat_stride, kv_new_token_stride;
+  const int64_t* tree_mask;    /* [batch, tokens] visibility words, rows tree_mask_stride apart (0: one row for all) */
+  int64_t tree_mask_stride;
+  const int32_t* draft_lens;   /* optional [batch] */
+  const void* k_pool;          /* [num_pages, page_size, 8, 128], contiguous */
+  const void* v_pool;
+  const void* k_scale;         /* [num_pages, page_size, 8] E8M0, or NULL (bf16 pools) */
+  const void* v_scale;
+  int32_t num_pages, page_size;
+  const int32_t* cache_seqlens;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  int32_t max_pages_per_seat;
+  int32_t batch, tokens, num_heads, num_kv_heads, head_dim;
+  float softmax_scale;
+  void* out;                   /* bf16 [batch, tokens, 16, 128], strides in elements */
+  int64_t out_seat_stride, out_token_stride;
+} q3_tree_attn;
+size_t q3_paged_tree_workspace_bytes(int32_t batch, int32_t tokens, int32_t quantised);
+int q3_paged_tree_attn(const q3_tree_attn* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -747,4 +747,163 @@ int q3_prefill(const void* q, int64_t q_row_stride, int64_t q_rows, const void* 
   return record(q3::launch_prefill(a, static_cast<cudaStream_t>(stream)));
 }
 
+static int quant_cache_check(const q3_quant_cache* c) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || c->num_pages <= 0 || c->page_size <= 0) return Q3_ERR_INVALID;
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 8) || !aligned(c->v_scale, 8))
+    return Q3_ERR_ALIGNMENT;
+  return Q3_OK;
+}
+
+// Checks and arguments common to the 8-bit cache's row entries (rows: the bf16 side, k_rows / v_rows).
+static int quant_common(q3::KvQuantArgs& a, const q3_quant_cache* cache, int32_t nkv, int32_t hd, const void* k_rows,
+                        const void* v_rows, int64_t row_stride, int32_t n_rows, int* dev) {
+  int rc;
+  if (nkv != q3::kKvHeads || hd != q3::kHeadDim) return Q3_ERR_UNSUPPORTED;
+  if ((rc = quant_cache_check(cache)) != Q3_OK) return rc;
+  if (!k_rows || !v_rows || row_stride < q3::kKvHeads * q3::kHeadDim) return Q3_ERR_INVALID;
+  if (!aligned(k_rows, 16) || !aligned(v_rows, 16) || (row_stride % 8)) return Q3_ERR_ALIGNMENT;
+  if ((rc = current_device(dev)) != Q3_OK) return rc;
+  if ((rc = status_ptr(*dev, &a.status)) != Q3_OK) return rc;
+  a.k_pool = static_cast<uint8_t*>(cache->k);
+  a.v_pool = static_cast<uint8_t*>(cache->v);
+  a.k_scale = static_cast<uint8_t*>(cache->k_scale);
+  a.v_scale = static_cast<uint8_t*>(cache->v_scale);
+  a.pool_rows = static_cast<long long>(cache->num_pages) * cache->page_size;
+  a.page_size = cache->page_size;
+  a.n_rows = n_rows;
+  return Q3_OK;
+}
+
+static int quant_paged(q3::KvQuantArgs& a, const int32_t* positions, const int32_t* seat_of_row,
+                       const int32_t* block_table, int64_t block_table_stride, int32_t num_seats, int32_t max_pages) {
+  if (!positions || !block_table || num_seats <= 0 || max_pages <= 0 || block_table_stride < max_pages)
+    return Q3_ERR_INVALID;
+  a.positions = positions;
+  a.seat_of_row = seat_of_row;
+  a.block_table = block_table;
+  a.bt_stride = block_table_stride;
+  a.num_seats = num_seats;
+  a.max_pages = max_pages;
+  return Q3_OK;
+}
+
+int q3_kv_quant_append_slots(const void* k, const void* v, int64_t row_stride, const q3_quant_cache* cache,
+                             int32_t num_kv_heads, int32_t head_dim, const int64_t* slots, int32_t n_rows, void* stream) {
+  if (n_rows < 0) return Q3_ERR_INVALID;
+  if (n_rows == 0) return Q3_OK;
+  if (!slots) return Q3_ERR_INVALID;
+  q3::KvQuantArgs a{};
+  a.slots = slots;
+  int dev = 0, rc = quant_common(a, cache, num_kv_heads, head_dim, k, v, row_stride, n_rows, &dev);
+  if (rc != Q3_OK) return rc;
+  a.k_rows = static_cast<const __nv_bfloat16*>(k);
+  a.v_rows = static_cast<const __nv_bfloat16*>(v);
+  a.rows_stride = row_stride;
+  return record(q3::launch_kv_quant_append(a, sm_count(dev), static_cast<cudaStream_t>(stream)));
+}
+
+int q3_kv_quant_append_paged(const void* k, const void* v, int64_t row_stride, const q3_quant_cache* cache,
+                             int32_t num_kv_heads, int32_t head_dim, const int32_t* positions,
+                             const int32_t* seat_of_row, const int32_t* block_table, int64_t block_table_stride,
+                             int32_t num_seats, int32_t max_pages_per_seat, int32_t n_rows, void* stream) {
+  if (n_rows < 0) return Q3_ERR_INVALID;
+  if (n_rows == 0) return Q3_OK;
+  q3::KvQuantArgs a{};
+  int dev = 0, rc = quant_paged(a, positions, seat_of_row, block_table, block_table_stride, num_seats, max_pages_per_seat);
+  if (rc != Q3_OK) return rc;
+  if ((rc = quant_common(a, cache, num_kv_heads, head_dim, k, v, row_stride, n_rows, &dev)) != Q3_OK) return rc;
+  a.k_rows = static_cast<const __nv_bfloat16*>(k);
+  a.v_rows = static_cast<const __nv_bfloat16*>(v);
+  a.rows_stride = row_stride;
+  return record(q3::launch_kv_quant_append(a, sm_count(dev), static_cast<cudaStream_t>(stream)));
+}
+
+int q3_kv_dequant_paged(const q3_quant_cache* cache, int32_t num_kv_heads, int32_t head_dim, const int32_t* positions,
+                        const int32_t* seat_of_row, const int32_t* block_table, int64_t block_table_stride,
+                        int32_t num_seats, int32_t max_pages_per_seat, void* k_out, void* v_out,
+                        int64_t out_row_stride, int32_t n_rows, void* stream) {
+  if (n_rows < 0) return Q3_ERR_INVALID;
+  if (n_rows == 0) return Q3_OK;
+  q3::KvQuantArgs a{};
+  int dev = 0, rc = quant_paged(a, positions, seat_of_row, block_table, block_table_stride, num_seats, max_pages_per_seat);
+  if (rc != Q3_OK) return rc;
+  if ((rc = quant_common(a, cache, num_kv_heads, head_dim, k_out, v_out, out_row_stride, n_rows, &dev)) != Q3_OK) return rc;
+  return record(q3::launch_kv_dequant(a, static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out),
+                                      out_row_stride, sm_count(dev), static_cast<cudaStream_t>(stream)));
+}
+
+size_t q3_paged_tree_workspace_bytes(int32_t batch, int32_t tokens, int32_t quantised) {
+  int dev = 0;
+  if (batch < 0 || tokens < 1 || tokens > q3::kTreeMaxTokens || current_device(&dev) != Q3_OK) return 0;
+  return q3::tree_workspace(quantised != 0, batch, tokens, sm_count(dev)).bytes;
+}
+
+int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!p) return Q3_ERR_INVALID;
+  int rc = check_family(p->num_heads, p->num_kv_heads, p->head_dim);
+  if (rc != Q3_OK) return rc;
+  if (p->tokens > q3::kTreeMaxTokens) return Q3_ERR_UNSUPPORTED;
+  if (p->batch < 0 || p->tokens < 1 || p->num_pages <= 0 || p->page_size <= 0 || p->max_pages_per_seat <= 0)
+    return Q3_ERR_INVALID;
+  if (p->batch == 0) return Q3_OK;
+  if (!p->q || !p->k_pool || !p->v_pool || !p->cache_seqlens || !p->block_table || !p->out ||
+      (p->k_new == nullptr) != (p->v_new == nullptr) || (p->k_scale == nullptr) != (p->v_scale == nullptr))
+    return Q3_ERR_INVALID;
+  const bool draft = p->k_new != nullptr;
+  constexpr int64_t kQ = q3::kQHeads * q3::kHeadDim, kKv = q3::kKvHeads * q3::kHeadDim;
+  if (p->q_token_stride < kQ || p->out_token_stride < kQ || p->q_seat_stride < 0 || p->out_seat_stride < 0 ||
+      p->block_table_stride < p->max_pages_per_seat ||
+      (draft && (!p->tree_mask || p->tree_mask_stride < 0 || p->kv_new_token_stride < kKv || p->kv_new_seat_stride < 0)))
+    return Q3_ERR_INVALID;
+  if (static_cast<long long>(p->max_pages_per_seat) * p->page_size > (1ll << 30) ||
+      static_cast<long long>(p->batch) * p->tokens > (1ll << 30))
+    return Q3_ERR_INVALID;
+  if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->k_pool, 16) || !aligned(p->v_pool, 16) ||
+      (p->q_seat_stride % 8) || (p->q_token_stride % 8) || (p->out_seat_stride % 8) || (p->out_token_stride % 8) ||
+      (p->k_scale && (!aligned(p->k_scale, 8) || !aligned(p->v_scale, 8))) ||
+      (draft && (!aligned(p->k_new, 16) || !aligned(p->v_new, 16) || !aligned(p->tree_mask, 8) ||
+                 (p->kv_new_seat_stride % 8) || (p->kv_new_token_stride % 8))))
+    return Q3_ERR_ALIGNMENT;
+  int dev = 0;
+  if ((rc = current_device(&dev)) != Q3_OK) return rc;
+  const q3::TreeWorkspace w = q3::tree_workspace(p->k_scale != nullptr, p->batch, p->tokens, sm_count(dev));
+  if (!workspace || workspace_bytes < w.bytes || !aligned(workspace, 256)) return Q3_ERR_WORKSPACE;
+  q3::TreeArgs a{};
+  if ((rc = status_ptr(dev, &a.status)) != Q3_OK) return rc;
+  a.q = static_cast<const __nv_bfloat16*>(p->q);
+  a.q_seat = p->q_seat_stride;
+  a.q_tok = p->q_token_stride;
+  if (draft) {
+    a.k_new = static_cast<const __nv_bfloat16*>(p->k_new);
+    a.v_new = static_cast<const __nv_bfloat16*>(p->v_new);
+    a.kv_seat = p->kv_new_seat_stride;
+    a.kv_tok = p->kv_new_token_stride;
+    a.mask = p->tree_mask;
+    a.mask_seat = p->tree_mask_stride;
+    a.draft_lens = p->draft_lens;
+  }
+  a.k_pool = p->k_pool;
+  a.v_pool = p->v_pool;
+  a.k_scale = static_cast<const uint8_t*>(p->k_scale);
+  a.v_scale = static_cast<const uint8_t*>(p->v_scale);
+  a.seqlens = p->cache_seqlens;
+  a.block_table = p->block_table;
+  a.bt_stride = p->block_table_stride;
+  a.max_pages = p->max_pages_per_seat;
+  a.num_pages = p->num_pages;
+  a.page_size = p->page_size;
+  a.B = p->batch;
+  a.tokens = p->tokens;
+  a.groups = w.groups;
+  a.scale_log2 = p->softmax_scale * q3::kLog2e;
+  a.out = static_cast<__nv_bfloat16*>(p->out);
+  a.out_seat = p->out_seat_stride;
+  a.out_tok = p->out_token_stride;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.ws_span = reinterpret_cast<int2*>(ws + w.span);
+  a.ws_ml = reinterpret_cast<float*>(ws + w.ml);
+  a.ws_o = reinterpret_cast<float*>(ws + w.o);
+  return record(q3::launch_paged_tree(a, w, static_cast<cudaStream_t>(stream)));
+}
+
 }  // extern "C"

@@ -1,0 +1,874 @@
+// Attention of a few drafted tokens per seat over a paged K/V cache (bf16 or e4m3 with E8M0 scales), sm_100a; with one
+// token and no draft rows it is decode attention over the 8-bit cache.
+//
+// Mathematics. Token i of a seat (head hq, KV head h = hq / 2) sees every cached row and those drafted rows j whose bit
+// j of mask[i] is set. In log2 units s_ij = scale * log2(e) * q_i . k_j and
+//   o_i = sum_j 2^(s_ij - m_i) v_j / sum_j 2^(s_ij - m_i),   m_i = max_j s_ij;   no visible row: o_i = 0,
+// accumulated online over tiles of 16 keys with one pass over the cache.
+// e4m3 rows: k_j = 2^ek(j) ky_j and v_j = 2^ev(j) vy_j. ek enters the score. ev must not be rounded into the 11 bits
+// of an fp16 probability, so P.V runs on w_ij = 2^(s_ij + ev(j) - m'_i) with a maximum of its own, m'_i =
+// max_j (s_ij + ev(j)); the sum of probabilities keeps m_i, and the result is scaled by 2^(m'_i - m_i) at the end. The
+// bytes of K and V convert to fp16 exactly; q is scaled by a power of two per (token, head) into fp16, exact unless an
+// element is 2^28 below the largest.
+//
+// Work split. A work item is a (seat, group of TOK tokens); its keys are cut into chunks of 16 cached rows and then
+// the drafted rows. The chunks of all items form one list, of which CTA c takes an equal contiguous share, so ragged
+// lengths balance and the grid depends only on the sizes the host knows. An item inside one CTA is written directly;
+// one that spans CTAs leaves an fp32 partial (output, maximum, sum) per CTA, which a second small kernel adds in CTA
+// order (deterministic; it is launched with programmatic stream serialisation, so its start-up hides under the first).
+//
+// Bound: HBM. A token row holds all 8 KV heads in 2048 (1024 for e4m3) contiguous bytes. One producer warp brings the
+// rows of a chunk into a ring of shared-memory stages, a lane per row and one bulk copy each, so any page size and page
+// boundary works; eight consumer warps take one KV head each. Rows are padded by 16 (64) bytes so that the fragment
+// loads of the matrix instructions are free of bank conflicts.
+// Scores S^T = K.Q^T and outputs O^T = V^T.P^T use mma.sync m16n8k16 with the 16 keys (dims) as the rows of A and the
+// 2 heads x 4 tokens as the 8 columns of B: with so few query columns the legacy tensor path is far below its limit.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "q3_common.cuh"
+#include "q3_kernels.h"
+
+namespace q3 {
+
+namespace {
+
+constexpr int kTreeConsumers = kKvHeads;                  // one warp per KV head
+constexpr int kTreeThreads = (kTreeConsumers + 1) * 32;   // and a producer warp
+constexpr int kTreeRows = 16;                             // cached rows per chunk
+
+// Stage layout. bf16: K rows 2112 bytes apart (four 16-byte units more than 2048), V rows 2064. e4m3: K and V rows
+// 1040 apart, then the scales [16][8] of K and of V; drafted rows (bf16, eight per chunk) use the same bytes, 2064
+// apart.
+template <bool FP8>
+struct TreeStage {
+  static constexpr int kRow = FP8 ? 1024 : 2048;
+  static constexpr int kKStride = FP8 ? 1040 : 2112;
+  static constexpr int kVStride = FP8 ? 1040 : 2064;
+  static constexpr int kV = kTreeRows * kKStride;
+  static constexpr int kScales = kV + kTreeRows * kVStride;
+  static constexpr int kBytes = kScales + (FP8 ? 2 * kTreeRows * kKvHeads : 0);
+  static constexpr int kDraftRows = FP8 ? 8 : 16;
+  static constexpr int kDraftKStride = FP8 ? 2064 : 2112;
+  static constexpr int kDraftVStride = 2064;
+  static_assert(kDraftRows * kDraftKStride <= kV && kV + kDraftRows * kDraftVStride <= kScales && kBytes % 16 == 0,
+                "drafted rows fit their stage");
+};
+
+struct Item {
+  int seat, tok0;      // first token of the group
+  int len, drafts;     // cached tokens; drafted rows
+  int nc, n;           // cache chunks; all chunks
+};
+
+template <int TOK, int DROWS>
+__device__ __forceinline__ Item tree_item(const TreeArgs& a, int w) {
+  Item it;
+  it.seat = a.groups == 1 ? w : w / a.groups;
+  it.tok0 = (w - it.seat * a.groups) * TOK;
+  const long long cap = static_cast<long long>(a.max_pages) * a.page_size;
+  const int raw = a.seqlens[it.seat];
+  it.len = raw < 0 ? 0 : static_cast<int>(raw > cap ? cap : raw);
+  it.drafts = a.k_new == nullptr ? 0 : a.tokens;
+  int live = a.tokens;
+  if (a.draft_lens != nullptr) {
+    const int d = a.draft_lens[it.seat];
+    live = it.drafts = d < 0 ? 0 : (d > a.tokens ? a.tokens : d);
+  }
+  it.nc = (it.len + kTreeRows - 1) / kTreeRows;
+  it.n = it.tok0 < live ? it.nc + (it.drafts + DROWS - 1) / DROWS : 0;
+  return it;
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                         __nv_bfloat16) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// An 8x8 matrix of 16-bit values (lane 4g + t: row g, columns 2t and 2t + 1) transposed across the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Two e4m3 bytes (the low 16 bits) as packed fp16, exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t x) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(x & 0xffffu), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+}
+
+__device__ __forceinline__ uint32_t pack_half2_rn(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ float max_over_rows(float v) {   // over the lanes that hold the same columns
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+__device__ __forceinline__ float sum_over_rows(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 4);
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+
+__device__ __forceinline__ uint32_t word4(const uint4& w, int e) {
+  return e == 0 ? w.x : (e == 1 ? w.y : (e == 2 ? w.z : w.w));
+}
+
+// What a consumer warp keeps of an item: lane 4g + t owns columns 2t and 2t + 1 (both heads of token 4 nt + t of the
+// group) of every 8-column tile nt, and of the outputs the dims row_dim(mt) (accumulators 0, 1) and row_dim(mt) + 1
+// (2, 3).
+template <bool FP8, int NT>
+struct TreeState {
+  uint32_t q[NT][8][2];    // B fragments of Q^T: for k-step s the four dims key_dim(t, s) .. + 3 of column g
+  float cf[NT][2];         // score factor of the lane's columns
+  float o[NT][8][4];
+  float m[NT][2];          // maximum that the outputs are relative to (FP8: of s + ev; else of s), the same in all g
+  float ms[NT][2];         // FP8: this lane's maximum of s, which l is relative to
+  float l[NT][2];          // this lane's part of the sum
+};
+
+template <bool FP8>
+__device__ __forceinline__ int key_dim(int t, int s) {
+  return FP8 ? 32 * t + 4 * s : 32 * (s >> 1) + 8 * t + 4 * (s & 1);
+}
+template <bool FP8>
+__device__ __forceinline__ int row_dim(int g, int mt) {
+  return FP8 ? 16 * g + 2 * mt : 64 * (mt >> 2) + 8 * g + 2 * (mt & 3);
+}
+
+template <bool FP8, int NT>
+__device__ __forceinline__ void tree_begin(const TreeArgs& a, const Item& it, int h, int lane, TreeState<FP8, NT>& st) {
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int tok = it.tok0 + 4 * nt + (g >> 1);
+    const bool have = tok < a.tokens;
+    const __nv_bfloat16* src = a.q + static_cast<long long>(it.seat) * a.q_seat + static_cast<long long>(have ? tok : 0) * a.q_tok +
+                               (2 * h + (g & 1)) * kHeadDim;
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const uint2 w = have ? __ldg(reinterpret_cast<const uint2*>(src + key_dim<FP8>(t, s))) : make_uint2(0, 0);
+      st.q[nt][s][0] = w.x;
+      st.q[nt][s][1] = w.y;
+      if (FP8) top = __vmaxu2(__vmaxu2(top, w.x & 0x7fff7fffu), w.y & 0x7fff7fffu);
+    }
+    float f = a.scale_log2;
+    if (FP8) {
+      // the column's largest magnitude to [2^14, 2^15)
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = max(static_cast<int>(max(top & 0xffffu, top >> 16) >> 7) - 127, -112);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);   // 2^(14 - e), 14 - e in [-114, 126]
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float2 x = bf16x2_to_float2(st.q[nt][s][k]);
+          st.q[nt][s][k] = pack_half2_rn(x.x * up, x.y * up);
+        }
+      f *= __uint_as_float(static_cast<uint32_t>(127 + e - 14 > 0 ? 127 + e - 14 : 0) << 23);   // 2^(e - 14)
+    }
+    // columns 2t, 2t + 1 sit in the lanes whose g is 2t, 2t + 1
+    st.cf[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
+    st.cf[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      st.m[nt][k] = st.ms[nt][k] = -INFINITY;
+      st.l[nt][k] = 0.f;
+    }
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) st.o[nt][mt][k] = 0.f;
+  }
+}
+
+// One tile's scores (s: rows g and g + 8 of columns 2t, 2t + 1, masked ones -inf) into the running state; returns the
+// P^T fragments of the tile. ev: the V exponents of keys g and g + 8 (FP8 cache rows; 0 for drafted rows).
+template <bool FP8, int NT, bool HALF_P>
+__device__ __forceinline__ void tree_softmax(TreeState<FP8, NT>& st, float (&s)[NT][4], float ev0, float ev1,
+                                             uint32_t (&pf)[NT][2], float (&p)[NT][4]) {
+  float alpha[NT][2];
+  bool moved = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float s0 = s[nt][k], s1 = s[nt][2 + k];
+      const float w0 = FP8 ? s0 + ev0 : s0, w1 = FP8 ? s1 + ev1 : s1;
+      const float old = st.m[nt][k];
+      const float mn = fmaxf(old, max_over_rows(fmaxf(w0, w1)));
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      alpha[nt][k] = exp2f(old - ref);
+      moved |= old != mn;
+      st.m[nt][k] = mn;
+      p[nt][k] = exp2f(w0 - ref);
+      p[nt][2 + k] = exp2f(w1 - ref);
+      if (FP8) {
+        const float so = st.ms[nt][k], sn = fmaxf(so, fmaxf(s0, s1));
+        const float sref = sn == -INFINITY ? 0.f : sn;
+        st.ms[nt][k] = sn;
+        st.l[nt][k] = st.l[nt][k] * exp2f(so - sref) + exp2f(s0 - sref) + exp2f(s1 - sref);
+      } else {
+        st.l[nt][k] = st.l[nt][k] * alpha[nt][k] + p[nt][k] + p[nt][2 + k];
+      }
+    }
+  if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt) {
+        st.o[nt][mt][0] *= alpha[nt][0];
+        st.o[nt][mt][1] *= alpha[nt][1];
+        st.o[nt][mt][2] *= alpha[nt][0];
+        st.o[nt][mt][3] *= alpha[nt][1];
+      }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    pf[nt][0] = transpose8(HALF_P ? pack_half2_rn(p[nt][0], p[nt][1]) : pack_bf16x2(p[nt][0], p[nt][1]));
+    pf[nt][1] = transpose8(HALF_P ? pack_half2_rn(p[nt][2], p[nt][3]) : pack_bf16x2(p[nt][2], p[nt][3]));
+  }
+}
+
+// 16 cached e4m3 rows (the first `rows` real).
+template <int NT>
+__device__ __forceinline__ void tree_tile_e4m3(TreeState<true, NT>& st, const uint8_t* stage, int h, int lane, int rows) {
+  using SL = TreeStage<true>;
+  const int g = lane >> 2, t = lane & 3;
+  float s[NT][4];
+  {
+    const uint8_t* kr = stage + g * SL::kKStride + h * kHeadDim + t * 32;
+    uint4 w[4];
+    w[0] = *reinterpret_cast<const uint4*>(kr);
+    w[1] = *reinterpret_cast<const uint4*>(kr + 16);
+    w[2] = *reinterpret_cast<const uint4*>(kr + 8 * SL::kKStride);
+    w[3] = *reinterpret_cast<const uint4*>(kr + 8 * SL::kKStride + 16);
+    float acc[2][NT][4] = {};
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const uint32_t r0 = word4(w[x >> 2], x & 3), r1 = word4(w[2 + (x >> 2)], x & 3);
+      const uint32_t af[4] = {e4m3x2_to_half2(r0), e4m3x2_to_half2(r1), e4m3x2_to_half2(r0 >> 16),
+                              e4m3x2_to_half2(r1 >> 16)};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mma16816(acc[x & 1][nt], af, st.q[nt][x][0], st.q[nt][x][1], __half());
+    }
+    const float k0 = e8m0_to_float(stage[SL::kScales + g * kKvHeads + h]);
+    const float k1 = e8m0_to_float(stage[SL::kScales + (g + 8) * kKvHeads + h]);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        s[nt][k] = (acc[0][nt][k] + acc[1][nt][k]) * ((k < 2 ? k0 : k1) * st.cf[nt][k & 1]);
+  }
+  const uint32_t e0 = stage[SL::kScales + (kTreeRows + g) * kKvHeads + h];
+  const uint32_t e1 = stage[SL::kScales + (kTreeRows + g + 8) * kKvHeads + h];
+  const float ev0 = e0 == 255u ? NAN : static_cast<float>(e0) - 127.f;
+  const float ev1 = e1 == 255u ? NAN : static_cast<float>(e1) - 127.f;
+  uint4 v[4];   // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 16 g .. + 15
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    v[k] = *reinterpret_cast<const uint4*>(stage + SL::kV + (2 * t + (k & 1) + 8 * (k >> 1)) * SL::kVStride +
+                                           h * kHeadDim + g * 16);
+  float e[2] = {ev0, ev1};
+  if (rows < kTreeRows) {   // the rows behind the last token are stale: no score, no scale, no value
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (g + 8 * (k >> 1) >= rows) s[nt][k] = -INFINITY;
+    if (g >= rows) e[0] = 0.f;
+    if (g + 8 >= rows) e[1] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (2 * t + (k & 1) + 8 * (k >> 1) >= rows) v[k] = make_uint4(0, 0, 0, 0);
+  }
+  uint32_t pf[NT][2];
+  float p[NT][4];
+  tree_softmax<true, NT, true>(st, s, e[0], e[1], pf, p);
+#pragma unroll
+  for (int mt = 0; mt < 8; ++mt) {
+    const uint32_t sel = (mt & 1) ? 0x7362u : 0x5140u;   // the two dims' bytes of both keys: (dim 0: k, k'), (dim 1: k, k')
+    const uint32_t x = __byte_perm(word4(v[0], mt >> 1), word4(v[1], mt >> 1), sel);
+    const uint32_t y = __byte_perm(word4(v[2], mt >> 1), word4(v[3], mt >> 1), sel);
+    const uint32_t af[4] = {e4m3x2_to_half2(x), e4m3x2_to_half2(x >> 16), e4m3x2_to_half2(y), e4m3x2_to_half2(y >> 16)};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) mma16816(st.o[nt][mt], af, pf[nt][0], pf[nt][1], __half());
+  }
+}
+
+__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {   // infinities and NaN replaced by zero
+  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
+  return w;
+}
+
+// A tile of bf16 rows: 16 cached ones, or drafted ones (DRAFT: 16, or 8 in the e4m3 kernel's stages), the first `rows`
+// real; see[nt]: bit j set when the lane's token of tile nt sees row j (DRAFT).
+template <bool FP8, int NT, bool DRAFT>
+__device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uint8_t* stage, int h, int lane, int rows,
+                                               const uint32_t (&see)[NT]) {
+  using SL = TreeStage<FP8>;
+  constexpr int kKeys = FP8 ? 8 : 16;
+  constexpr int kKS = DRAFT ? SL::kDraftKStride : SL::kKStride, kVS = DRAFT ? SL::kDraftVStride : SL::kVStride;
+  static_assert(DRAFT || !FP8, "an e4m3 cache's rows have their own tile");
+  const int g = lane >> 2, t = lane & 3;
+  float s[NT][4];
+  {
+    const uint8_t* kr = stage + g * kKS + h * kHeadBytes;
+    float acc[2][NT][4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int off = 2 * key_dim<FP8>(t, 2 * i);   // eight dims: k-steps 2i and 2i + 1
+      const uint4 w0 = *reinterpret_cast<const uint4*>(kr + off);
+      const uint4 w1 = kKeys == 16 ? *reinterpret_cast<const uint4*>(kr + 8 * kKS + off) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t af[4] = {x ? w0.z : w0.x, x ? w1.z : w1.x, x ? w0.w : w0.y, x ? w1.w : w1.y};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          uint32_t b0 = st.q[nt][2 * i + x][0], b1 = st.q[nt][2 * i + x][1];
+          if (FP8) {   // the fp16 values are bf16 ones times a power of two
+            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&b0));
+            const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&b1));
+            b0 = pack_bf16x2(f0.x, f0.y);
+            b1 = pack_bf16x2(f1.x, f1.y);
+          }
+          mma16816(acc[x][nt], af, b0, b1, __nv_bfloat16());
+        }
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[nt][k] = (acc[0][nt][k] + acc[1][nt][k]) * st.cf[nt][k & 1];
+  }
+  uint4 v[4][2];   // keys 2t, 2t + 1, 2t + 8, 2t + 9: the lane's 16 dims
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int key = 2 * t + (k & 1) + 8 * (k >> 1);
+    const uint8_t* vr = stage + SL::kV + key * kVS + h * kHeadBytes;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      v[k][i] = key < kKeys ? *reinterpret_cast<const uint4*>(vr + 2 * row_dim<FP8>(g, 4 * i)) : make_uint4(0, 0, 0, 0);
+  }
+  bool odd = false;   // DRAFT: a value that must not meet a zero probability
+  if (DRAFT || rows < kTreeRows) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int key = g + 8 * (k >> 1);
+        if (key >= rows || (DRAFT && !((see[nt] >> key) & 1u))) s[nt][k] = -INFINITY;
+      }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool real = 2 * t + (k & 1) + 8 * (k >> 1) < rows;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint4& w = v[k][i];
+        if (!real) w = make_uint4(0, 0, 0, 0);
+        if (DRAFT) {
+          const uint4 f = make_uint4(finite_bf16x2(w.x), finite_bf16x2(w.y), finite_bf16x2(w.z), finite_bf16x2(w.w));
+          odd |= f.x != w.x || f.y != w.y || f.z != w.z || f.w != w.w;
+          w = f;
+        }
+      }
+    }
+  }
+  uint32_t pf[NT][2];
+  float p[NT][4];
+  tree_softmax<FP8, NT, false>(st, s, 0.f, 0.f, pf, p);
+#pragma unroll
+  for (int mt = 0; mt < 8; ++mt) {
+    const uint32_t a0 = word4(v[0][mt >> 2], mt & 3), a1 = word4(v[1][mt >> 2], mt & 3);
+    const uint32_t a2 = word4(v[2][mt >> 2], mt & 3), a3 = word4(v[3][mt >> 2], mt & 3);
+    const uint32_t af[4] = {__byte_perm(a0, a1, 0x5410), __byte_perm(a0, a1, 0x7632), __byte_perm(a2, a3, 0x5410),
+                            __byte_perm(a2, a3, 0x7632)};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) mma16816(st.o[nt][mt], af, pf[nt][0], pf[nt][1], __nv_bfloat16());
+  }
+  if (DRAFT && __any_sync(0xffffffffu, odd)) {
+    // a drafted row holds an infinity or NaN: only the tokens that see the row take it (0 * inf would reach the others)
+#pragma unroll 1
+    for (int j = 0; j < rows; ++j) {
+      const uint8_t* vr = stage + SL::kV + j * kVS + h * kHeadBytes;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int src = 4 * (j & 7) + t;
+        const float p0 = __shfl_sync(0xffffffffu, j < 8 ? p[nt][0] : p[nt][2], src);
+        const float p1 = __shfl_sync(0xffffffffu, j < 8 ? p[nt][1] : p[nt][3], src);
+        if (!((see[nt] >> j) & 1u)) continue;
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(vr + 2 * row_dim<FP8>(g, mt));
+          const float2 x = bf16x2_to_float2(w);
+          if ((w & 0x7f80u) == 0x7f80u) {
+            st.o[nt][mt][0] += p0 * x.x;
+            st.o[nt][mt][1] += p1 * x.x;
+          }
+          if ((w & 0x7f800000u) == 0x7f800000u) {
+            st.o[nt][mt][2] += p0 * x.y;
+            st.o[nt][mt][3] += p1 * x.y;
+          }
+        }
+      }
+    }
+  }
+}
+
+// End of an item's chunks in this CTA. slot < 0: the item is complete and its rows are written; else its partial goes
+// to that workspace slot: outputs [8 heads][2 TOK columns][128] fp32 and (maximum, sum) pairs.
+template <bool FP8, int NT>
+__device__ __forceinline__ void tree_finish(const TreeArgs& a, const Item& it, int h, int lane, TreeState<FP8, NT>& st,
+                                            int slot) {
+  constexpr int kCols = 8 * NT;
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int tok = it.tok0 + 4 * nt + t;
+    const bool padded = a.draft_lens != nullptr && tok >= it.drafts;
+    float r[2], mx[2], l[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (FP8) {
+        mx[k] = max_over_rows(st.ms[nt][k]);
+        const float ref = mx[k] == -INFINITY ? 0.f : mx[k];
+        l[k] = sum_over_rows(st.l[nt][k] * exp2f(st.ms[nt][k] - ref));
+        r[k] = st.m[nt][k] == -INFINITY ? 1.f : exp2f(st.m[nt][k] - ref);
+      } else {
+        mx[k] = st.m[nt][k];
+        l[k] = sum_over_rows(st.l[nt][k]);
+        r[k] = 1.f;
+      }
+      if (slot < 0) r[k] = (padded || l[k] == 0.f) ? 0.f : r[k] / l[k];
+    }
+    if (tok >= a.tokens) continue;
+    if (slot < 0) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        __nv_bfloat16* dst = a.out + static_cast<long long>(it.seat) * a.out_seat + static_cast<long long>(tok) * a.out_tok +
+                             (2 * h + k) * kHeadDim;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint4 w;
+          uint32_t* wp = &w.x;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float(&o)[4] = st.o[nt][4 * i + x];
+            // a row without keys is zero whatever the accumulators hold
+            wp[x] = r[k] == 0.f ? 0u : pack_bf16x2(o[k] * r[k], o[2 + k] * r[k]);
+          }
+          *reinterpret_cast<uint4*>(dst + row_dim<FP8>(g, 4 * i)) = w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const long long col = (static_cast<long long>(slot) * kKvHeads + h) * kCols + 8 * nt + 2 * t + k;
+        float* dst = a.ws_o + col * kHeadDim;
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt)
+          *reinterpret_cast<float2*>(dst + row_dim<FP8>(g, mt)) =
+              make_float2(st.o[nt][mt][k] * r[k], st.o[nt][mt][2 + k] * r[k]);
+        if (g == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * col) = make_float2(mx[k], l[k]);
+      }
+    }
+  }
+}
+
+struct TreePlan {
+  long long N, c0, c1;   // chunks of all items; this CTA's range
+  long long first;       // global index of the first chunk of item `w`
+  int Ge, w;             // CTAs that have chunks; the item that holds chunk c0
+};
+
+// Work split of the CTA, by all its threads. Items without chunks (nothing to attend, or padded tokens alone) get
+// their zero rows here. Returns false when the CTA has no chunk.
+template <int TOK, int DROWS>
+__device__ __forceinline__ bool tree_plan(const TreeArgs& a, TreePlan& P) {
+  constexpr int kWarps = kTreeThreads / 32;
+  __shared__ long long sums[kWarps];
+  __shared__ long long found_first;
+  __shared__ int found_item;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = gridDim.x, c = blockIdx.x, W = a.B * a.groups;
+  long long local = 0;
+  for (int w = tid; w < W; w += kTreeThreads) {
+    const Item it = tree_item<TOK, DROWS>(a, w);
+    local += it.n;
+    if (c == 0 && (a.seqlens[it.seat] < 0 || a.seqlens[it.seat] > it.len ||
+                   (a.draft_lens != nullptr && a.draft_lens[it.seat] != it.drafts)))
+      atomicOr(a.status, kStatusBadLength);
+    if (it.n == 0 && w % G == c) {
+      for (int tok = it.tok0; tok < min(it.tok0 + TOK, a.tokens); ++tok) {
+        uint4* o = reinterpret_cast<uint4*>(a.out + static_cast<long long>(it.seat) * a.out_seat +
+                                            static_cast<long long>(tok) * a.out_tok);
+        for (int k = 0; k < kQHeads * kHeadDim / 8; ++k) o[k] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) local += __shfl_xor_sync(0xffffffffu, local, o);
+  if (lane == 0) sums[warp] = local;
+  __syncthreads();
+  long long N = 0;
+#pragma unroll
+  for (int k = 0; k < kWarps; ++k) N += sums[k];
+  P.N = N;
+  P.Ge = static_cast<int>(N < G ? N : G);
+  if (c >= P.Ge) return false;
+  P.c0 = N * c / P.Ge;
+  P.c1 = N * (c + 1) / P.Ge;
+  long long base = 0;
+  for (int w0 = 0; w0 < W; w0 += kTreeThreads) {
+    const int w = w0 + tid;
+    const int n = w < W ? tree_item<TOK, DROWS>(a, w).n : 0;
+    long long incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    long long before = base, total = 0;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+      if (k < warp) before += sums[k];
+      total += sums[k];
+    }
+    incl += before;
+    if (n > 0 && incl - n <= P.c0 && P.c0 < incl) {
+      found_item = w;
+      found_first = incl - n;
+    }
+    base += total;
+    if (base > P.c0) break;   // uniform
+  }
+  __syncthreads();
+  P.w = found_item;
+  P.first = found_first;
+  return true;
+}
+
+__device__ __forceinline__ void cp_async8(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+// One arrival on `bar` (counted in its expected ones) when this thread's earlier cp.async copies have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// Pool row of token `tok` of `seat`; an entry outside the pool reads page 0 and raises its status bit.
+__device__ __forceinline__ long long tree_pool_row(const TreeArgs& a, int seat, int tok) {
+  const int pidx = tok / a.page_size;
+  int pg = a.block_table[static_cast<long long>(seat) * a.bt_stride + pidx];
+  if (pg < 0 || pg >= a.num_pages) {
+    atomicOr(a.status, kStatusBadPage);
+    pg = 0;
+  }
+  return static_cast<long long>(pg) * a.page_size + (tok - pidx * a.page_size);
+}
+
+// The producer warp: lanes 0..15 bring the chunk's K rows, lanes 16..31 its V rows, one bulk copy each; with an e4m3
+// cache also the row's eight scales. The addresses of the next chunk are looked up before the wait for a free stage.
+template <bool FP8, int TOK, int STAGES>
+__device__ __forceinline__ void tree_produce(const TreeArgs& a, const TreePlan& P, uint8_t* stages, uint64_t* full,
+                                             uint64_t* empty, volatile int* abort_flag, int lane) {
+  using SL = TreeStage<FP8>;
+  const int row = lane & 15, which = lane >> 4;
+  int w = P.w;
+  long long first = P.first;
+  Item it = tree_item<TOK, SL::kDraftRows>(a, w);
+  long long k = 0;
+  for (long long i = P.c0; i < P.c1; ++i, ++k) {
+    while (i >= first + it.n) {
+      first += it.n;
+      it = tree_item<TOK, SL::kDraftRows>(a, ++w);
+    }
+    const int j = static_cast<int>(i - first);
+    const bool draft = j >= it.nc;
+    const int r0 = draft ? (j - it.nc) * SL::kDraftRows : j * kTreeRows;
+    const int rows = draft ? min(SL::kDraftRows, it.drafts - r0) : min(kTreeRows, it.len - r0);
+    const uint8_t* src = nullptr;
+    long long prow = 0;
+    if (row < rows) {
+      if (draft) {
+        src = reinterpret_cast<const uint8_t*>((which ? a.v_new : a.k_new) + static_cast<long long>(it.seat) * a.kv_seat +
+                                               static_cast<long long>(r0 + row) * a.kv_tok);
+      } else {
+        prow = tree_pool_row(a, it.seat, r0 + row);
+        src = static_cast<const uint8_t*>(which ? a.v_pool : a.k_pool) + prow * SL::kRow;
+      }
+    }
+    const int stage = static_cast<int>(k % STAGES);
+    uint8_t* base = stages + stage * SL::kBytes;
+    if (k >= STAGES && !mbar_wait_bounded(&empty[stage], static_cast<uint32_t>((k / STAGES - 1) & 1))) {
+      atomicOr(a.status, kStatusWaitTimeout);
+      *abort_flag = 1;
+    }
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
+    fence_proxy_async_smem();
+    if (lane == 0) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(2 * rows * (draft ? kRowBytes : SL::kRow)));
+    __syncwarp();
+    if (src != nullptr) {
+      const int stride = draft ? (which ? SL::kDraftVStride : SL::kDraftKStride) : (which ? SL::kVStride : SL::kKStride);
+      bulk_g2s(base + which * SL::kV + row * stride, src, draft ? kRowBytes : SL::kRow, &full[stage]);
+      if (FP8 && !draft)
+        cp_async8(base + SL::kScales + (which * kTreeRows + row) * kKvHeads,
+                  (which ? a.v_scale : a.k_scale) + prow * kKvHeads);
+    }
+    if (FP8) cp_async_arrive(&full[stage]);
+  }
+  // the last chunks issued may still be landing when a consumer has given up: wait for them (bounded)
+  if (*abort_flag != 0)
+    for (long long j = k > STAGES ? k - STAGES : 0; j < k; ++j)
+      mbar_wait_bounded(&full[j % STAGES], static_cast<uint32_t>((j / STAGES) & 1), 100000000ull);
+}
+
+template <bool FP8, int NT, int STAGES>
+struct TreeSmem {
+  static constexpr int kBars = STAGES * TreeStage<FP8>::kBytes;
+  static constexpr int kAbort = kBars + 2 * STAGES * 8;
+  static constexpr int kBytes = kAbort + 16;
+};
+
+template <bool FP8, int NT, int STAGES, int MIN_CTAS>
+__global__ void __launch_bounds__(kTreeThreads, MIN_CTAS) paged_tree_kernel(const TreeArgs a) {
+  using SL = TreeStage<FP8>;
+  using SM = TreeSmem<FP8, NT, STAGES>;
+  constexpr int TOK = 4 * NT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::kBars);
+  uint64_t* empty = full + STAGES;
+  volatile int* abort_flag = reinterpret_cast<int*>(smem + SM::kAbort);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be scheduled; it waits for this grid
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], FP8 ? 33 : 1);
+      mbar_init(&empty[s], kTreeConsumers);
+    }
+    *abort_flag = 0;
+    a.ws_span[blockIdx.x] = make_int2(-1, 0);
+    fence_mbar_init();
+  }
+  TreePlan P;
+  if (!tree_plan<TOK, SL::kDraftRows>(a, P)) return;   // its barriers published the barrier init
+
+  if (warp == kTreeConsumers) {
+    tree_produce<FP8, TOK, STAGES>(a, P, smem, full, empty, abort_flag, lane);
+    return;
+  }
+  const int h = warp, t = lane & 3, c = static_cast<int>(blockIdx.x);
+  TreeState<FP8, NT> st;
+  int w = P.w;
+  long long first = P.first, i = P.c0, k = 0;
+  bool ok = true;
+  while (i < P.c1 && ok) {
+    Item it = tree_item<TOK, SL::kDraftRows>(a, w);
+    while (i >= first + it.n) {
+      first += it.n;
+      it = tree_item<TOK, SL::kDraftRows>(a, ++w);
+    }
+    tree_begin<FP8, NT>(a, it, h, lane, st);
+    const long long end = first + it.n < P.c1 ? first + it.n : P.c1;
+    for (; i < end; ++i, ++k) {
+      const int stage = static_cast<int>(k % STAGES);
+      if (!mbar_wait_bounded(&full[stage], static_cast<uint32_t>((k / STAGES) & 1))) {
+        atomicOr(a.status, kStatusWaitTimeout);
+        *abort_flag = 1;
+      }
+      if (__any_sync(0xffffffffu, *abort_flag != 0)) {
+        ok = false;
+        break;
+      }
+      const uint8_t* base = smem + stage * SL::kBytes;
+      const int j = static_cast<int>(i - first);
+      uint32_t see[NT] = {};
+      if (j < it.nc) {
+        const int rows = min(kTreeRows, it.len - j * kTreeRows);
+        if constexpr (FP8) tree_tile_e4m3<NT>(st, base, h, lane, rows);
+        else tree_tile_bf16<false, NT, false>(st, base, h, lane, rows, see);
+      } else {
+        const int r0 = (j - it.nc) * SL::kDraftRows;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int tok = it.tok0 + 4 * nt + t;
+          if (tok < it.drafts)
+            see[nt] = static_cast<uint32_t>(
+                static_cast<unsigned long long>(a.mask[static_cast<long long>(it.seat) * a.mask_seat + tok]) >> r0);
+        }
+        tree_tile_bf16<FP8, NT, true>(st, base, h, lane, min(SL::kDraftRows, it.drafts - r0), see);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+    }
+    if (!ok) break;
+    // slot 2c + 1 holds the item that starts here and goes on, 2c the one that came in from the CTA before
+    const bool from_before = first < P.c0, goes_on = first + it.n > P.c1;
+    tree_finish<FP8, NT>(a, it, h, lane, st, from_before ? 2 * c : (goes_on ? 2 * c + 1 : -1));
+    if (!from_before && goes_on && h == 0 && lane == 0) {
+      // the last CTA of the item: the one that holds chunk e = its last; c(e) = the largest with N * c / Ge <= e
+      const long long e = first + it.n - 1;
+      a.ws_span[c] = make_int2(w, static_cast<int>(((e + 1) * P.Ge + P.N - 1) / P.N - 1));
+    }
+  }
+  if (!ok && lane == 0)
+    for (int s = 0; s < STAGES; ++s)
+      mbar_wait_bounded(&full[(k + s) % STAGES], static_cast<uint32_t>(((k + s) / STAGES) & 1), 100000000ull);
+}
+
+// Adds the partials of the item that starts in CTA c and goes on (if there is one) for KV head h: CTA (c, h).
+// cols = 2 heads x TOK tokens; each column's 128 dims in a warp, and with fewer columns than warps the partials of a
+// column are shared out over several warps.
+constexpr int kMergeWarps = 8;
+
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_tree_merge_kernel(const TreeArgs a, int tok_per_group) {
+  __shared__ float4 part[kMergeWarps][32];
+  __shared__ float part_l[kMergeWarps];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int2 span = __ldcg(&a.ws_span[c]);
+  if (span.x < 0) return;
+  const int seat = span.x / a.groups, tok0 = (span.x - seat * a.groups) * tok_per_group;
+  const int cols = 2 * tok_per_group, parts = span.y - c + 1;
+  const int live = 2 * min(tok_per_group, a.tokens - tok0);
+  int drafts = a.tokens;
+  if (a.draft_lens != nullptr) drafts = a.draft_lens[seat];
+  int share = 1;                                     // warps per column: the largest power of two that leaves none over
+  while (share * 2 * live <= kMergeWarps) share *= 2;
+  const int per = kMergeWarps / share;               // columns at a time
+  for (int col0 = 0; col0 < live; col0 += per) {     // uniform
+    const int col = col0 + warp % per, sub = warp / per;
+    const bool mine = col < live;
+    // partial x of the column: slot 2c + 1 for x = 0, then slot 2(c + x)
+    auto at = [&](int x) {
+      return (static_cast<long long>(x == 0 ? 2 * c + 1 : 2 * (c + x)) * kKvHeads + h) * cols + col;
+    };
+    float M = -INFINITY;
+    if (mine)
+      for (int x = lane; x < parts; x += 32) M = fmaxf(M, __ldcg(a.ws_ml + 2 * at(x)));
+    M = warp_max(M);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float4 o = make_float4(0, 0, 0, 0);
+    float l = 0.f;
+    if (mine) {
+#pragma unroll 4
+      for (int x = sub; x < parts; x += share) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + 2 * at(x)));
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(a.ws_o + at(x) * kHeadDim) + lane);
+        const float f = exp2f(ml.x - ref);
+        l += ml.y * f;
+        o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+      }
+    }
+    if (share > 1) {
+      part[warp][lane] = o;
+      if (lane == 0) part_l[warp] = l;
+      __syncthreads();
+      if (sub == 0) {
+        for (int x = 1; x < share; ++x) {
+          const float4 v = part[warp + x * per][lane];
+          o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+          l += part_l[warp + x * per];
+        }
+      }
+      __syncthreads();
+    }
+    if (mine && sub == 0) {
+      const int tok = tok0 + (col >> 1);
+      const bool none = l == 0.f || tok >= drafts;
+      const float r = 1.f / l;
+      __nv_bfloat16* dst = a.out + static_cast<long long>(seat) * a.out_seat + static_cast<long long>(tok) * a.out_tok +
+                           (2 * h + (col & 1)) * kHeadDim;
+      *(reinterpret_cast<uint2*>(dst) + lane) =
+          none ? make_uint2(0, 0) : float4_to_bf16x4(make_float4(o.x * r, o.y * r, o.z * r, o.w * r));
+    }
+  }
+}
+
+struct TreeConfig {
+  int tok, ctas_per_sm;
+};
+
+// Tokens per group: 4 (one 8-column tile) or 8 (two). Longer drafts run as groups of 8 that each read the cache.
+TreeConfig tree_config(bool fp8, int tokens) {
+  const int tok = tokens <= 4 ? 4 : 8;
+  return {tok, fp8 && tok == 4 ? 2 : 1};
+}
+
+long long tree_grid(bool fp8, int batch, int tokens, int num_sms) {
+  (void)batch;
+  return static_cast<long long>(num_sms) * tree_config(fp8, tokens).ctas_per_sm;
+}
+
+template <bool FP8, int NT, int STAGES, int MIN_CTAS>
+cudaError_t launch_tree_main(const TreeArgs& a, int grid, cudaStream_t stream) {
+  using SM = TreeSmem<FP8, NT, STAGES>;
+  auto kern = paged_tree_kernel<FP8, NT, STAGES, MIN_CTAS>;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (configured_device != dev) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kBytes);
+    if (e != cudaSuccess) return e;
+    configured_device = dev;
+  }
+  kern<<<grid, kTreeThreads, SM::kBytes, stream>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+TreeWorkspace tree_workspace(bool fp8, int batch, int tokens, int num_sms) {
+  TreeWorkspace w;
+  const TreeConfig cfg = tree_config(fp8, tokens);
+  w.grid = static_cast<int>(tree_grid(fp8, batch, tokens, num_sms));
+  const size_t cols = 2ull * w.grid * kKvHeads * 2 * cfg.tok;   // two slots per CTA
+  w.span = 0;
+  w.ml = (static_cast<size_t>(w.grid) * sizeof(int2) + 255) / 256 * 256;
+  w.o = w.ml + cols * 2 * sizeof(float);
+  w.bytes = w.o + cols * kHeadDim * sizeof(float);
+  w.groups = (tokens + cfg.tok - 1) / cfg.tok;
+  return w;
+}
+
+cudaError_t launch_paged_tree(const TreeArgs& a, const TreeWorkspace& w, cudaStream_t stream) {
+  const bool fp8 = a.k_scale != nullptr;
+  const TreeConfig cfg = tree_config(fp8, a.tokens);
+  cudaError_t e;
+  if (fp8) e = cfg.tok == 4 ? launch_tree_main<true, 1, 3, 2>(a, w.grid, stream) : launch_tree_main<true, 2, 6, 1>(a, w.grid, stream);
+  else e = cfg.tok == 4 ? launch_tree_main<false, 1, 3, 1>(a, w.grid, stream) : launch_tree_main<false, 2, 3, 1>(a, w.grid, stream);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(w.grid, kKvHeads);
+  lc.blockDim = dim3(kMergeWarps * 32);
+  lc.stream = stream;
+  lc.attrs = &at;
+  lc.numAttrs = 1;
+  return cudaLaunchKernelEx(&lc, paged_tree_merge_kernel, a, cfg.tok);
+}
+
+}  // namespace q3

@@ -59,6 +59,11 @@ __device__ __forceinline__ float round_bf16(float x) {
   return __bfloat162float(__float2bfloat16_rn(x));
 }
 
+// The value of an E8M0 scale byte: 2^(s - 127), NaN for 255.
+__device__ __forceinline__ float e8m0_to_float(uint32_t s) {
+  return __uint_as_float((s << 23) | (s == 0u || s == 255u ? 0x400000u : 0u));
+}
+
 // ---------------------------------------------------------------- q/k RMSNorm + rotate-half RoPE of one head
 // One head of 128 dims held 4 dims per lane (lane l: dims 4l..4l+3), x = the raw head as floats (bf16 values).
 // Arithmetic and rounding points of engine/ops.py:51-60 run in bf16:

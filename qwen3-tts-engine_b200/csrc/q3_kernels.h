@@ -73,6 +73,67 @@ struct AppendArgs {
 
 cudaError_t launch_kv_append(const AppendArgs& a, int num_sms, cudaStream_t stream);
 
+// Rows of the 8-bit cache: e4m3 [pool_rows, 8, 128] and one E8M0 byte per (row, head).
+struct KvQuantArgs {
+  const __nv_bfloat16* k_rows;     // append: [n_rows, 8, 128] with row stride rows_stride (elements)
+  const __nv_bfloat16* v_rows;
+  long long rows_stride;
+  uint8_t* k_pool;
+  uint8_t* v_pool;
+  uint8_t* k_scale;                // [pool_rows, 8]
+  uint8_t* v_scale;
+  long long pool_rows;             // num_pages * page_size
+  int page_size;
+  int n_rows;
+  const int64_t* slots;            // flat pool row per row, or nullptr
+  const int32_t* positions;        // token position per row (paged mode)
+  const int32_t* seat_of_row;      // seat per row (paged mode; nullptr = row i belongs to seat i)
+  const int32_t* block_table;
+  long long bt_stride;
+  int num_seats;                   // rows of block_table
+  int max_pages;
+  uint32_t* status;
+};
+cudaError_t launch_kv_quant_append(const KvQuantArgs& a, int num_sms, cudaStream_t stream);
+cudaError_t launch_kv_dequant(const KvQuantArgs& a, __nv_bfloat16* k_out, __nv_bfloat16* v_out, long long out_stride,
+                              int num_sms, cudaStream_t stream);
+
+// Attention of up to 64 drafted tokens per seat over the paged cache and each other (paged_tree.cu); decode attention
+// over the 8-bit cache with tokens = 1 and no draft rows.
+constexpr int kTreeMaxTokens = 64;    // a visibility word has 64 bits
+struct TreeArgs {
+  const __nv_bfloat16* q;          // [B, tokens, 16, 128], seat and token strides in elements
+  long long q_seat, q_tok;
+  const __nv_bfloat16* k_new;      // [B, tokens, 8, 128] drafted rows, or nullptr (none)
+  const __nv_bfloat16* v_new;
+  long long kv_seat, kv_tok;
+  const int64_t* mask;             // visibility words [B, tokens] (mask_seat 0: one row for all seats)
+  long long mask_seat;
+  const int32_t* draft_lens;       // [B] drafted tokens of each seat, or nullptr (tokens each)
+  const void* k_pool;              // [num_pages, page_size, 8, 128] bf16 or e4m3
+  const void* v_pool;
+  const uint8_t* k_scale;          // [num_pages, page_size, 8] E8M0 (e4m3), or nullptr (bf16)
+  const uint8_t* v_scale;
+  const int32_t* seqlens;          // [B] cached tokens
+  const int32_t* block_table;
+  long long bt_stride;
+  int max_pages, num_pages, page_size;
+  int B, tokens, groups;           // groups of tokens per seat (set from the workspace layout)
+  float scale_log2;
+  __nv_bfloat16* out;              // [B, tokens, 16, 128]
+  long long out_seat, out_tok;
+  int2* ws_span;                   // [grid] (item that starts in the CTA and goes on, its last CTA), item -1: none
+  float* ws_ml;                    // [2 grid slots][8 heads][2 tok columns] (maximum, sum)
+  float* ws_o;                     // the same columns' [128] fp32 outputs
+  uint32_t* status;
+};
+struct TreeWorkspace {
+  int grid, groups;
+  size_t span, ml, o, bytes;       // byte offsets, total
+};
+TreeWorkspace tree_workspace(bool fp8, int batch, int tokens, int num_sms);
+cudaError_t launch_paged_tree(const TreeArgs& a, const TreeWorkspace& w, cudaStream_t stream);
+
 struct PrefixCopyArgs {
   const __nv_bfloat16* k_src;      // row (l, slot, r) at l * src_layer_stride + slot * src_slot_stride + r * row_elems
   const __nv_bfloat16* v_src;

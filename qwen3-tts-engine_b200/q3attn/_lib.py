@@ -31,6 +31,26 @@ class Sampler(ctypes.Structure):
                 ("seed", ctypes.c_uint64), ("rng_state", _P), ("out_ids", _P), ("out_stride", _I64), ("emb", _P),
                 ("emb_row_stride", _I64), ("emb_dim", _I32), ("emb_out", _P), ("emb_out_row_stride", _I64)]
 
+
+class QuantCache(ctypes.Structure):
+    """struct q3_quant_cache (include/q3attn.h): an e4m3 paged cache with E8M0 scales."""
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("num_pages", _I32), ("page_size", _I32)]
+
+
+_QC = ctypes.POINTER(QuantCache)
+
+
+class TreeAttn(ctypes.Structure):
+    """struct q3_tree_attn (include/q3attn.h): attention of drafted tokens over a paged cache."""
+    _fields_ = [("q", _P), ("q_seat_stride", _I64), ("q_token_stride", _I64), ("k_new", _P), ("v_new", _P),
+                ("kv_new_seat_stride", _I64), ("kv_new_token_stride", _I64), ("tree_mask", _P),
+                ("tree_mask_stride", _I64), ("draft_lens", _P), ("k_pool", _P), ("v_pool", _P), ("k_scale", _P),
+                ("v_scale", _P), ("num_pages", _I32), ("page_size", _I32), ("cache_seqlens", _P), ("block_table", _P),
+                ("block_table_stride", _I64), ("max_pages_per_seat", _I32), ("batch", _I32), ("tokens", _I32),
+                ("num_heads", _I32), ("num_kv_heads", _I32), ("head_dim", _I32), ("softmax_scale", _F32), ("out", _P),
+                ("out_seat_stride", _I64), ("out_token_stride", _I64)]
+
+
 # name -> (restype, argtypes); every symbol include/q3attn.h declares
 SIGNATURES = {
     "q3_version": (ctypes.c_int, []),
@@ -68,6 +88,11 @@ SIGNATURES = {
                                            _I32, _I32, _I32, _F32, _I32, _P, _I64, _I64, _P]),
     "q3_kv_copy_prefix": (ctypes.c_int, [_P, _P, _I64, _I64, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _I32, _I32,
                                          _P, _I64, _I32, _P]),
+    "q3_kv_quant_append_slots": (ctypes.c_int, [_P, _P, _I64, _QC, _I32, _I32, _P, _I32, _P]),
+    "q3_kv_quant_append_paged": (ctypes.c_int, [_P, _P, _I64, _QC, _I32, _I32, _P, _P, _P, _I64, _I32, _I32, _I32, _P]),
+    "q3_kv_dequant_paged": (ctypes.c_int, [_QC, _I32, _I32, _P, _P, _P, _I64, _I32, _I32, _P, _P, _I64, _I32, _P]),
+    "q3_paged_tree_workspace_bytes": (_SZ, [_I32, _I32, _I32]),
+    "q3_paged_tree_attn": (ctypes.c_int, [ctypes.POINTER(TreeAttn), _P, _SZ, _P]),
     "q3_cp_step_qkv": (ctypes.c_int, [_P, _I64, _NR, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _I32,
                                       _I32, _F32, _P, _I64, _P]),
 }
