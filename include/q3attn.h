@@ -366,6 +366,31 @@ typedef struct q3_tree_attn {
 size_t q3_paged_tree_workspace_bytes(int32_t batch, int32_t tokens, int32_t quantised);
 int q3_paged_tree_attn(const q3_tree_attn* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Log probabilities of given tokens, with the entropy of each row and its top alternatives: the scores that accept or
+ * reject drafted tokens. For row r, p = softmax(logits[r] / temperature):
+ *   logprobs[r, i] = ln p(ids[r, i])  (-inf for an id outside 0 .. vocab - 1)
+ *   entropy[r]     = -sum p ln p
+ *   top_ids[r, :], top_logprobs[r, :]: the top_n tokens by (logit descending, id ascending), NaN above everything.
+ * Logits of -inf have probability 0. A row with NaN or +inf, or of -inf alone, has NaN for its numbers. The statistics
+ * are fp32. One launch, no workspace; top_n <= min(64, vocab); outputs are contiguous. No reference counterpart. */
+typedef struct q3_logprobs {
+  const void* logits;          /* [rows, vocab] rows, row_stride elements apart */
+  int32_t logits_dtype;        /* 0 = bf16, 1 = fp32, 2 = fp16 */
+  int64_t row_stride;
+  int64_t rows;                /* <= 2^27 */
+  int32_t vocab;               /* <= 2^30 */
+  float temperature;           /* > 0 */
+  const int64_t* ids;          /* [rows, given], rows ids_row_stride apart */
+  int64_t ids_row_stride;
+  int32_t given;
+  float* logprobs;             /* [rows, given] */
+  float* entropy;              /* optional [rows] */
+  int32_t top_n;
+  int64_t* top_ids;            /* [rows, top_n] (top_n > 0) */
+  float* top_logprobs;
+} q3_logprobs;
+int q3_token_logprobs(const q3_logprobs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -84,10 +84,11 @@ def tree_attention(q, k, v, mask, k_pool, v_pool, seqlens, table, scale, draft_l
 
 
 def logprobs(logits, ids, top_n, temperature=1.0):
-    """(log probabilities of ids [N] or [N, M], entropy [N], top ids [N, n], their log probabilities)."""
+    """(log probabilities of ids [N] or [N, M], entropy [N], top ids [N, n], their log probabilities). The maximum is
+    taken off first (64 bits too lose digits of the sum next to a logit of 1e38), so a row with +inf is NaN."""
     x = logits.double()
-    z = x / temperature
-    lp = z - torch.logsumexp(z, -1, keepdim=True)
+    z = (x - x.amax(-1, keepdim=True)) / temperature
+    lp = z - torch.log(torch.exp(z).sum(-1, keepdim=True))
     ent = -torch.where(lp > -math.inf, lp.exp() * lp, torch.where(torch.isnan(lp), lp, 0.0)).sum(-1)
     order = torch.sort(x, dim=-1, descending=True, stable=True)[1][:, :top_n]
     return torch.gather(lp, 1, ids.view(len(x), -1)).view(ids.shape), ent, order, torch.gather(lp, 1, order)

@@ -906,4 +906,37 @@ int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_
   return record(q3::launch_paged_tree(a, w, static_cast<cudaStream_t>(stream)));
 }
 
+int q3_token_logprobs(const q3_logprobs* p, void* stream) {
+  if (!p || p->rows < 0 || p->rows > (1ll << 27)) return Q3_ERR_INVALID;
+  if (p->vocab < 1 || p->vocab > (1 << 30) || p->given < 0 || p->top_n < 0 || p->top_n > p->vocab ||
+      !(p->temperature > 0.f) || p->logits_dtype < 0 || p->logits_dtype > 2)
+    return Q3_ERR_INVALID;
+  if (p->top_n > q3::kLogprobMaxTop) return Q3_ERR_UNSUPPORTED;
+  if (p->rows == 0) return Q3_OK;
+  if (!p->logits || p->row_stride < p->vocab || (p->given > 0 && (!p->ids || !p->logprobs || p->ids_row_stride < p->given)) ||
+      (p->top_n > 0 && (!p->top_ids || !p->top_logprobs)))
+    return Q3_ERR_INVALID;
+  if (!aligned(p->logits, p->logits_dtype == 1 ? 4 : 2) || !aligned(p->ids, 8) || !aligned(p->logprobs, 4) ||
+      !aligned(p->entropy, 4) || !aligned(p->top_ids, 8) || !aligned(p->top_logprobs, 4))
+    return Q3_ERR_ALIGNMENT;
+  int dev = 0, rc = current_device(&dev);
+  if (rc != Q3_OK) return rc;
+  q3::LogprobArgs a{};
+  a.logits = p->logits;
+  a.dtype = p->logits_dtype;
+  a.row_stride = p->row_stride;
+  a.rows = p->rows;
+  a.vocab = p->vocab;
+  a.ids = p->ids;
+  a.ids_stride = p->ids_row_stride;
+  a.given = p->given;
+  a.inv_temp = 1.f / p->temperature;
+  a.logprobs = p->logprobs;
+  a.entropy = p->entropy;
+  a.top_n = p->top_n;
+  a.top_ids = p->top_ids;
+  a.top_logprobs = p->top_logprobs;
+  return record(q3::launch_logprobs(a, sm_count(dev), static_cast<cudaStream_t>(stream)));
+}
+
 }  // extern "C"

@@ -209,6 +209,25 @@ struct SampleArgs {
 
 cudaError_t launch_sample_topk(const SampleArgs& a, cudaStream_t stream);
 
+constexpr int kLogprobMaxTop = 64;
+struct LogprobArgs {
+  const void* logits;              // [rows, vocab], row stride row_stride (elements)
+  int dtype;                       // 0 bf16, 1 fp32, 2 fp16
+  long long row_stride;
+  long long rows;
+  int vocab;
+  const int64_t* ids;              // [rows, given] tokens, rows ids_stride apart
+  long long ids_stride;
+  int given;
+  float inv_temp;
+  float* logprobs;                 // [rows, given]
+  float* entropy;                  // [rows], optional
+  int top_n;                       // 0 .. min(64, vocab)
+  int64_t* top_ids;                // [rows, top_n]
+  float* top_logprobs;
+};
+cudaError_t launch_logprobs(const LogprobArgs& a, int num_sms, cudaStream_t stream);
+
 struct RowNormArgs {
   __nv_bfloat16* x;                // [rows, H] residual stream (updated in place when r is given)
   long long x_stride;

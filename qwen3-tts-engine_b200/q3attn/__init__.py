@@ -13,7 +13,7 @@ from .ops import (SamplerRng, add_rms_norm, cp_step_qkv, kv_append_paged, kv_app
                   paged_decode, paged_decode_append, paged_decode_qkv, prefill, prefill_paged, qk_norm_rope_,
                   ring_window_attn, sample_topk, set_decode_variant, set_prefill_kernel, set_ring_chunk_kernel,
                   set_ring_frame_kernel, silu_mul)
-from .spec import (empty_quant_cache, kv_dequant_paged, kv_quant_append_paged, kv_quant_append_slots,  # noqa: F401
-                   paged_decode_quant, paged_tree_attn, tree_mask)
+from .spec import (TokenLogprobs, empty_quant_cache, kv_dequant_paged, kv_quant_append_paged,  # noqa: F401
+                   kv_quant_append_slots, paged_decode_quant, paged_tree_attn, token_logprobs, tree_mask)
 
 __version__ = "0.1.0"

@@ -51,6 +51,14 @@ class TreeAttn(ctypes.Structure):
                 ("out_seat_stride", _I64), ("out_token_stride", _I64)]
 
 
+
+class Logprobs(ctypes.Structure):
+    """struct q3_logprobs (include/q3attn.h): log probabilities, entropy and top alternatives of rows of logits."""
+    _fields_ = [("logits", _P), ("logits_dtype", _I32), ("row_stride", _I64), ("rows", _I64), ("vocab", _I32),
+                ("temperature", _F32), ("ids", _P), ("ids_row_stride", _I64), ("given", _I32), ("logprobs", _P),
+                ("entropy", _P), ("top_n", _I32), ("top_ids", _P), ("top_logprobs", _P)]
+
+
 # name -> (restype, argtypes); every symbol include/q3attn.h declares
 SIGNATURES = {
     "q3_version": (ctypes.c_int, []),
@@ -93,6 +101,7 @@ SIGNATURES = {
     "q3_kv_dequant_paged": (ctypes.c_int, [_QC, _I32, _I32, _P, _P, _P, _I64, _I32, _I32, _P, _P, _I64, _I32, _P]),
     "q3_paged_tree_workspace_bytes": (_SZ, [_I32, _I32, _I32]),
     "q3_paged_tree_attn": (ctypes.c_int, [ctypes.POINTER(TreeAttn), _P, _SZ, _P]),
+    "q3_token_logprobs": (ctypes.c_int, [ctypes.POINTER(Logprobs), _P]),
     "q3_cp_step_qkv": (ctypes.c_int, [_P, _I64, _NR, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _I32,
                                       _I32, _F32, _P, _I64, _P]),
 }

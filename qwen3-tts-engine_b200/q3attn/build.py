@@ -3,8 +3,9 @@
     python -m q3attn.build            (from qwen3-tts-engine_b200/)   or   q3attn.build.build()
 
 Every .cu under qwen3-tts-engine_b200/csrc is compiled separately (in parallel) and linked into
-qwen3-tts-engine_b200/q3attn/libq3attn.so next to this file, where q3attn._lib loads it. Objects go to
-qwen3-tts-engine_b200/_build/. The library is rebuilt unless the SHA-256 of every source, header and this script (and
+qwen3-tts-engine_b200/q3attn/libq3attn.so next to this file, where q3attn._lib loads it; csrc/torch_ops.cpp (PyTorch
+bindings written in C++) becomes libq3torch.so beside it, linked against libq3attn.so and torch's own libraries. Objects go
+to qwen3-tts-engine_b200/_build/. The library is rebuilt unless the SHA-256 of every source, header and this script (and
 the nvcc flags) equals the digest stamped beside it when it was last built, so a copied tree never runs a library that
 was built from other sources, whatever the files' modification times say.
 """
@@ -23,6 +24,8 @@ CSRC = os.path.join(ROOT, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 BUILD_DIR = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG_DIR, "libq3attn.so")
+TORCH_LIB = os.path.join(PKG_DIR, "libq3torch.so")
+TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
 STAMP = LIB + ".sha256"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -41,7 +44,7 @@ def sources():
 
 
 def _deps():
-    return sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) + \
+    return sources() + [TORCH_SRC] + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) + \
         glob.glob(os.path.join(INCLUDE, "*.h")) + [os.path.abspath(__file__)]
 
 
@@ -56,10 +59,24 @@ def source_digest() -> str:
 
 
 def up_to_date() -> bool:
-    if not (os.path.exists(LIB) and os.path.exists(STAMP)):
+    if not (os.path.exists(LIB) and os.path.exists(TORCH_LIB) and os.path.exists(STAMP)):
         return False
     with open(STAMP) as f:
         return f.read().strip() == source_digest()
+
+
+def torch_flags():
+    """Compile and link flags of the PyTorch bindings, from the torch that imports here."""
+    import torch
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), INCLUDE]
+    compile_ = ["-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + \
+        [f for i in inc for f in ("-isystem" if i != INCLUDE else "-I", i)]
+    link = ["-L" + os.path.join(root, "lib"), "-ltorch_cpu", "-lc10", "-lc10_cuda", "-L" + PKG_DIR, "-lq3attn",
+            "-Wl,-rpath,$ORIGIN", "-Wl,--no-as-needed"]
+    return compile_, link
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
@@ -77,8 +94,18 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
             raise RuntimeError(f"nvcc failed on {os.path.basename(src)}:\n{r.stderr}")
         return obj, r.stderr
 
+    cflags, lflags = torch_flags()
+    torch_obj = os.path.join(BUILD_DIR, "torch_ops.o")
+
+    def compile_torch():
+        r = subprocess.run(["g++", "-c", TORCH_SRC, "-o", torch_obj] + cflags, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed on torch_ops.cpp:\n{r.stderr}")
+
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        bindings = ex.submit(compile_torch)
         results = list(ex.map(compile_one, sources()))
+        bindings.result()
     if verbose or ptxas_info:
         for _, err in results:
             if err.strip():
@@ -89,6 +116,11 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
+    tmp = TORCH_LIB + ".tmp"
+    r = subprocess.run(["g++", "-shared", "-o", tmp, torch_obj] + lflags, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"linking the PyTorch bindings failed:\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
     with open(STAMP, "w") as f:
         f.write(source_digest() + "\n")
     return LIB

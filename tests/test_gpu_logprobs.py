@@ -1,0 +1,141 @@
+"""GPU parity: log probabilities of given tokens, entropy and top alternatives, against the 64-bit oracle. Top ids are
+compared exactly (value descending, id ascending).
+
+Tolerance, derived: a thread adds up to K = V / 256 + 16 fp32 terms (each sum off by 2^-24 of itself), the exponential
+and z = (x - m) log2(e) / T are off by a few 2^-24 each: ln s by (K + 40) 2^-24 at most; (x - m) / T by 2^-22 of itself.
+The entropy's second term t / s has the same relative error, and is at most ln V + H.
+"""
+import math
+
+import pytest
+import torch
+
+from helpers import poison_allocator
+from oracle import spec as OSP
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def q3():
+    import q3attn
+    q3attn._lib.load()
+    return q3attn
+
+
+def logits(n, v, seed, dtype, scale=3.0):
+    return (torch.randn(n, v, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype)
+
+
+def check(q3, x, ids, top, T=1.0, dev_x=None):
+    n, v = x.shape
+    for _ in range(2):
+        poison_allocator((n, max(top, 1)), torch.float32)
+    got = q3.token_logprobs(x.to(DEV) if dev_x is None else dev_x, ids.to(DEV), top, T)
+    lp, ent, best, best_lp = [t.cpu() for t in got]
+    rlp, rent, rbest, rbest_lp = OSP.logprobs(x, ids.clamp(0, v - 1), top, T)
+    outside = (ids < 0) | (ids >= v)
+    rlp = rlp.masked_fill(outside, -math.inf)
+    assert torch.equal(best, rbest)
+    base = (v / 256 + 56) * 2.0 ** -24
+    for g, r, tol in ((lp, rlp, base + rlp.abs() * 2.0 ** -22), (best_lp, rbest_lp, base + rbest_lp.abs() * 2.0 ** -22),
+                      (ent, rent, base * (2 + math.log(v) + rent.abs()))):
+        assert g.shape == r.shape and g.dtype == torch.float32
+        # the outputs are fp32: (x - m) / T = -3.39e38 / 0.5 = -6.8e38 lies below its range (3.40e38) and is -inf
+        fin = torch.isfinite(r.float())
+        assert torch.equal(torch.isnan(g), torch.isnan(r)) and torch.equal(g[~fin & ~torch.isnan(r)], r[~fin & ~torch.isnan(r)].float())
+        d = (g.double() - r).abs()[fin]
+        assert (d <= tol[fin]).all(), float((d / tol[fin]).max())
+
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,top", [(1, 1, 1), (3, 2, 2), (5, 63, 20), (16, 2048, 5), (4, 4099, 64), (2, 8191, 0),
+                                     (1, 150001, 20), (7, 40000, 64), (2400, 700, 3)])
+def test_rows(q3, dtype, n, v, top):
+    x = logits(n, v, n + v, dtype)
+    ids = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3))
+    check(q3, x, ids, top)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [0.3, 0.9, 4.0])
+def test_temperature_and_several_ids(q3, dtype, T):
+    x = logits(9, 5003, 4, dtype)
+    ids = torch.randint(0, 5003, (9, 300), generator=torch.Generator().manual_seed(5))
+    ids[2, 7], ids[3, 0], ids[8, 299] = -1, 5003, 1 << 40
+    check(q3, x, ids, 11, T)
+    check(q3, x, ids[:, :0], 11, T)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_special_rows(q3, dtype):
+    v = 20000
+    x = logits(16, v, 6, dtype)
+    low = torch.finfo(dtype).min
+    x[0] = -math.inf
+    x[1, 1:] = -math.inf
+    x[2] = low
+    x[3, ::2] = low
+    x[4, 700] = math.nan
+    x[5, 19999] = math.inf
+    x[6] = 0
+    x[6, 3::7] = -0.0
+    x[7] = torch.arange(v).to(dtype) / 1024                       # rising
+    x[8] = -torch.arange(v).to(dtype) / 1024                      # falling
+    x[9] = torch.finfo(dtype).max
+    x[10, 5000:] = -math.inf
+    x[11] = (torch.arange(v) % 8).to(dtype)                       # massive ties
+    x[12, 17] = 60.0                                              # nearly certain
+    x[13] = low
+    x[13, 5] = 1.0
+    x[14, :] = math.nan
+    x[15] *= 100
+    check(q3, x, torch.arange(16) * 1250, 64)
+    check(q3, x, torch.arange(16), 1, 0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("start", [0, 1, 3, 7])
+def test_strided_rows_and_odd_starts(q3, dtype, start):
+    wide = logits(6, 3011, 8, dtype)
+    x = wide[:, start:start + 2999]
+    d = wide.to(DEV)[:, start:start + 2999]
+    check(q3, x, torch.arange(6) * 400, 30, dev_x=d)
+    check(q3, x[:1], torch.arange(1), 30, dev_x=d[:1])
+    t = wide.t().contiguous().to(DEV).t()[:, start:start + 2999]          # columns first: copied
+    check(q3, x, torch.arange(6), 2, dev_x=t)
+
+
+@pytest.mark.parametrize("n", [1, 2, 70])
+def test_values_in_one_place(q3, n):
+    """All of the top alternatives side by side, at the row's end, and in one thread's vectors."""
+    v = 100000
+    for at in (slice(0, 64), slice(v - 64, v), slice(5000, 5016)):
+        x = logits(n, v, 9, torch.float32, 0.1)
+        x[:, at] += 50 + torch.arange(at.stop - at.start) * 0.5
+        check(q3, x, torch.full((n,), at.start), 40)
+
+
+def test_graph_replay(q3):
+    x = logits(12, 30000, 10, torch.bfloat16).to(DEV)
+    ids = torch.arange(12, device=DEV)
+    q3.token_logprobs(x, ids, 5)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = q3.token_logprobs(x, ids, 5)
+    y = logits(12, 30000, 11, torch.bfloat16)
+    x.copy_(y)
+    g.replay()
+    want = q3.token_logprobs(y.to(DEV), ids, 5)
+    for a, b in zip(out, want):
+        assert torch.equal(a, b)
+
+
+def test_no_rows(q3):
+    got = q3.token_logprobs(torch.empty(0, 100, device=DEV), torch.empty(0, dtype=torch.int64, device=DEV), 3)
+    assert got.logprobs.shape == (0,) and got.top_ids.shape == (0, 3)
