@@ -10,12 +10,14 @@
 // preserving bits above the complement of the id, all different.
 //
 // Bound: HBM (the logits are read once). A row is shared by a cluster of 1 to 8 CTAs when there are few rows; every
-// CTA streams its part in tiles of 512 16-byte vectors, the next tile's loads in flight while one is worked on.
-// Selection rides on the same pass: a thread compares the largest of its tile values with the n-th best key found so
-// far, and one counting barrier per tile says how many threads have candidates (none, for most tiles). Candidates go
-// to a shared-memory list, which is cut back to n when it grows. When nearly all threads have some (the first tile, a
-// rising row) the n-th largest of 128 group maxima is a bound first: at most n groups reach it, so a tile never adds
-// more than n * 2 threads * 16 values.
+// CTA streams its part in tiles of 512 16-byte vectors, the next tile's loads in flight while one is worked on; the
+// arithmetic is packed in pairs, one exponential per logit.
+// Selection needs no pass of its own. m is a thread's largest value; the n-th largest maximum of 128 groups of two
+// threads bounds the top n from below, and only the few threads that reach it (n to 2n of 256) have their vectors
+// read again, out of the L2 cache, shared out over all threads. Rows where more than the list holds reach the bound
+// (massive ties, fewer than n logits above -inf, values in one thread's vectors) take select_tiles, which is bounded for
+// every row: it goes through the tiles with the n-th best key so far, and where nearly all threads have candidates the
+// n-th largest group maximum of the tile is a bound first, so that a tile adds n * 2 threads * 16 values at most.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -59,34 +61,56 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ float exp2_fast(float x) {   // 2 ulp; results below 2^-126 are zero
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <typename T>
-struct Vec;   // one 16-byte vector of logits
+struct Vec;   // one 16-byte vector of logits: kN values; pairs of them as floats; their largest (NaN if there is one)
 template <>
 struct Vec<float> {
   static constexpr int kN = 4;
-  static __device__ __forceinline__ float at(const uint4& w, int i) {
-    return __uint_as_float(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w);
+  static __device__ __forceinline__ float2 pair(const uint4& w, int i) {
+    return i == 0 ? make_float2(__uint_as_float(w.x), __uint_as_float(w.y))
+                  : make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
+  }
+  static __device__ __forceinline__ float top(const uint4& w) {
+    return max_nan(max_nan(__uint_as_float(w.x), __uint_as_float(w.y)), max_nan(__uint_as_float(w.z), __uint_as_float(w.w)));
   }
 };
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int kN = 8;
   static constexpr uint32_t kNegInf = 0xff80u;
-  static __device__ __forceinline__ float at(const uint4& w, int i) {
-    const uint32_t x = (i >> 1) == 0 ? w.x : (i >> 1) == 1 ? w.y : (i >> 1) == 2 ? w.z : w.w;
-    return __uint_as_float((i & 1) ? (x & 0xffff0000u) : (x << 16));
+  static __device__ __forceinline__ float2 pair(const uint4& w, int i) {
+    return bf16x2_to_float2(i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w);
+  }
+  static __device__ __forceinline__ float top(const uint4& w) {
+    const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&w);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+    return max_nan(__low2float(m), __high2float(m));
   }
 };
 template <>
 struct Vec<__half> {
   static constexpr int kN = 8;
   static constexpr uint32_t kNegInf = 0xfc00u;
-  static __device__ __forceinline__ float at(const uint4& w, int i) {
-    const uint32_t x = (i >> 1) == 0 ? w.x : (i >> 1) == 1 ? w.y : (i >> 1) == 2 ? w.z : w.w;
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
-    return (i & 1) ? f.y : f.x;
+  static __device__ __forceinline__ float2 pair(const uint4& w, int i) {
+    return __half22float2(reinterpret_cast<const __half2*>(&w)[i]);
+  }
+  static __device__ __forceinline__ float top(const uint4& w) {
+    const __half2* p = reinterpret_cast<const __half2*>(&w);
+    const __half2 m = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+    return max_nan(__low2float(m), __high2float(m));
   }
 };
+template <typename T>
+__device__ __forceinline__ float value_at(const uint4& w, int i) {
+  const float2 f = Vec<T>::pair(w, i >> 1);
+  return (i & 1) ? f.y : f.x;
+}
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -96,27 +120,19 @@ struct Stat {
   float m, s, t;
 };
 
-// (m, s, t) of two disjoint parts as of their union.
-__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float c) {
-  Stat r;
-  r.m = max_nan(a.m, b.m);
-  const float ref = r.m == -INFINITY ? 0.f : r.m;
-  const float da = fmaxf((a.m - ref) * c, -1000.f), db = fmaxf((b.m - ref) * c, -1000.f);   // -inf: s is 0
-  const float fa = exp2f(da), fb = exp2f(db);
-  r.s = a.s * fa + b.s * fb;
-  r.t = fa * (a.t + da * a.s) + fb * (b.t + db * b.s);
-  return r;
-}
-
-// Shared state of one CTA's selection.
+// Shared state of one CTA.
 struct LpShared {
   Key list[kLpList];
   Key best[kLogprobMaxTop];       // the CTA's top n, best first (0: none)
-  Key groups[kLpGroups];
-  Stat stat[kLpWarps];
+  Key groups[kLpGroups];          // group maxima (select_tiles)
+  alignas(16) uint32_t group_bits[kLpGroups];   // order bits of the group maxima over the CTA's part
+  uint32_t warp_top[kLpWarps];
+  float2 warp_sum[kLpWarps];
   Stat total;
   Key bound;                      // only keys above it can be among the top n
-  int count;
+  uint32_t bound_bits;
+  int count, reaching;
+  uint8_t who[kLpThreads];        // the threads whose maximum reaches bound_bits
 };
 
 // The list cut back to its n largest keys, best first, and the bound raised to the n-th. By all threads; m = the
@@ -139,100 +155,60 @@ __device__ __forceinline__ void cut_list(LpShared& sh, int n, int m) {
   __syncthreads();
 }
 
+// A CTA's part of a row: vectors [v0, v1) of the row; vector v holds ids v N - off .. + N - 1 and is aligned in memory
+// (the row's first and last may be cut).
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobArgs a) {
+struct Part {
+  const T* x;
+  int vocab, off, v0, v1;
+  static constexpr int N = Vec<T>::kN;
+
+  __device__ __forceinline__ uint4 load(int v) const {   // ids outside the row, vectors outside the part: -inf
+    const int id = v * N - off;
+    if (v < v1 && id >= 0 && id + N <= vocab) return __ldg(reinterpret_cast<const uint4*>(x + id));
+    uint32_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (N == 4) {
+        q[i] = 0xff800000u;
+        if (v < v1 && id + i >= 0 && id + i < vocab) q[i] = reinterpret_cast<const uint32_t*>(x)[id + i];
+      } else {
+        uint32_t lo = Vec<T>::kNegInf, hi = Vec<T>::kNegInf;
+        if (v < v1 && id + 2 * i >= 0 && id + 2 * i < vocab) lo = reinterpret_cast<const uint16_t*>(x)[id + 2 * i];
+        if (v < v1 && id + 2 * i + 1 >= 0 && id + 2 * i + 1 < vocab)
+          hi = reinterpret_cast<const uint16_t*>(x)[id + 2 * i + 1];
+        q[i] = lo | (hi << 16);
+      }
+    }
+    return make_uint4(q[0], q[1], q[2], q[3]);
+  }
+  __device__ __forceinline__ bool real(int v, int id) const { return v < v1 && id >= 0 && id < vocab; }
+};
+
+// The CTA's top n into sh.list / sh.best, whatever the values: tile by tile with the n-th best key so far.
+template <typename T>
+__device__ __noinline__ void select_tiles(LpShared& sh, const Part<T> part, int n) {
   constexpr int N = Vec<T>::kN;
-  __shared__ LpShared sh;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
-  const long long row = blockIdx.x / parts;
-  const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-  const int n = a.top_n;
-  const float c = a.inv_temp * kLog2e;
-
-  // vectors of the row: vector v holds ids v N - off .. + N - 1 (aligned in memory; the first and last may be cut)
-  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % N);
-  const int vecs = (a.vocab + off + N - 1) / N;
-  const int v0 = static_cast<int>(static_cast<long long>(vecs) * part / parts);
-  const int v1 = static_cast<int>(static_cast<long long>(vecs) * (part + 1) / parts);
-
+  const int tid = threadIdx.x;
+  __syncthreads();
   if (tid == 0) {
     sh.count = 0;
     sh.bound = 0ull;
   }
   __syncthreads();
-
-  auto load = [&](int v) -> uint4 {   // ids outside the row read as -inf
-    uint4 w;
-    const int id = v * N - off;
-    if (v < v1 && id >= 0 && id + N <= a.vocab) {
-      w = __ldcs(reinterpret_cast<const uint4*>(x + id));
-    } else {
-      uint32_t q[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (N == 4) {
-          q[i] = 0xff800000u;
-          if (v < v1 && id + i >= 0 && id + i < a.vocab) q[i] = __float_as_uint(to_float(x[id + i]));
-        } else {
-          uint32_t lo = Vec<T>::kNegInf, hi = Vec<T>::kNegInf;
-          if (v < v1 && id + 2 * i >= 0 && id + 2 * i < a.vocab) lo = reinterpret_cast<const uint16_t*>(x)[id + 2 * i];
-          if (v < v1 && id + 2 * i + 1 >= 0 && id + 2 * i + 1 < a.vocab)
-            hi = reinterpret_cast<const uint16_t*>(x)[id + 2 * i + 1];
-          q[i] = lo | (hi << 16);
-        }
-      }
-      w = make_uint4(q[0], q[1], q[2], q[3]);
-    }
-    return w;
-  };
-
-  Stat st = {-INFINITY, 0.f, 0.f};
-  uint4 next[kLpVecs];
-#pragma unroll
-  for (int j = 0; j < kLpVecs; ++j) next[j] = load(v0 + j * kLpThreads + tid);
-  for (int tile = v0; tile < v1; tile += kLpTileVecs) {
+  for (int tile = part.v0; tile < part.v1; tile += kLpTileVecs) {
     uint4 w[kLpVecs];
 #pragma unroll
-    for (int j = 0; j < kLpVecs; ++j) w[j] = next[j];
-    if (tile + kLpTileVecs < v1) {
-#pragma unroll
-      for (int j = 0; j < kLpVecs; ++j) next[j] = load(tile + kLpTileVecs + j * kLpThreads + tid);
-    }
+    for (int j = 0; j < kLpVecs; ++j) w[j] = part.load(tile + j * kLpThreads + tid);
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kLpVecs; ++j)
-#pragma unroll
-      for (int i = 0; i < N; ++i) top = max_nan(top, Vec<T>::at(w[j], i));
-    if (!(top <= st.m)) {
-      const float d = fmaxf((st.m - top) * c, -1000.f), f = exp2f(d);   // nothing yet: s = t = 0
-      st.t = f * (st.t + d * st.s);
-      st.s *= f;
-      st.m = top;
-    }
-    const float ref = st.m == -INFINITY ? 0.f : st.m;
-#pragma unroll
-    for (int j = 0; j < kLpVecs; ++j)
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float z = (Vec<T>::at(w[j], i) - ref) * c;
-        const float p = exp2f(z);
-        st.s += p;
-        st.t = fmaf(p, fmaxf(z, -1000.f), st.t);   // 0 * -inf would be NaN
-      }
-    if (n == 0) continue;
-
-    // ---- candidates of the tile
-    const uint32_t bound_hi = static_cast<uint32_t>(sh.bound >> 32);
+    for (int j = 0; j < kLpVecs; ++j) top = max_nan(top, Vec<T>::top(w[j]));
     // strictly above: the bound is a value of an earlier tile, whose ids are smaller, and equal values rank by id
-    const bool some = order_bits(top) > bound_hi;
+    const bool some = order_bits(top) > static_cast<uint32_t>(sh.bound >> 32);
     const int threads = __syncthreads_count(some);
     if (threads == 0) continue;
     const int m = sh.count;
     Key bound = sh.bound;
-    auto id_of = [&](int j, int i) { return (tile + j * kLpThreads + tid) * N - off + i; };
-    auto real = [&](int j, int id) { return tile + j * kLpThreads + tid < v1 && id >= 0 && id < a.vocab; };
     if (m + threads * kLpVecs * N > kLpList || threads > kLpThreads / 2) {
       // many: the n-th largest group maximum bounds the tile's part of the top n from below
       Key mine = 0ull;
@@ -240,9 +216,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobAr
       for (int j = 0; j < kLpVecs; ++j)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int id = id_of(j, i);
-          if (real(j, id)) {
-            const Key k = make_key(Vec<T>::at(w[j], i), static_cast<uint32_t>(id));
+          const int v = tile + j * kLpThreads + tid, id = v * N - part.off + i;
+          if (part.real(v, id)) {
+            const Key k = make_key(value_at<T>(w[j], i), static_cast<uint32_t>(id));
             mine = k > mine ? k : mine;
           }
         }
@@ -267,43 +243,164 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobAr
       for (int j = 0; j < kLpVecs; ++j)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int id = id_of(j, i);
-          const Key k = make_key(Vec<T>::at(w[j], i), static_cast<uint32_t>(id));
-          if (k > bound && real(j, id)) sh.list[atomicAdd(&sh.count, 1)] = k;
+          const int v = tile + j * kLpThreads + tid, id = v * N - part.off + i;
+          const Key k = make_key(value_at<T>(w[j], i), static_cast<uint32_t>(id));
+          if (k > bound && part.real(v, id)) sh.list[atomicAdd(&sh.count, 1)] = k;
         }
     }
     __syncthreads();
     if (sh.count > n + kLpSlack) cut_list(sh, n, sh.count);
   }
+  cut_list(sh, n, sh.count);
+}
 
-  // ---- the CTA's (m, s, t) and top n
+template <typename T>
+__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobArgs a) {
+  constexpr int N = Vec<T>::kN;
+  __shared__ LpShared sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const long long row = blockIdx.x / parts;
+  const int n = a.top_n;
+  const float c = a.inv_temp * kLog2e;
+  Part<T> part;
+  part.x = static_cast<const T*>(a.logits) + row * a.row_stride;
+  part.vocab = a.vocab;
+  part.off = static_cast<int>((reinterpret_cast<uintptr_t>(part.x) / sizeof(T)) % N);
+  const int vecs = (a.vocab + part.off + N - 1) / N;
+  part.v0 = static_cast<int>(static_cast<long long>(vecs) * rank / parts);
+  part.v1 = static_cast<int>(static_cast<long long>(vecs) * (rank + 1) / parts);
+
+  if (tid == 0) sh.count = sh.reaching = 0;
+  if (tid < kLogprobMaxTop) sh.best[tid] = 0ull;
+
+  // ---- one pass: the thread's (m, s, t), s and t in two halves
+  float m = -INFINITY;
+  float2 s2 = make_float2(0.f, 0.f), t2 = s2;
+  uint4 next[kLpVecs];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Stat b = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                    __shfl_xor_sync(0xffffffffu, st.t, o)};
-    st = join(st, b, c);
+  for (int j = 0; j < kLpVecs; ++j) next[j] = part.load(part.v0 + j * kLpThreads + tid);
+  for (int tile = part.v0; tile < part.v1; tile += kLpTileVecs) {
+    uint4 w[kLpVecs];
+#pragma unroll
+    for (int j = 0; j < kLpVecs; ++j) w[j] = next[j];
+    if (tile + kLpTileVecs < part.v1) {
+#pragma unroll
+      for (int j = 0; j < kLpVecs; ++j) next[j] = part.load(tile + kLpTileVecs + j * kLpThreads + tid);
+    }
+    float top = Vec<T>::top(w[0]);
+#pragma unroll
+    for (int j = 1; j < kLpVecs; ++j) top = max_nan(top, Vec<T>::top(w[j]));
+    if (!(top <= m)) {
+      const float d = fmaxf((m - top) * c, -1000.f), f = exp2_fast(d);   // nothing yet: s = t = 0
+      t2 = make_float2(f * (t2.x + d * s2.x), f * (t2.y + d * s2.y));
+      s2 = make_float2(f * s2.x, f * s2.y);
+      m = max_nan(m, top);   // a NaN stays
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    const float2 nref = make_float2(-ref, -ref), cc = make_float2(c, c);
+#pragma unroll
+    for (int j = 0; j < kLpVecs; ++j)
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        const float2 z = __fmul2_rn(__fadd2_rn(Vec<T>::pair(w[j], i), nref), cc);
+        const float2 p = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+        s2 = __fadd2_rn(s2, p);
+        t2 = __ffma2_rn(p, make_float2(fmaxf(z.x, -1000.f), fmaxf(z.y, -1000.f)), t2);   // 0 * -inf would be NaN
+      }
   }
-  if (lane == 0) sh.stat[warp] = st;
+  float s = s2.x + s2.y, t = t2.x + t2.y;
+
+  // ---- the CTA's (m, s, t)
+  const uint32_t bits = order_bits(m);
+  const uint32_t wtop = __reduce_max_sync(0xffffffffu, bits);
+  const uint32_t pair_top = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+  if ((tid & 1) == 0) sh.group_bits[tid >> 1] = pair_top;
+  if (lane == 0) sh.warp_top[warp] = wtop;
   __syncthreads();
+  uint32_t all = sh.warp_top[0];
+#pragma unroll
+  for (int k = 1; k < kLpWarps; ++k) all = max(all, sh.warp_top[k]);
+  const float M = order_value(all);
+  {
+    const float d = fmaxf((m - (M == -INFINITY ? 0.f : M)) * c, -1000.f), f = exp2_fast(d);
+    t = M != M ? NAN : f * (t + d * s);
+    s = M != M ? NAN : f * s;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    if (lane == 0) sh.warp_sum[warp] = make_float2(s, t);
+  }
+  // ---- the n-th largest group maximum, the threads that reach it, and the values of theirs that do
   if (n > 0) {
-    if (tid < n) sh.best[tid] = 0ull;
+    if (tid < kLpGroups) {
+      const uint32_t k = sh.group_bits[tid];
+      int above = 0;
+#pragma unroll 4
+      for (int g = 0; g < kLpGroups; g += 4) {
+        const uint4 q = *reinterpret_cast<const uint4*>(&sh.group_bits[g]);
+        above += (q.x > k || (q.x == k && g < tid)) + (q.y > k || (q.y == k && g + 1 < tid)) +
+                 (q.z > k || (q.z == k && g + 2 < tid)) + (q.w > k || (q.w == k && g + 3 < tid));
+      }
+      if (above == n - 1) sh.bound_bits = k;
+    }
     __syncthreads();
-    cut_list(sh, n, sh.count);
+    const uint32_t bound = sh.bound_bits;
+    if (bits >= bound) sh.who[atomicAdd(&sh.reaching, 1)] = static_cast<uint8_t>(tid);
+    __syncthreads();
+    const int reaching = sh.reaching;
+    const int items = reaching * ((part.v1 - part.v0 + kLpThreads - 1) / kLpThreads);
+    for (int i = tid; i < items; i += kLpThreads) {
+      const int v = part.v0 + i / reaching * kLpThreads + sh.who[i % reaching];
+      const uint4 w = part.load(v);
+      if (order_bits(Vec<T>::top(w)) < bound) continue;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float x = value_at<T>(w, e);
+        const int id = v * N - part.off + e;
+        if (order_bits(x) >= bound && part.real(v, id)) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kLpList) sh.list[at] = make_key(x, static_cast<uint32_t>(id));
+        }
+      }
+    }
+    __syncthreads();
+    const int found = sh.count;
+    __syncthreads();
+    if (tid == 0) sh.bound = 0ull;
+    if (found <= kLpList) cut_list(sh, n, found);
+    else select_tiles<T>(sh, part, n);
+  } else {
+    __syncthreads();
   }
   if (tid == 0) {
-    Stat r = sh.stat[0];
-    for (int k = 1; k < kLpWarps; ++k) r = join(r, sh.stat[k], c);
-    sh.total = r;
+    float2 r = sh.warp_sum[0];
+    for (int k = 1; k < kLpWarps; ++k) {
+      r.x += sh.warp_sum[k].x;
+      r.y += sh.warp_sum[k].y;
+    }
+    sh.total = {M, r.x, r.y};
   }
   __syncthreads();
 
   // ---- joined over the row's CTAs, by the first of them
   if (parts > 1) {
     cluster.sync();
-    if (part == 0) {
+    if (rank == 0) {
       if (tid == 0) {
-        Stat r = sh.total;
-        for (int k = 1; k < parts; ++k) r = join(r, cluster.map_shared_rank(&sh, k)->total, c);
+        float top = sh.total.m;
+        for (int k = 1; k < parts; ++k) top = max_nan(top, cluster.map_shared_rank(&sh, k)->total.m);
+        const float ref = top == -INFINITY ? 0.f : top;
+        Stat r = {top, 0.f, 0.f};
+        for (int k = 0; k < parts; ++k) {
+          const Stat p = cluster.map_shared_rank(&sh, k)->total;
+          const float d = fmaxf((p.m - ref) * c, -1000.f), f = exp2_fast(d);
+          r.s += f * p.s;
+          r.t += f * (p.t + d * p.s);
+        }
         sh.total = r;
       }
       if (n > 0) {
@@ -315,21 +412,21 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobAr
       __syncthreads();
     }
     cluster.sync();   // the other CTAs' shared memory has been read
-    if (part != 0) return;
+    if (rank != 0) return;
   }
   const Stat r = sh.total;
-  const float ref = r.m, log_s = logf(r.s);
+  const float log_s = logf(r.s);
   if (tid == 0 && a.entropy) a.entropy[row] = log_s - 0.6931471805599453f * (r.t / r.s);
   for (int i = tid; i < a.given; i += kLpThreads) {
     const long long id = a.ids[row * a.ids_stride + i];
     float lp = -INFINITY;                              // an id outside the vocabulary has no probability
-    if (id >= 0 && id < a.vocab) lp = (to_float(x[id]) - ref) * a.inv_temp - log_s;
+    if (id >= 0 && id < a.vocab) lp = (to_float(part.x[id]) - r.m) * a.inv_temp - log_s;
     a.logprobs[row * a.given + i] = lp;
   }
   if (tid < n) {
     const Key k = sh.best[tid];
     a.top_ids[row * n + tid] = static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(k));
-    a.top_logprobs[row * n + tid] = (order_value(static_cast<uint32_t>(k >> 32)) - ref) * a.inv_temp - log_s;
+    a.top_logprobs[row * n + tid] = (order_value(static_cast<uint32_t>(k >> 32)) - r.m) * a.inv_temp - log_s;
   }
 }
 
