@@ -308,7 +308,7 @@ int q3_sample_topk(const q3_sampler* sampler, void* stream);
 typedef struct q3_quant_cache {
   void* k;                     /* [num_pages, page_size, 8, 128] e4m3, contiguous, 16-byte aligned */
   void* v;
-  void* k_scale;               /* [num_pages, page_size, 8] E8M0 bytes, contiguous, 8-byte aligned */
+  void* k_scale;               /* [num_pages, page_size, 8] E8M0 bytes, contiguous, 16-byte aligned */
   void* v_scale;
   int32_t num_pages;
   int32_t page_size;

@@ -749,7 +749,7 @@ int q3_prefill(const void* q, int64_t q_row_stride, int64_t q_rows, const void* 
 
 static int quant_cache_check(const q3_quant_cache* c) {
   if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || c->num_pages <= 0 || c->page_size <= 0) return Q3_ERR_INVALID;
-  if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 8) || !aligned(c->v_scale, 8))
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 16) || !aligned(c->v_scale, 16))
     return Q3_ERR_ALIGNMENT;
   return Q3_OK;
 }
@@ -835,7 +835,10 @@ int q3_kv_dequant_paged(const q3_quant_cache* cache, int32_t num_kv_heads, int32
 size_t q3_paged_tree_workspace_bytes(int32_t batch, int32_t tokens, int32_t quantised) {
   int dev = 0;
   if (batch < 0 || tokens < 1 || tokens > q3::kTreeMaxTokens || current_device(&dev) != Q3_OK) return 0;
-  return q3::tree_workspace(quantised != 0, batch, tokens, sm_count(dev)).bytes;
+  // the larger of the two kernels' (which one runs depends on the scale's sign too)
+  const size_t x = q3::tree_workspace(quantised != 0, tokens, 1.f, sm_count(dev)).bytes;
+  const size_t y = q3::tree_workspace(quantised != 0, tokens, -1.f, sm_count(dev)).bytes;
+  return x > y ? x : y;
 }
 
 int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -860,13 +863,13 @@ int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_
     return Q3_ERR_INVALID;
   if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->k_pool, 16) || !aligned(p->v_pool, 16) ||
       (p->q_seat_stride % 8) || (p->q_token_stride % 8) || (p->out_seat_stride % 8) || (p->out_token_stride % 8) ||
-      (p->k_scale && (!aligned(p->k_scale, 8) || !aligned(p->v_scale, 8))) ||
+      (p->k_scale && (!aligned(p->k_scale, 16) || !aligned(p->v_scale, 16))) ||
       (draft && (!aligned(p->k_new, 16) || !aligned(p->v_new, 16) || !aligned(p->tree_mask, 8) ||
                  (p->kv_new_seat_stride % 8) || (p->kv_new_token_stride % 8))))
     return Q3_ERR_ALIGNMENT;
   int dev = 0;
   if ((rc = current_device(&dev)) != Q3_OK) return rc;
-  const q3::TreeWorkspace w = q3::tree_workspace(p->k_scale != nullptr, p->batch, p->tokens, sm_count(dev));
+  const q3::TreeWorkspace w = q3::tree_workspace(p->k_scale != nullptr, p->tokens, p->softmax_scale, sm_count(dev));
   if (!workspace || workspace_bytes < w.bytes || !aligned(workspace, 256)) return Q3_ERR_WORKSPACE;
   q3::TreeArgs a{};
   if ((rc = status_ptr(dev, &a.status)) != Q3_OK) return rc;
@@ -892,6 +895,9 @@ int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_
   a.max_pages = p->max_pages_per_seat;
   a.num_pages = p->num_pages;
   a.page_size = p->page_size;
+  a.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (p->page_size == 1 << s) a.page_shift = s;
   a.B = p->batch;
   a.tokens = p->tokens;
   a.groups = w.groups;

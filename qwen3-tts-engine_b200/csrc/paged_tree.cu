@@ -26,8 +26,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
-#include "q3_common.cuh"
-#include "q3_kernels.h"
+#include "tree_common.cuh"
 
 namespace q3 {
 
@@ -54,31 +53,6 @@ struct TreeStage {
   static_assert(kDraftRows * kDraftKStride <= kV && kV + kDraftRows * kDraftVStride <= kScales && kBytes % 16 == 0,
                 "drafted rows fit their stage");
 };
-
-struct Item {
-  int seat, tok0;      // first token of the group
-  int len, drafts;     // cached tokens; drafted rows
-  int nc, n;           // cache chunks; all chunks
-};
-
-template <int TOK, int DROWS>
-__device__ __forceinline__ Item tree_item(const TreeArgs& a, int w) {
-  Item it;
-  it.seat = a.groups == 1 ? w : w / a.groups;
-  it.tok0 = (w - it.seat * a.groups) * TOK;
-  const long long cap = static_cast<long long>(a.max_pages) * a.page_size;
-  const int raw = a.seqlens[it.seat];
-  it.len = raw < 0 ? 0 : static_cast<int>(raw > cap ? cap : raw);
-  it.drafts = a.k_new == nullptr ? 0 : a.tokens;
-  int live = a.tokens;
-  if (a.draft_lens != nullptr) {
-    const int d = a.draft_lens[it.seat];
-    live = it.drafts = d < 0 ? 0 : (d > a.tokens ? a.tokens : d);
-  }
-  it.nc = (it.len + kTreeRows - 1) / kTreeRows;
-  it.n = it.tok0 < live ? it.nc + (it.drafts + DROWS - 1) / DROWS : 0;
-  return it;
-}
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
   asm volatile(
@@ -151,7 +125,7 @@ __device__ __forceinline__ int row_dim(int g, int mt) {
 }
 
 template <bool FP8, int NT>
-__device__ __forceinline__ void tree_begin(const TreeArgs& a, const Item& it, int h, int lane, TreeState<FP8, NT>& st) {
+__device__ __forceinline__ void tree_begin(const TreeArgs& a, const TreeItem& it, int h, int lane, TreeState<FP8, NT>& st) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -435,7 +409,7 @@ __device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uin
 // End of an item's chunks in this CTA. slot < 0: the item is complete and its rows are written; else its partial goes
 // to that workspace slot: outputs [8 heads][2 TOK columns][128] fp32 and (maximum, sum) pairs.
 template <bool FP8, int NT>
-__device__ __forceinline__ void tree_finish(const TreeArgs& a, const Item& it, int h, int lane, TreeState<FP8, NT>& st,
+__device__ __forceinline__ void tree_finish(const TreeArgs& a, const TreeItem& it, int h, int lane, TreeState<FP8, NT>& st,
                                             int slot) {
   constexpr int kCols = 8 * NT;
   const int g = lane >> 2, t = lane & 3;
@@ -492,101 +466,6 @@ __device__ __forceinline__ void tree_finish(const TreeArgs& a, const Item& it, i
   }
 }
 
-struct TreePlan {
-  long long N, c0, c1;   // chunks of all items; this CTA's range
-  long long first;       // global index of the first chunk of item `w`
-  int Ge, w;             // CTAs that have chunks; the item that holds chunk c0
-};
-
-// Work split of the CTA, by all its threads. Items without chunks (nothing to attend, or padded tokens alone) get
-// their zero rows here. Returns false when the CTA has no chunk.
-template <int TOK, int DROWS>
-__device__ __forceinline__ bool tree_plan(const TreeArgs& a, TreePlan& P) {
-  constexpr int kWarps = kTreeThreads / 32;
-  __shared__ long long sums[kWarps];
-  __shared__ long long found_first;
-  __shared__ int found_item;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int G = gridDim.x, c = blockIdx.x, W = a.B * a.groups;
-  long long local = 0;
-  for (int w = tid; w < W; w += kTreeThreads) {
-    const Item it = tree_item<TOK, DROWS>(a, w);
-    local += it.n;
-    if (c == 0 && (a.seqlens[it.seat] < 0 || a.seqlens[it.seat] > it.len ||
-                   (a.draft_lens != nullptr && a.draft_lens[it.seat] != it.drafts)))
-      atomicOr(a.status, kStatusBadLength);
-    if (it.n == 0 && w % G == c) {
-      for (int tok = it.tok0; tok < min(it.tok0 + TOK, a.tokens); ++tok) {
-        uint4* o = reinterpret_cast<uint4*>(a.out + static_cast<long long>(it.seat) * a.out_seat +
-                                            static_cast<long long>(tok) * a.out_tok);
-        for (int k = 0; k < kQHeads * kHeadDim / 8; ++k) o[k] = make_uint4(0, 0, 0, 0);
-      }
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) local += __shfl_xor_sync(0xffffffffu, local, o);
-  if (lane == 0) sums[warp] = local;
-  __syncthreads();
-  long long N = 0;
-#pragma unroll
-  for (int k = 0; k < kWarps; ++k) N += sums[k];
-  P.N = N;
-  P.Ge = static_cast<int>(N < G ? N : G);
-  if (c >= P.Ge) return false;
-  P.c0 = N * c / P.Ge;
-  P.c1 = N * (c + 1) / P.Ge;
-  long long base = 0;
-  for (int w0 = 0; w0 < W; w0 += kTreeThreads) {
-    const int w = w0 + tid;
-    const int n = w < W ? tree_item<TOK, DROWS>(a, w).n : 0;
-    long long incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
-    }
-    __syncthreads();
-    if (lane == 31) sums[warp] = incl;
-    __syncthreads();
-    long long before = base, total = 0;
-#pragma unroll
-    for (int k = 0; k < kWarps; ++k) {
-      if (k < warp) before += sums[k];
-      total += sums[k];
-    }
-    incl += before;
-    if (n > 0 && incl - n <= P.c0 && P.c0 < incl) {
-      found_item = w;
-      found_first = incl - n;
-    }
-    base += total;
-    if (base > P.c0) break;   // uniform
-  }
-  __syncthreads();
-  P.w = found_item;
-  P.first = found_first;
-  return true;
-}
-
-__device__ __forceinline__ void cp_async8(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
-}
-// One arrival on `bar` (counted in its expected ones) when this thread's earlier cp.async copies have landed.
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
-// Pool row of token `tok` of `seat`; an entry outside the pool reads page 0 and raises its status bit.
-__device__ __forceinline__ long long tree_pool_row(const TreeArgs& a, int seat, int tok) {
-  const int pidx = tok / a.page_size;
-  int pg = a.block_table[static_cast<long long>(seat) * a.bt_stride + pidx];
-  if (pg < 0 || pg >= a.num_pages) {
-    atomicOr(a.status, kStatusBadPage);
-    pg = 0;
-  }
-  return static_cast<long long>(pg) * a.page_size + (tok - pidx * a.page_size);
-}
-
 // The producer warp: lanes 0..15 bring the chunk's K rows, lanes 16..31 its V rows, one bulk copy each; with an e4m3
 // cache also the row's eight scales. The addresses of the next chunk are looked up before the wait for a free stage.
 template <bool FP8, int TOK, int STAGES>
@@ -596,12 +475,12 @@ __device__ __forceinline__ void tree_produce(const TreeArgs& a, const TreePlan& 
   const int row = lane & 15, which = lane >> 4;
   int w = P.w;
   long long first = P.first;
-  Item it = tree_item<TOK, SL::kDraftRows>(a, w);
+  TreeItem it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, w);
   long long k = 0;
   for (long long i = P.c0; i < P.c1; ++i, ++k) {
     while (i >= first + it.n) {
       first += it.n;
-      it = tree_item<TOK, SL::kDraftRows>(a, ++w);
+      it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, ++w);
     }
     const int j = static_cast<int>(i - first);
     const bool draft = j >= it.nc;
@@ -671,7 +550,7 @@ __global__ void __launch_bounds__(kTreeThreads, MIN_CTAS) paged_tree_kernel(cons
     fence_mbar_init();
   }
   TreePlan P;
-  if (!tree_plan<TOK, SL::kDraftRows>(a, P)) return;   // its barriers published the barrier init
+  if (!tree_plan<TOK, kTreeRows, SL::kDraftRows, kTreeThreads>(a, P, blockIdx.x, gridDim.x, 0, kQHeads)) return;   // its barriers published the barrier init
 
   if (warp == kTreeConsumers) {
     tree_produce<FP8, TOK, STAGES>(a, P, smem, full, empty, abort_flag, lane);
@@ -683,10 +562,10 @@ __global__ void __launch_bounds__(kTreeThreads, MIN_CTAS) paged_tree_kernel(cons
   long long first = P.first, i = P.c0, k = 0;
   bool ok = true;
   while (i < P.c1 && ok) {
-    Item it = tree_item<TOK, SL::kDraftRows>(a, w);
+    TreeItem it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, w);
     while (i >= first + it.n) {
       first += it.n;
-      it = tree_item<TOK, SL::kDraftRows>(a, ++w);
+      it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, ++w);
     }
     tree_begin<FP8, NT>(a, it, h, lane, st);
     const long long end = first + it.n < P.c1 ? first + it.n : P.c1;
@@ -726,9 +605,7 @@ __global__ void __launch_bounds__(kTreeThreads, MIN_CTAS) paged_tree_kernel(cons
     const bool from_before = first < P.c0, goes_on = first + it.n > P.c1;
     tree_finish<FP8, NT>(a, it, h, lane, st, from_before ? 2 * c : (goes_on ? 2 * c + 1 : -1));
     if (!from_before && goes_on && h == 0 && lane == 0) {
-      // the last CTA of the item: the one that holds chunk e = its last; c(e) = the largest with N * c / Ge <= e
-      const long long e = first + it.n - 1;
-      a.ws_span[c] = make_int2(w, static_cast<int>(((e + 1) * P.Ge + P.N - 1) / P.N - 1));
+      a.ws_span[c] = make_int2(w, tree_last_share(P, first + it.n - 1));
     }
   }
   if (!ok && lane == 0)
@@ -737,8 +614,8 @@ __global__ void __launch_bounds__(kTreeThreads, MIN_CTAS) paged_tree_kernel(cons
 }
 
 // Adds the partials of the item that starts in CTA c and goes on (if there is one) for KV head h: CTA (c, h).
-// cols = 2 heads x TOK tokens; each column's 128 dims in a warp, and with fewer columns than warps the partials of a
-// column are shared out over several warps.
+// cols = 2 heads x TOK tokens, eight to a CTA (blockIdx.z); each column's 128 dims in a warp, and with fewer columns than
+// warps the partials of a column are shared out over several warps.
 constexpr int kMergeWarps = 8;
 
 __global__ void __launch_bounds__(kMergeWarps * 32) paged_tree_merge_kernel(const TreeArgs a, int tok_per_group) {
@@ -750,15 +627,16 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_tree_merge_kernel(cons
   if (span.x < 0) return;
   const int seat = span.x / a.groups, tok0 = (span.x - seat * a.groups) * tok_per_group;
   const int cols = 2 * tok_per_group, parts = span.y - c + 1;
-  const int live = 2 * min(tok_per_group, a.tokens - tok0);
+  const int col0 = blockIdx.z * kMergeWarps, live = min(2 * min(tok_per_group, a.tokens - tok0) - col0, kMergeWarps);
+  if (live <= 0) return;
   int drafts = a.tokens;
   if (a.draft_lens != nullptr) drafts = a.draft_lens[seat];
   int share = 1;                                     // warps per column: the largest power of two that leaves none over
   while (share * 2 * live <= kMergeWarps) share *= 2;
   const int per = kMergeWarps / share;               // columns at a time
-  for (int col0 = 0; col0 < live; col0 += per) {     // uniform
+  {
     const int col = col0 + warp % per, sub = warp / per;
-    const bool mine = col < live;
+    const bool mine = warp % per < live;
     // partial x of the column: slot 2c + 1 for x = 0, then slot 2(c + x)
     auto at = [&](int x) {
       return (static_cast<long long>(x == 0 ? 2 * c + 1 : 2 * (c + x)) * kKvHeads + h) * cols + col;
@@ -806,18 +684,17 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_tree_merge_kernel(cons
 }
 
 struct TreeConfig {
-  int tok, ctas_per_sm;
+  bool tc;               // the tcgen05 kernel
+  int tok, shares;       // tokens per group; shares of the chunk list
 };
 
-// Tokens per group: 4 (one 8-column tile) or 8 (two). Longer drafts run as groups of 8 that each read the cache.
-TreeConfig tree_config(bool fp8, int tokens) {
+// Up to 8 tokens: the kernel above, a group of 4 (one 8-column tile) or 8 (two), as many shares as CTAs fit. More: the
+// tcgen05 kernel, whose time does not grow with the tokens, one share per 8 SMs (a CTA per KV head). Its row maximum
+// takes the scale for positive; other scales run here in groups of 8 that each read the cache.
+TreeConfig tree_config(bool fp8, int tokens, float scale, int num_sms) {
+  if (tokens > 8 && scale > 0.f) return {true, tokens, max(1, num_sms / kKvHeads)};
   const int tok = tokens <= 4 ? 4 : 8;
-  return {tok, fp8 && tok == 4 ? 2 : 1};
-}
-
-long long tree_grid(bool fp8, int batch, int tokens, int num_sms) {
-  (void)batch;
-  return static_cast<long long>(num_sms) * tree_config(fp8, tokens).ctas_per_sm;
+  return {false, tok, fp8 && tok == 4 ? 2 * num_sms : num_sms};
 }
 
 template <bool FP8, int NT, int STAGES, int MIN_CTAS>
@@ -839,36 +716,40 @@ cudaError_t launch_tree_main(const TreeArgs& a, int grid, cudaStream_t stream) {
 
 }  // namespace
 
-TreeWorkspace tree_workspace(bool fp8, int batch, int tokens, int num_sms) {
+TreeWorkspace tree_workspace(bool fp8, int tokens, float scale, int num_sms) {
   TreeWorkspace w;
-  const TreeConfig cfg = tree_config(fp8, tokens);
-  w.grid = static_cast<int>(tree_grid(fp8, batch, tokens, num_sms));
-  const size_t cols = 2ull * w.grid * kKvHeads * 2 * cfg.tok;   // two slots per CTA
-  w.span = 0;
-  w.ml = (static_cast<size_t>(w.grid) * sizeof(int2) + 255) / 256 * 256;
-  w.o = w.ml + cols * 2 * sizeof(float);
-  w.bytes = w.o + cols * kHeadDim * sizeof(float);
+  const TreeConfig cfg = tree_config(fp8, tokens, scale, num_sms);
+  w.tc = cfg.tc;
+  w.tok = cfg.tok;
+  w.shares = cfg.shares;
   w.groups = (tokens + cfg.tok - 1) / cfg.tok;
+  const size_t cols = 2ull * w.shares * kKvHeads * 2 * cfg.tok;   // two slots per share
+  w.span = 0;
+  w.ml = (static_cast<size_t>(w.shares) * sizeof(int2) + 255) / 256 * 256;
+  w.o = w.ml + (cols * 2 * sizeof(float) + 255) / 256 * 256;
+  w.bytes = w.o + cols * kHeadDim * sizeof(float);
   return w;
 }
 
 cudaError_t launch_paged_tree(const TreeArgs& a, const TreeWorkspace& w, cudaStream_t stream) {
   const bool fp8 = a.k_scale != nullptr;
-  const TreeConfig cfg = tree_config(fp8, a.tokens);
   cudaError_t e;
-  if (fp8) e = cfg.tok == 4 ? launch_tree_main<true, 1, 3, 2>(a, w.grid, stream) : launch_tree_main<true, 2, 6, 1>(a, w.grid, stream);
-  else e = cfg.tok == 4 ? launch_tree_main<false, 1, 3, 1>(a, w.grid, stream) : launch_tree_main<false, 2, 3, 1>(a, w.grid, stream);
+  if (w.tc) e = launch_paged_tree_tc(a, w.shares, stream);
+  else if (fp8 && w.tok == 4) e = launch_tree_main<true, 1, 3, 2>(a, w.shares, stream);
+  else if (fp8) e = launch_tree_main<true, 2, 6, 1>(a, w.shares, stream);
+  else if (w.tok == 4) e = launch_tree_main<false, 1, 3, 1>(a, w.shares, stream);
+  else e = launch_tree_main<false, 2, 3, 1>(a, w.shares, stream);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(w.grid, kKvHeads);
+  lc.gridDim = dim3(w.shares, kKvHeads, (2 * w.tok + kMergeWarps - 1) / kMergeWarps);
   lc.blockDim = dim3(kMergeWarps * 32);
   lc.stream = stream;
   lc.attrs = &at;
   lc.numAttrs = 1;
-  return cudaLaunchKernelEx(&lc, paged_tree_merge_kernel, a, cfg.tok);
+  return cudaLaunchKernelEx(&lc, paged_tree_merge_kernel, a, w.tok);
 }
 
 }  // namespace q3

@@ -1,0 +1,718 @@
+// Attention of 9 to 64 drafted tokens per seat over a paged K/V cache (bf16 or e4m3), on the 5th-generation tensor
+// cores (tcgen05 + TMEM), sm_100a. The mathematics, the contract and the chunk list are those of paged_tree.cu.
+//
+// One CTA = (share of the chunk list, KV head h). Accumulator row r = 2 token + (q head & 1): the up to 128 rows of a seat
+// share every K/V tile, so the cache is read once however many tokens were drafted. Tiles of 64 keys:
+//   S = Q K^T      M = 128 rows, N = 64 keys:  A = Q, B = K from shared memory (128-byte swizzle)
+//   O += P V       M = 128, N = 128 dims:      A = P (bf16) from TMEM, B = V from shared memory
+// The 8 CTAs of a share walk the same keys at the same time, one head each, so the 256 (128) contiguous bytes a CTA
+// takes of a token row join the other heads' in the DRAM page. Warps:
+//   copies (4/3)  bring the head's part of 64 token rows by TMA tensor copies of 128 bytes x R rows, R the largest
+//                 power of two up to 64 that divides the page size (a box never leaves its page), with the table
+//                 entries looked up a tile ahead. bf16 rows land swizzled, as operands. e4m3 rows (and their scales)
+//                 land in a ring of raw tiles. (Four-row gathers serve any page the same way but took 66 cycles each,
+//                 64 of them a tile: 341 us on 24 seats x 64 tokens x 1000 to 8000 rows.) Issuing a tile's copies
+//                 takes a warp longer than the tile's bytes take HBM, so the warps take tiles in turn.
+//   loaders (4/8) turn raw e4m3 tiles into bf16 operands, exactly (four significant bits times a power of two); write Q of
+//                 a new seat and the drafted rows (the last tile of a seat); zero V rows past a seat's last token.
+//   MMA (1)       lane 0 issues S(t+1) before P(t) V(t), so the tensor core works while the softmax does.
+//   softmax (4)   thread r owns row r: online softmax with a lazy maximum (O is rescaled in TMEM when it grows by more
+//                 than 2^8), P(t) as bf16 into TMEM over S(t); at a seat's end O to the output, or as a partial to the
+//                 workspace. Warps without live rows have no part in any of it.
+// An infinity or NaN in a drafted V row would reach rows that do not see it as 0 * inf: the loaders write zero in its
+// place and raise a flag, and the rows that do see it get it back at the end.
+//
+// Bound: HBM for few tokens; for 64 the exponentials come near it (128 x 64 per tile against 32 KB of K and V: 512 of
+// 1424 cycles of the SM's share of the measured copy rate).
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cstring>
+
+#include "prefill_common.cuh"
+#include "tensor_map.cuh"
+#include "tree_common.cuh"
+
+namespace q3 {
+
+namespace {
+
+constexpr int kTcRows = 64;                     // keys per tile (cached rows, or all drafted rows)
+constexpr int kTcTok = kTreeMaxTokens;          // tokens per item: the whole draft
+constexpr int kTcTmemCols = 256;
+constexpr uint32_t kTcOCol = 128;               // S(t), P(t) at column 64 * (t & 1); O at 128
+constexpr int kTcOddSlots = 8;
+constexpr int kTcLoaderWarp = 4;                // after the softmax warps 0-3
+
+// LARGE: more than 32 tokens. Q takes 256 bytes per accumulator row of live warps (the rows after them are whatever
+// follows in shared memory: they only reach rows nobody reads); what it leaves goes to the rings.
+template <bool FP8, bool LARGE>
+struct TcSmem {
+  static constexpr int kLoaders = FP8 ? 8 : 4;               // loader warps
+  static constexpr int kCopyWarps = FP8 ? 3 : 4;
+  static constexpr int kMmaWarp = kTcLoaderWarp + kLoaders, kCopyWarp = kMmaWarp + 1;
+  static constexpr int kThreads = (kCopyWarp + kCopyWarps) * 32;
+  static constexpr int kStages = FP8 ? (LARGE ? 3 : 4) : (LARGE ? 5 : 6);   // operand tiles
+  static constexpr int kRawSlots = FP8 ? 3 : 0;
+  static constexpr int kCopySlots = FP8 ? kRawSlots : kStages;   // tiles the copies fill
+  static constexpr int kQBytes = LARGE ? 32768 : 16384, kTile = 16384, kHalf = 8192;
+  static constexpr int kQ = 0;                               // two Q buffers: [2 dim halves][128 or 64 rows][128 B]
+  static constexpr int kKv = 2 * kQBytes;                    // stage s: K then V, [2 dim halves][64 keys][128 B] each
+  static constexpr int kRaw = kKv + kStages * 2 * kTile;     // raw e4m3: K then V [64 rows][128 B], scales [2][64][8]
+  static constexpr int kRawBytes = 2 * kTcRows * kHeadDim + 2 * kTcRows * kKvHeads;
+  static constexpr int kBars = kRaw + kRawSlots * kRawBytes;
+  static constexpr int kFull = 0, kEmpty = kStages, kCopied = 2 * kStages, kRawFree = kCopied + kCopySlots,
+                       kSFull = kRawFree + kRawSlots, kPFull = kSFull + 2, kPvDone = kPFull + 2, kOFree = kPvDone + 2,
+                       kFinal = kOFree + 1, kNumBars = kFinal + 1;
+  static constexpr int kTmemSlot = kBars + 8 * kNumBars;
+  static constexpr int kAbort = kTmemSlot + 4;
+  static constexpr int kIssued = kAbort + 4;                 // per copy warp, 1 + its last tile issued (abort path)
+  static constexpr int kOdd = kIssued + 4 * kCopyWarps;
+  static constexpr int kBytes = kOdd + 4 * kTcOddSlots;
+  static constexpr int kAlloc = kBytes + 1024;               // slack to align the base to 1024 B (swizzle atoms)
+  static_assert(kAlloc <= 232448 && kRawBytes % 1024 == 0, "shared memory");
+};
+
+struct TcParams {
+  TreeArgs a;
+  CUtensorMap k, v;    // the pools as [rows][1024]: boxes of box_rows rows x 128 bytes
+  int box_rows;
+};
+
+// A box of rows from `row` on, 128 bytes each from column x.
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int row, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar)
+      : "memory");
+}
+// Wait for phase `parity` of `bar`; false after 2 s or once another role has raised the abort flag. The waits sleep in the
+// barrier (up to 20 us at a time): 14 to 16 warps that poll instead take the issue slots the softmax warps need.
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  auto poll = [&]() -> bool {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    return ok != 0;
+  };
+  if (poll()) return true;
+  const uint64_t t0 = global_timer_ns();
+#pragma unroll 1
+  while (!poll())
+    if (*abort_flag || global_timer_ns() - t0 > 2000000000ull) return false;
+  return true;
+}
+
+// The MMAs without the optional mask of output lanes.
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)));
+}
+__device__ __forceinline__ void tc_mma_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)));
+}
+__device__ __forceinline__ void st_shared16(uint32_t dst, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8_at(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// Byte offset of 16-byte unit c (0..15) of a row in an operand tile whose dim halves are `half` bytes apart.
+__device__ __forceinline__ uint32_t tc_unit(int row, int c, int half) {
+  return static_cast<uint32_t>((c >> 3) * half + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+}
+
+// Where a warp stands in the CTA's tiles 0 .. n - 1 (tile k = chunk P.c0 + k): the item that holds tile k, its tiles here
+// [begin, end) and the item's chunk index of tile `begin`. Each role walks the tiles on its own; a step within an item is a
+// comparison (one warp's instructions run one after another, five cycles or so each, and every role is on the tile's path).
+struct TcCursor {
+  int w, index;          // item; how many items of this CTA came before it
+  int begin, end, j0;
+  long long first;
+  TreeItem it;
+};
+__device__ __forceinline__ void tc_enter(const TreePlan& P, TcCursor& c) {
+  c.begin = static_cast<int>(max(c.first - P.c0, 0ll));
+  c.end = static_cast<int>(min(c.first + c.it.n, P.c1) - P.c0);
+  c.j0 = static_cast<int>(max(P.c0 - c.first, 0ll));
+}
+// To tile k >= the present one; true when that is another item.
+__device__ __forceinline__ bool tc_seek(const TreeArgs& a, const TreePlan& P, TcCursor& c, int k) {
+  if (k < c.end) return false;
+  while (P.c0 + k >= c.first + c.it.n) {
+    c.first += c.it.n;
+    c.it = tree_item<kTcTok, kTcRows, kTcTok>(a, ++c.w);
+    c.index += c.it.n > 0;
+  }
+  tc_enter(P, c);
+  return true;
+}
+__device__ __forceinline__ int tc_chunk(const TcCursor& c, int k) { return c.j0 + k - c.begin; }
+
+// Four e4m3 bytes times f as two packed bf16 words, exact.
+__device__ __forceinline__ uint2 dequant4(uint32_t w, float2 f) {
+  const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
+  const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
+  const float2 x = __fmul2_rn(__half22float2(*reinterpret_cast<const __half2*>(&lo)), f);
+  const float2 y = __fmul2_rn(__half22float2(*reinterpret_cast<const __half2*>(&hi)), f);
+  return make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(y.x, y.y));
+}
+
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
+  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
+  return w;
+}
+
+// ------------------------------------------------------------------ the copy warps: warp cw, tiles cw, cw + kCopyWarps, ..
+// Lane l looks after rows 4 (l & 15) .. + 3 of a tile, of K (l < 16) or V, and copies the boxes that start there. With
+// boxes of four rows or more those rows are neighbours in the pool: one table entry, one box at most. All of a tile's
+// addresses are ready before its slot is waited for.
+template <bool FP8, bool LARGE>
+__device__ __forceinline__ void tc_copies(const TcParams& p, const TreePlan& P, TcCursor cur, uint8_t* smem, uint64_t* bars,
+                                          volatile int* abort_flag, volatile int* issued, int h, int cw, int lane) {
+  using SM = TcSmem<FP8, LARGE>;
+  const TreeArgs& a = p.a;
+  const int n = static_cast<int>(P.c1 - P.c0), which = lane >> 4, r0 = 4 * (lane & 15);
+  const CUtensorMap* map = which ? &p.v : &p.k;
+  const uint32_t base = smem_addr(smem) + (FP8 ? SM::kRaw + which * kTcRows * kHeadDim : SM::kKv + which * SM::kTile) + r0 * 128;
+  const uint8_t* scale = FP8 ? (which ? a.v_scale : a.k_scale) : nullptr;
+  const uint32_t scale_dst = smem_addr(smem) + SM::kRaw + 2 * kTcRows * kHeadDim + (which * kTcRows + r0) * kKvHeads;
+  const int x0 = h * kHeadDim, R = p.box_rows;
+  const bool wide = R >= 4, copies = !wide || r0 % R == 0;
+  const int slot_bytes = FP8 ? SM::kRawBytes : 2 * SM::kTile;
+  int pages[4], len = 0, tok = 0;
+  bool starts = true;
+  auto look_up = [&](int k) {   // asks for the table entries of tile k; len: 0 for a drafted tile
+    starts = tc_seek(a, P, cur, k) || k == 0;
+    const int j = tc_chunk(cur, k);
+    len = j < cur.it.nc ? cur.it.len : 0;
+    tok = j * kTcRows + r0;
+    if (wide) {
+      int first[1];
+      tree_pages<1, 1>(a, cur.it.seat, tok, len, first);
+      pages[0] = first[0];
+    } else {
+      tree_pages<4, 1>(a, cur.it.seat, tok, len, pages);
+    }
+  };
+  if (cw >= n) return;
+  look_up(cw);
+  for (int k = cw; k < n; k += SM::kCopyWarps) {
+    const int slot = k % SM::kCopySlots;
+    const bool cached = len > 0;
+    // rows past the last token: any row of the pool (their scores are not kept, their V rows are zeroed)
+    int rows[4];
+    rows[0] = static_cast<int>(max(tree_row(a, pages[0], tok, len), 0ll));
+    if (!wide) {
+#pragma unroll
+      for (int x = 1; x < 4; ++x) rows[x] = static_cast<int>(max(tree_row(a, pages[x], tok + x, len), 0ll));
+    }
+    if (starts) {   // a new seat's Q into the L2 cache
+      for (int r = lane; r < 4 * a.tokens; r += 32)
+        prefetch_l2(a.q + static_cast<long long>(cur.it.seat) * a.q_seat + static_cast<long long>(r >> 2) * a.q_tok +
+                    (2 * h + ((r >> 1) & 1)) * kHeadDim + (r & 1) * (kHeadDim / 2));
+    }
+    if (!cached) {   // so are drafted rows: the loaders read them
+      const __nv_bfloat16* src = (which ? a.v_new : a.k_new) + static_cast<long long>(cur.it.seat) * a.kv_seat + x0;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (r0 + x < cur.it.drafts) {
+          prefetch_l2(src + static_cast<long long>(r0 + x) * a.kv_tok);
+          prefetch_l2(src + static_cast<long long>(r0 + x) * a.kv_tok + kHeadDim / 2);
+        }
+    }
+    if (k + SM::kCopyWarps < n) look_up(k + SM::kCopyWarps);
+    if (k >= SM::kCopySlots) {
+      const int bar = FP8 ? SM::kRawFree + slot : SM::kEmpty + slot;
+      if (!__all_sync(0xffffffffu, tc_wait(&bars[bar], (k / SM::kCopySlots - 1) & 1, abort_flag))) {
+        if (lane == 0) tw_fail(a.status, abort_flag);
+        return;
+      }
+      fence_proxy_async_smem();   // generic reads and writes of the slot before the copies overwrite it
+    }
+    uint64_t* bar = &bars[SM::kCopied + slot];
+    if (lane == 0) {
+      if (cached) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(FP8 ? 2 * kTcRows * kHeadDim : 2 * SM::kTile));
+      else mbar_arrive(bar);
+      issued[cw] = k + 1;
+    }
+    __syncwarp();
+    if (cached) {
+      const uint32_t dst = base + slot * slot_bytes, b = smem_addr(bar);
+      if (wide) {
+        if (copies) {
+          tma_load_2d(dst, map, x0, rows[0], b);
+          if (!FP8) tma_load_2d(dst + SM::kHalf, map, x0 + 64, rows[0], b);
+        }
+        if (FP8) {
+          const uint8_t* src = scale + static_cast<long long>(rows[0]) * kKvHeads;
+          cp_async16_at(scale_dst + slot * slot_bytes, src);
+          cp_async16_at(scale_dst + slot * slot_bytes + 16, src + 16);
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (x % R == 0) {
+            tma_load_2d(dst + x * 128, map, x0, rows[x], b);
+            if (!FP8) tma_load_2d(dst + SM::kHalf + x * 128, map, x0 + 64, rows[x], b);
+          }
+          if (FP8) cp_async8_at(scale_dst + slot * slot_bytes + x * kKvHeads, scale + static_cast<long long>(rows[x]) * kKvHeads);
+        }
+      }
+    }
+    if (FP8) cp_async_arrive(bar);
+  }
+}
+
+// ------------------------------------------------------------------ the loader warps
+template <bool FP8, bool LARGE>
+struct TcLoader {
+  using SM = TcSmem<FP8, LARGE>;
+  static constexpr int kThreads = SM::kLoaders * 32, kRowStep = kThreads / 16;   // 16 threads per row of 256 bytes
+  const TreeArgs& a;
+  const TreePlan& P;
+  uint32_t sbase;
+  uint8_t* smem;
+  uint64_t* bars;
+  volatile int* abort_flag;
+  int h, tid;
+
+  // Everything of tile k that the copies do not write, then the tile is handed to the tensor core. last0, last1: the
+  // last tiles of the item before and of the one before that (-1: none).
+  __device__ __forceinline__ bool tile(int k, TcCursor& c, int& last0, int& last1, volatile int* odd) {
+    const int stage = k % SM::kStages;
+    const bool starts = tc_seek(a, P, c, k) || k == 0;
+    const int j = tc_chunk(c, k);
+    const uint32_t dst = sbase + SM::kKv + static_cast<uint32_t>(stage) * 2 * SM::kTile;
+    if (k >= SM::kStages && !wait(SM::kEmpty + stage, (k / SM::kStages - 1) & 1)) return false;
+    if (starts) {
+      // the Q buffer's last user is two items back; once its stage has been handed out again it is done
+      last1 = last0;
+      last0 = k - 1;
+      if (last1 >= 0 && k < last1 + SM::kStages && !wait(SM::kEmpty + last1 % SM::kStages, (last1 / SM::kStages) & 1))
+        return false;
+      load_q(c.it.seat, sbase + SM::kQ + (c.index & 1) * SM::kQBytes);
+    }
+    const int real = c.it.len - j * kTcRows;   // cached tiles: rows that hold a token
+    bool wrote = starts;
+    if (FP8) {
+      const int slot = k % (SM::kRawSlots + !FP8);
+      if (!wait(SM::kCopied + slot, (k / (SM::kRawSlots + !FP8)) & 1)) return false;
+      if (j < c.it.nc) convert(smem + SM::kRaw + slot * SM::kRawBytes, dst, real);
+      __syncwarp();
+      if ((tid & 31) == 0) mbar_arrive(&bars[SM::kRawFree + slot]);
+      wrote = true;
+    } else if (j < c.it.nc && real < kTcRows) {
+      // whatever lies in the rows behind the last token, their probability 0 must meet a 0
+      if (!wait(SM::kCopied + stage, (k / SM::kStages) & 1)) return false;
+      for (int i = tid; i < (kTcRows - real) * 16; i += kThreads)
+        st_shared16(dst + SM::kTile + tc_unit(real + (i >> 4), i & 15, SM::kHalf), make_uint4(0, 0, 0, 0));
+      wrote = true;
+    }
+    if (j >= c.it.nc) {
+      if (load_draft(c.it, dst)) odd[c.index % kTcOddSlots] = c.index + 1;
+      wrote = true;
+    }
+    if (wrote) fence_proxy_async_smem();   // this thread's writes before the tensor core reads
+    __syncwarp();
+    if ((tid & 31) == 0) mbar_arrive(&bars[SM::kFull + stage]);
+    return true;
+  }
+
+  // A raw e4m3 tile as bf16 operands; rows past `real` as zeros. 8 threads per row, 16 values each.
+  __device__ __forceinline__ void convert(const uint8_t* raw, uint32_t dst, int real) {
+    const int u = tid & 7;
+#pragma unroll
+    for (int x = 0; x < 2 * kTcRows * 8 / kThreads; ++x) {
+      const int i = (tid >> 3) + (kThreads / 8) * x, which = i / kTcRows, r = i % kTcRows;
+      uint4 w = *reinterpret_cast<const uint4*>(raw + i * kHeadDim + u * 16);
+      const float s = e8m0_to_float(raw[2 * kTcRows * kHeadDim + i * kKvHeads + h]);
+      const float2 f = make_float2(s, s);
+      const uint2 p0 = dequant4(w.x, f), p1 = dequant4(w.y, f), p2 = dequant4(w.z, f), p3 = dequant4(w.w, f);
+      uint4 lo = make_uint4(p0.x, p0.y, p1.x, p1.y), hi = make_uint4(p2.x, p2.y, p3.x, p3.y);
+      if (r >= real) lo = hi = make_uint4(0, 0, 0, 0);
+      const uint32_t t = dst + which * SM::kTile;
+      // dims 16u .. + 15 are units 2u and 2u + 1; the lanes of the second half write the odd unit first (banks)
+      const bool swap = u >= 4;
+      st_shared16(t + tc_unit(r, 2 * u + swap, SM::kHalf), swap ? hi : lo);
+      st_shared16(t + tc_unit(r, 2 * u + !swap, SM::kHalf), swap ? lo : hi);
+    }
+  }
+
+  __device__ __forceinline__ bool wait(int bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, tc_wait(&bars[bar], parity, abort_flag))) return true;
+    tw_fail(a.status, abort_flag);
+    return false;
+  }
+  __device__ __forceinline__ void load_q(int seat, uint32_t dst) {
+    const int u = tid & 15, rows = (2 * a.tokens + 31) / 32 * 32;   // rows of live warps
+    for (int r0 = 0; r0 < rows; r0 += 4 * kRowStep) {
+      uint4 v[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int r = r0 + (tid >> 4) + kRowStep * x;
+        v[x] = make_uint4(0, 0, 0, 0);
+        if (r < 2 * a.tokens)
+          v[x] = __ldg(reinterpret_cast<const uint4*>(a.q + static_cast<long long>(seat) * a.q_seat +
+                                                      static_cast<long long>(r >> 1) * a.q_tok +
+                                                      (2 * h + (r & 1)) * kHeadDim) + u);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int r = r0 + (tid >> 4) + kRowStep * x;
+        if (r < SM::kQBytes / 256) st_shared16(dst + tc_unit(r, u, SM::kQBytes / 2), v[x]);
+      }
+    }
+  }
+  // The drafted rows as one tile; true when a V value was an infinity or NaN.
+  __device__ __forceinline__ bool load_draft(const TreeItem& it, uint32_t dst) {
+    const int u = tid & 15;
+    bool odd = false;
+#pragma unroll
+    for (int x0 = 0; x0 < kTcRows / kRowStep; x0 += 4) {
+      uint4 k[4], v[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int r = (tid >> 4) + kRowStep * (x0 + x);
+        k[x] = v[x] = make_uint4(0, 0, 0, 0);
+        if (r < it.drafts) {
+          const long long off = static_cast<long long>(it.seat) * a.kv_seat + static_cast<long long>(r) * a.kv_tok + h * kHeadDim;
+          k[x] = __ldg(reinterpret_cast<const uint4*>(a.k_new + off) + u);
+          v[x] = __ldg(reinterpret_cast<const uint4*>(a.v_new + off) + u);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t at = tc_unit((tid >> 4) + kRowStep * (x0 + x), u, SM::kHalf);
+        const uint4 f = make_uint4(finite_or_zero(v[x].x), finite_or_zero(v[x].y), finite_or_zero(v[x].z), finite_or_zero(v[x].w));
+        odd |= f.x != v[x].x || f.y != v[x].y || f.z != v[x].z || f.w != v[x].w;
+        st_shared16(dst + at, k[x]);
+        st_shared16(dst + SM::kTile + at, f);
+      }
+    }
+    return odd;
+  }
+};
+
+template <bool FP8, bool LARGE>
+__global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc_kernel(const __grid_constant__ TcParams p) {
+  using SM = TcSmem<FP8, LARGE>;
+  const TreeArgs& a = p.a;
+  constexpr int kSt = SM::kStages;
+  extern __shared__ __align__(1024) uint8_t tc_raw[];
+  uint8_t* smem = tc_raw + ((1024u - (smem_addr(tc_raw) & 1023u)) & 1023u);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::kBars);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::kTmemSlot);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM::kAbort);
+  volatile int* odd = reinterpret_cast<volatile int*>(smem + SM::kOdd);
+  volatile int* issued = reinterpret_cast<volatile int*>(smem + SM::kIssued);
+  const uint32_t sbase = smem_addr(smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int h = blockIdx.x & 7, share = blockIdx.x >> 3, shares = gridDim.x >> 3;
+  const int live_warps = (2 * a.tokens + 31) / 32;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be scheduled; it waits for this grid
+  if (tid == 0) {
+    for (int i = 0; i < kSt; ++i) {
+      mbar_init(&bars[SM::kFull + i], SM::kLoaders);            // one arrival per loader warp
+      mbar_init(&bars[SM::kEmpty + i], 1);
+    }
+    for (int i = 0; i < SM::kCopySlots; ++i) mbar_init(&bars[SM::kCopied + i], FP8 ? 33 : 1);   // + a lane's scales each
+    for (int i = 0; i < SM::kRawSlots; ++i) mbar_init(&bars[SM::kRawFree + i], SM::kLoaders);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars[SM::kSFull + i], 1);
+      mbar_init(&bars[SM::kPFull + i], live_warps);
+      mbar_init(&bars[SM::kPvDone + i], 1);
+    }
+    mbar_init(&bars[SM::kOFree], live_warps);
+    mbar_init(&bars[SM::kFinal], 1);
+    *abort_flag = 0;
+    for (int i = 0; i < SM::kCopyWarps; ++i) issued[i] = 0;
+    for (int i = 0; i < kTcOddSlots; ++i) odd[i] = 0;
+    if (h == 0) a.ws_span[share] = make_int2(-1, 0);
+    fence_mbar_init();
+  }
+  TreePlan P;
+  if (!tree_plan<kTcTok, kTcRows, kTcTok, SM::kThreads>(a, P, share, shares, 2 * h, 2)) return;   // nothing allocated yet
+  if (warp == SM::kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                 "r"(kTcTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int n = static_cast<int>(P.c1 - P.c0);
+  TcCursor cur = {P.w, 0, 0, 0, 0, P.first, tree_item<kTcTok, kTcRows, kTcTok>(a, P.w)};
+  tc_enter(P, cur);
+
+  if (warp >= SM::kCopyWarp) {
+    tc_copies<FP8, LARGE>(p, P, cur, smem, bars, abort_flag, issued, h, warp - SM::kCopyWarp, lane);
+  } else if (warp >= kTcLoaderWarp && warp < SM::kMmaWarp) {
+    TcLoader<FP8, LARGE> ld{a, P, sbase, smem, bars, abort_flag, h, tid - 32 * kTcLoaderWarp};
+    int last0 = -1, last1 = -1;
+    for (int k = 0; k < n; ++k)
+      if (!ld.tile(k, cur, last0, last1, odd)) break;
+  } else if (warp == SM::kMmaWarp) {
+    // one thread: S(k), then P(k - 1) V(k - 1)
+    if (lane == 0) {
+      constexpr uint32_t kIdescQK = umma_idesc_bf16(128, kTcRows, 0, 0), kIdescPV = umma_idesc_bf16(128, kHeadDim, 0, 1);
+      const uint64_t dq = sw128_desc(sbase + SM::kQ, 1024, 16), dk = sw128_desc(sbase + SM::kKv, 1024, 16);
+      const uint64_t dv = sw128_desc(sbase + SM::kKv + SM::kTile, 1024, SM::kHalf);
+      bool ok = true;
+      TcCursor pv = cur;
+      auto wait = [&](int bar, int phase) { return tc_wait(&bars[bar], static_cast<uint32_t>(phase & 1), abort_flag); };
+      for (int k = 0; k <= n && ok; ++k) {
+        if (k < n) {
+          const int stage = k % kSt;
+          tc_seek(a, P, cur, k);
+          ok = wait(SM::kFull + stage, k / kSt) && (FP8 || wait(SM::kCopied + stage, k / kSt)) &&
+               (k < 2 || wait(SM::kPvDone + (k & 1), (k - 2) >> 1));   // P(k - 2) lay where S(k) goes
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t q = dq + (cur.index & 1) * (SM::kQBytes >> 4), kk = dk + stage * (2 * SM::kTile >> 4);
+          const uint32_t t_s = tmem + 64u * static_cast<uint32_t>(k & 1);
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)
+            tc_mma(t_s, q + ((ks >> 2) * (SM::kQBytes / 2) + (ks & 3) * 32) / 16,
+                   kk + ((ks >> 2) * SM::kHalf + (ks & 3) * 32) / 16, kIdescQK, ks > 0);
+          umma_commit(&bars[SM::kSFull + (k & 1)]);
+        }
+        if (k > 0) {
+          const int p = k - 1, stage = p % kSt, b = p & 1;
+          const bool next = tc_seek(a, P, pv, p), starts = next || p == 0;
+          ok = wait(SM::kPFull + b, p >> 1) &&
+               (!next || wait(SM::kOFree, pv.index - 1));   // the last item's O has been read
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t v = dv + stage * (2 * SM::kTile >> 4);
+#pragma unroll
+          for (int ks = 0; ks < kTcRows / 16; ++ks)
+            tc_mma_tmem_a(tmem + kTcOCol, tmem + 64u * b + 8u * ks, v + ks * (2048 / 16), kIdescPV, !starts || ks > 0);
+          umma_commit(&bars[SM::kEmpty + stage]);
+          umma_commit(&bars[SM::kPvDone + b]);
+        }
+      }
+      if (!ok) tw_fail(a.status, abort_flag);
+    }
+    __syncwarp();
+  } else if (warp < live_warps) {
+    const int r = tid, tok = r >> 1;
+    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    int k = 0;
+    bool ok = true;
+    while (k < n && ok) {
+      tc_seek(a, P, cur, k);
+      const int end = cur.end;
+      unsigned long long see = 0;
+      if (tok < cur.it.drafts)
+        see = static_cast<unsigned long long>(a.mask[static_cast<long long>(cur.it.seat) * a.mask_seat + tok]) &
+              (~0ull >> (64 - cur.it.drafts));
+      float m_run = -INFINITY, l_run = 0.f;
+      for (const int k0 = k; k < end; ++k) {
+        const int b = k & 1, j = tc_chunk(cur, k);
+        ok = __all_sync(0xffffffffu, tc_wait(&bars[SM::kSFull + b], (k >> 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        float sv[2][32];
+        tmem_ld32(tmem + 64u * b + lane_base, sv[0]);
+        tmem_ld32(tmem + 64u * b + 32u + lane_base, sv[1]);
+        tc_wait_ld();
+        if (j >= cur.it.nc) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t bits = static_cast<uint32_t>(see >> (32 * u));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sv[u][i] = ((bits >> i) & 1u) ? sv[u][i] : -INFINITY;
+          }
+        } else if (cur.it.len - j * kTcRows < kTcRows) {
+          const int real = cur.it.len - j * kTcRows;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sv[u][i] = u * 32 + i < real ? sv[u][i] : -INFINITY;
+        }
+        float cm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) cm[i & 3] = fmaxf(cm[i & 3], sv[u][i]);
+        const float cmax = fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3])) * a.scale_log2;   // the scale is positive
+        const bool grow = cmax > m_run + 8.f || (m_run == -INFINITY && cmax > -INFINITY);
+        const float m_new = grow ? cmax : m_run;
+        const float alpha = grow ? ex2_approx(m_run - m_new) : 1.f;
+        const float mm = m_new == -INFINITY ? 0.f : m_new;
+        const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(-mm, -mm);
+        float2 ls2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t pk[32];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float2 x = __ffma2_rn(make_float2(sv[u][i], sv[u][i + 1]), sc2, nm2);
+            const float2 pp = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            ls2[(i >> 1) & 3] = __fadd2_rn(ls2[(i >> 1) & 3], pp);
+            pk[u * 16 + i / 2] = pack_bf16x2(pp.x, pp.y);
+          }
+        const float2 ls = __fadd2_rn(__fadd2_rn(ls2[0], ls2[1]), __fadd2_rn(ls2[2], ls2[3]));
+        l_run = l_run * alpha + (ls.x + ls.y);
+        m_run = m_new;
+        if (k > k0 && __any_sync(0xffffffffu, alpha != 1.f)) {   // the item's first tile starts O from zero
+          ok = __all_sync(0xffffffffu, tc_wait(&bars[SM::kPvDone + ((k - 1) & 1)], ((k - 1) >> 1) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float ov[32];
+            tmem_ld32(tmem + kTcOCol + lane_base + c * 32, ov);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ov[i] *= alpha;
+            tmem_st32(tmem + kTcOCol + lane_base + c * 32, ov);
+          }
+          tc_wait_st();
+        }
+        tmem_st32u(tmem + 64u * b + lane_base, pk);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[SM::kPFull + b]);
+      }
+      if (ok) ok = __all_sync(0xffffffffu, tc_wait(&bars[SM::kPvDone + ((k - 1) & 1)], ((k - 1) >> 1) & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      // ---- the item's rows: written when it is complete here, else left as a partial (slot 2 share + 1: it starts here
+      // and goes on; 2 share: it came in from the share before)
+      const bool from_before = cur.first < P.c0, goes_on = cur.first + cur.it.n > P.c1;
+      const int slot = from_before ? 2 * share : (goes_on ? 2 * share + 1 : -1);
+      const bool mine = r < 2 * a.tokens;
+      const bool none = l_run == 0.f || (a.draft_lens != nullptr && tok >= cur.it.drafts);
+      const float inv = none ? 0.f : 1.f / l_run;
+      const unsigned long long fix = !goes_on && odd[cur.index % kTcOddSlots] == cur.index + 1 ? see : 0ull;
+      const long long col = (static_cast<long long>(max(slot, 0)) * kKvHeads + h) * (2 * a.tokens) + r;
+      __nv_bfloat16* dst = a.out + static_cast<long long>(cur.it.seat) * a.out_seat +
+                           static_cast<long long>(mine ? tok : 0) * a.out_tok + (2 * h + (r & 1)) * kHeadDim;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float ov[32];
+        tmem_ld32(tmem + kTcOCol + lane_base + c * 32, ov);
+        tc_wait_ld();
+        for (unsigned long long v = fix; v != 0; v &= v - 1) {   // infinities and NaN of drafted rows this row sees
+          const __nv_bfloat16* src = a.v_new + static_cast<long long>(cur.it.seat) * a.kv_seat +
+                                     static_cast<long long>(__ffsll(v) - 1) * a.kv_tok + h * kHeadDim + c * 32;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float x = __bfloat162float(src[i]);
+            if (!(fabsf(x) < INFINITY)) ov[i] += x;
+          }
+        }
+        if (mine && slot < 0) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 w;
+            w.x = pack_bf16x2(ov[i] * inv, ov[i + 1] * inv);
+            w.y = pack_bf16x2(ov[i + 2] * inv, ov[i + 3] * inv);
+            w.z = pack_bf16x2(ov[i + 4] * inv, ov[i + 5] * inv);
+            w.w = pack_bf16x2(ov[i + 6] * inv, ov[i + 7] * inv);
+            *reinterpret_cast<uint4*>(dst + c * 32 + i) = none ? make_uint4(0, 0, 0, 0) : w;
+          }
+        } else if (mine) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(a.ws_o + col * kHeadDim + c * 32 + i) = make_float4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
+        }
+        __syncwarp();   // the TMEM loads are the whole warp's
+      }
+      if (slot >= 0 && mine) *reinterpret_cast<float2*>(a.ws_ml + 2 * col) = make_float2(m_run, l_run);
+      if (slot == 2 * share + 1 && h == 0 && tid == 0)
+        a.ws_span[share] = make_int2(cur.w, tree_last_share(P, cur.first + cur.it.n - 1));
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[SM::kOFree]);
+    }
+    if (!ok && lane == 0) tw_fail(a.status, abort_flag);
+  }
+
+  // ------------------------------------------------------------------ teardown
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && tid == SM::kMmaWarp * 32) {   // let MMAs and copies in flight finish (bounded)
+    umma_commit(&bars[SM::kFinal]);
+    mbar_wait_bounded(&bars[SM::kFinal], 0, 200000000ull);
+    int top = 0;
+    for (int i = 0; i < SM::kCopyWarps; ++i) top = max(top, issued[i]);
+    for (int k = max(top - SM::kCopySlots - SM::kCopyWarps, 0); k < top; ++k)
+      if (k < issued[k % SM::kCopyWarps])
+        mbar_wait_bounded(&bars[SM::kCopied + k % SM::kCopySlots], (k / SM::kCopySlots) & 1, 200000000ull);
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == SM::kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTcTmemCols));
+}
+
+// A pool as rows of 1024 elements, read 128 bytes x box_rows rows at a time. bf16: 128-byte swizzle.
+template <bool FP8>
+bool make_pool_map(CUtensorMap* m, const void* base, long long rows, int box_rows) {
+  const EncodeTiled enc = tensor_map_encoder();
+  if (!enc || rows > (1ll << 31) - 1) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(kKvHeads * kHeadDim), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(FP8 ? kRowBytes / 2 : kRowBytes)};
+  const cuuint32_t box[2] = {FP8 ? 128u : 64u, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1u, 1u};
+  return enc(m, FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
+             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, FP8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+             FP8 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool FP8, bool LARGE>
+cudaError_t launch_tc(const TreeArgs& a, int grid, cudaStream_t stream) {
+  auto kern = paged_tree_tc_kernel<FP8, LARGE>;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (configured_device != dev) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<FP8, LARGE>::kAlloc);
+    if (e != cudaSuccess) return e;
+    configured_device = dev;
+  }
+  TcParams p;
+  memset(&p, 0, sizeof(p));
+  p.a = a;
+  const long long rows = static_cast<long long>(a.num_pages) * a.page_size;
+  p.box_rows = a.page_size & -a.page_size;
+  if (p.box_rows > kTcRows) p.box_rows = kTcRows;
+  if (!make_pool_map<FP8>(&p.k, a.k_pool, rows, p.box_rows) || !make_pool_map<FP8>(&p.v, a.v_pool, rows, p.box_rows))
+    return cudaErrorInvalidValue;
+  kern<<<grid, TcSmem<FP8, LARGE>::kThreads, TcSmem<FP8, LARGE>::kAlloc, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_paged_tree_tc(const TreeArgs& a, int shares, cudaStream_t stream) {
+  const bool large = a.tokens > 32;
+  const int grid = shares * kKvHeads;
+  if (a.k_scale != nullptr) return large ? launch_tc<true, true>(a, grid, stream) : launch_tc<true, false>(a, grid, stream);
+  return large ? launch_tc<false, true>(a, grid, stream) : launch_tc<false, false>(a, grid, stream);
+}
+
+}  // namespace q3

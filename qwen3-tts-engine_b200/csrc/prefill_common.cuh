@@ -1,4 +1,4 @@
-// Device helpers shared by the prefill kernels (prefill.cu, prefill_tma.cu): tcgen05 MMA issue, commit and fences,
+// Device helpers shared by the tcgen05 kernels (prefill.cu, prefill_tma.cu, paged_tree_tc.cu): tcgen05 MMA issue, commit and fences,
 // TMEM loads and stores, UMMA shared-memory and instruction descriptors, and the per-sequence geometry of a prefill
 // call (which query rows, new key rows and cached prefix keys a sequence owns).
 #pragma once
@@ -16,6 +16,17 @@ __device__ __forceinline__ uint64_t umma_smem_desc(uint32_t addr, uint32_t lbo, 
   d |= static_cast<uint64_t>((sbo >> 4) & 0x3fff) << 32;
   d |= static_cast<uint64_t>(1) << 46;                       // descriptor version for sm_100
   return d;                                                  // base offset 0, lbo mode 0, layout type 0 (no swizzle)
+}
+
+// UMMA shared-memory descriptor of a 128-byte-swizzled operand: 8-row groups `sbo` bytes apart; `lbo` = the distance
+// between 64-element column blocks for an MN-major operand (unused, 16, for K-major).
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t sbo, uint32_t lbo) {
+  uint64_t d = static_cast<uint64_t>((addr >> 4) & 0x3fff);
+  d |= static_cast<uint64_t>((lbo >> 4) & 0x3fff) << 16;
+  d |= static_cast<uint64_t>((sbo >> 4) & 0x3fff) << 32;
+  d |= static_cast<uint64_t>(1) << 46;        // descriptor version for sm_100
+  d |= static_cast<uint64_t>(2) << 61;        // layout: 128-byte swizzle
+  return d;
 }
 
 // Instruction descriptor of kind::f16: bf16 A and B, fp32 D, M x N, A/B major-ness (0 = K-major, 1 = MN-major).
@@ -110,6 +121,25 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) 
         "r"(__float_as_uint(v[26])), "r"(__float_as_uint(v[27])), "r"(__float_as_uint(v[28])),
         "r"(__float_as_uint(v[29])), "r"(__float_as_uint(v[30])), "r"(__float_as_uint(v[31]))
       : "memory");
+}
+
+// Wait for phase `parity` of `bar`; false after 2 s or once another role has raised the abort flag.
+__device__ __forceinline__ bool tw_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+#pragma unroll 1
+  for (int i = 0; i < 1024; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+#pragma unroll 1
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (global_timer_ns() - t0 > 2000000000ull) return false;
+  }
+}
+
+__device__ __forceinline__ void tw_fail(uint32_t* status, volatile int* abort_flag) {
+  atomicOr(status, kStatusWaitTimeout);
+  *abort_flag = 1;
 }
 
 struct PfSeq {

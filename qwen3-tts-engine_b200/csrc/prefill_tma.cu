@@ -76,17 +76,6 @@ struct PfTmaParams {
   int pool_maps;     // tkp / tvp are valid
 };
 
-// UMMA shared-memory descriptor of a 128-byte-swizzled operand: 8-row groups `sbo` bytes apart; `lbo` = the distance
-// between 64-element column blocks for an MN-major operand (unused, 16, for K-major).
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t sbo, uint32_t lbo) {
-  uint64_t d = static_cast<uint64_t>((addr >> 4) & 0x3fff);
-  d |= static_cast<uint64_t>((lbo >> 4) & 0x3fff) << 16;
-  d |= static_cast<uint64_t>((sbo >> 4) & 0x3fff) << 32;
-  d |= static_cast<uint64_t>(1) << 46;        // descriptor version for sm_100
-  d |= static_cast<uint64_t>(2) << 61;        // layout: 128-byte swizzle
-  return d;
-}
-
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
@@ -115,25 +104,6 @@ __device__ __forceinline__ int new_tiles_of(const PfSeq& s, int q, int causal) {
   const int L = s.P + s.Nn, shift = L - s.R;
   const int key_end = causal ? min(L, shift + min(s.R - 1, q * 64 + 63) + 1) : L;
   return (max(key_end - s.P, 0) + 63) / 64;
-}
-
-// Wait for phase `parity` of `bar`; false after 2 s or once another role has raised the abort flag.
-__device__ __forceinline__ bool tw_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-#pragma unroll 1
-  for (int i = 0; i < 1024; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_timer_ns();
-#pragma unroll 1
-  while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*abort_flag) return false;
-    if (global_timer_ns() - t0 > 2000000000ull) return false;
-  }
-}
-
-__device__ __forceinline__ void tw_fail(uint32_t* status, volatile int* abort_flag) {
-  atomicOr(status, kStatusWaitTimeout);
-  *abort_flag = 1;
 }
 
 // The page writes of a chunked prefill (write_kv) for KV head h: new rows [r0, r1) of the sequence go to positions

@@ -118,21 +118,24 @@ struct TreeArgs {
   const int32_t* block_table;
   long long bt_stride;
   int max_pages, num_pages, page_size;
+  int page_shift;                  // log2(page_size), or -1
   int B, tokens, groups;           // groups of tokens per seat (set from the workspace layout)
   float scale_log2;
   __nv_bfloat16* out;              // [B, tokens, 16, 128]
   long long out_seat, out_tok;
-  int2* ws_span;                   // [grid] (item that starts in the CTA and goes on, its last CTA), item -1: none
-  float* ws_ml;                    // [2 grid slots][8 heads][2 tok columns] (maximum, sum)
+  int2* ws_span;                   // [shares] (item that starts in the share and goes on, its last share), item -1: none
+  float* ws_ml;                    // [2 shares slots][8 heads][2 tok columns] (maximum, sum)
   float* ws_o;                     // the same columns' [128] fp32 outputs
   uint32_t* status;
 };
 struct TreeWorkspace {
-  int grid, groups;
+  bool tc;                         // the tcgen05 kernel (paged_tree_tc.cu)
+  int tok, groups, shares;         // tokens per group, groups per seat, shares of the chunk list
   size_t span, ml, o, bytes;       // byte offsets, total
 };
-TreeWorkspace tree_workspace(bool fp8, int batch, int tokens, int num_sms);
+TreeWorkspace tree_workspace(bool fp8, int tokens, float scale, int num_sms);
 cudaError_t launch_paged_tree(const TreeArgs& a, const TreeWorkspace& w, cudaStream_t stream);
+cudaError_t launch_paged_tree_tc(const TreeArgs& a, int shares, cudaStream_t stream);
 
 struct PrefixCopyArgs {
   const __nv_bfloat16* k_src;      // row (l, slot, r) at l * src_layer_stride + slot * src_slot_stride + r * row_elems
