@@ -76,12 +76,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// Two e4m3 bytes (the low 16 bits) as packed fp16, exact.
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t x) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(x & 0xffffu), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
-}
-
 __device__ __forceinline__ uint32_t pack_half2_rn(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -110,8 +104,8 @@ struct TreeState {
   uint32_t q[NT][8][2];    // B fragments of Q^T: for k-step s the four dims key_dim(t, s) .. + 3 of column g
   float cf[NT][2];         // score factor of the lane's columns
   float o[NT][8][4];
-  float m[NT][2];          // maximum that the outputs are relative to (FP8: of s + ev; else of s), the same in all g
-  float ms[NT][2];         // FP8: this lane's maximum of s, which l is relative to
+  float nm[NT][2];         // minus the maximum that the outputs are relative to (FP8: of s + ev; else of s); +inf: none
+  float ns[NT][2];         // FP8: minus the maximum of s that l is relative to
   float l[NT][2];          // this lane's part of the sum
 };
 
@@ -162,7 +156,7 @@ __device__ __forceinline__ void tree_begin(const TreeArgs& a, const TreeItem& it
     st.cf[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      st.m[nt][k] = st.ms[nt][k] = -INFINITY;
+      st.nm[nt][k] = st.ns[nt][k] = INFINITY;
       st.l[nt][k] = 0.f;
     }
 #pragma unroll
@@ -172,115 +166,142 @@ __device__ __forceinline__ void tree_begin(const TreeArgs& a, const TreeItem& it
   }
 }
 
-// One tile's scores (s: rows g and g + 8 of columns 2t, 2t + 1, masked ones -inf) into the running state; returns the
-// P^T fragments of the tile. ev: the V exponents of keys g and g + 8 (FP8 cache rows; 0 for drafted rows).
-template <bool FP8, int NT, bool HALF_P>
-__device__ __forceinline__ void tree_softmax(TreeState<FP8, NT>& st, float (&s)[NT][4], float ev0, float ev1,
-                                             uint32_t (&pf)[NT][2], float (&p)[NT][4]) {
-  float alpha[NT][2];
-  bool moved = false;
+// The fp32 products of one tile (acc: keys g and g + 8 of columns 2t, 2t + 1) into the running state; returns the P^T
+// fragments and the probabilities. k0, k1: score factors of the two keys; ev0, ev1: their V exponents (FP8 cache rows; 1
+// and 0 for others). MASKED: hide[nt] bit 0 / 1 set: the lane's token does not see key g / g + 8.
+// The maxima are lazy: they move when some score passes one by more than 2^8 (or comes first: +inf - the initial
+// maximum), which is voted on and rare, so a tile has no exchange between lanes and no rescaling.
+template <bool FP8, int NT, bool HALF_P, bool MASKED>
+__device__ __forceinline__ void tree_softmax(TreeState<FP8, NT>& st, const float (&acc)[NT][4], float k0, float k1,
+                                             float ev0, float ev1, const uint32_t (&hide)[NT], uint32_t (&pf)[NT][2],
+                                             float (&p)[NT][4]) {
+  float x[NT][4], top = -INFINITY;   // p: s + ev against nm; x: s against ns
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float s0 = s[nt][k], s1 = s[nt][2 + k];
-      const float w0 = FP8 ? s0 + ev0 : s0, w1 = FP8 ? s1 + ev1 : s1;
-      const float old = st.m[nt][k];
-      const float mn = fmaxf(old, max_over_rows(fmaxf(w0, w1)));
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      alpha[nt][k] = exp2f(old - ref);
-      moved |= old != mn;
-      st.m[nt][k] = mn;
-      p[nt][k] = exp2f(w0 - ref);
-      p[nt][2 + k] = exp2f(w1 - ref);
+    for (int k = 0; k < 4; ++k) {
+      const float f = HALF_P ? (k < 2 ? k0 : k1) * st.cf[nt][k & 1] : st.cf[nt][k & 1];
+      const bool hidden = MASKED && ((hide[nt] >> (k >> 1)) & 1u);
+      p[nt][k] = fmaf(acc[nt][k], f, HALF_P ? st.nm[nt][k & 1] + (k < 2 ? ev0 : ev1) : st.nm[nt][k & 1]);
+      if (hidden) p[nt][k] = -INFINITY;
+      top = fmaxf(top, p[nt][k]);
       if (FP8) {
-        const float so = st.ms[nt][k], sn = fmaxf(so, fmaxf(s0, s1));
-        const float sref = sn == -INFINITY ? 0.f : sn;
-        st.ms[nt][k] = sn;
-        st.l[nt][k] = st.l[nt][k] * exp2f(so - sref) + exp2f(s0 - sref) + exp2f(s1 - sref);
-      } else {
-        st.l[nt][k] = st.l[nt][k] * alpha[nt][k] + p[nt][k] + p[nt][2 + k];
+        x[nt][k] = fmaf(acc[nt][k], f, st.ns[nt][k & 1]);
+        if (hidden) x[nt][k] = -INFINITY;
+        top = fmaxf(top, x[nt][k]);
       }
     }
-  if (__any_sync(0xffffffffu, moved)) {
+  if (__any_sync(0xffffffffu, top > 8.f)) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int mt = 0; mt < 8; ++mt) {
-        st.o[nt][mt][0] *= alpha[nt][0];
-        st.o[nt][mt][1] *= alpha[nt][1];
-        st.o[nt][mt][2] *= alpha[nt][0];
-        st.o[nt][mt][3] *= alpha[nt][1];
+      for (int c = 0; c < 2; ++c) {
+        float s[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float f = HALF_P ? (r ? k1 : k0) * st.cf[nt][c] : st.cf[nt][c];
+          s[r] = MASKED && ((hide[nt] >> r) & 1u) ? -INFINITY : acc[nt][2 * r + c] * f;
+        }
+        const float w0 = HALF_P ? s[0] + ev0 : s[0], w1 = HALF_P ? s[1] + ev1 : s[1];
+        const float mw = max_over_rows(fmaxf(w0, w1));
+        float ref = st.nm[nt][c];
+        if (mw + ref > 8.f) {   // uniform over the lanes of a column
+          const float alpha = tree_exp2(-ref - mw);   // 0 at first
+          ref = st.nm[nt][c] = -mw;
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {
+            st.o[nt][mt][c] *= alpha;
+            st.o[nt][mt][2 + c] *= alpha;
+          }
+          if (!FP8) st.l[nt][c] *= alpha;
+        }
+        if (ref == INFINITY) ref = 0.f;               // nothing seen yet
+        p[nt][c] = w0 + ref;
+        p[nt][2 + c] = w1 + ref;
+        if (FP8) {
+          const float ms = max_over_rows(fmaxf(s[0], s[1]));
+          float rs = st.ns[nt][c];
+          if (ms + rs > 8.f) {
+            st.l[nt][c] *= tree_exp2(-rs - ms);
+            rs = st.ns[nt][c] = -ms;
+          }
+          if (rs == INFINITY) rs = 0.f;
+          x[nt][c] = s[0] + rs;
+          x[nt][2 + c] = s[1] + rs;
+        }
       }
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      p[nt][k] = tree_exp2(p[nt][k]);
+      st.l[nt][k & 1] += FP8 ? tree_exp2(x[nt][k]) : p[nt][k];
+    }
     pf[nt][0] = transpose8(HALF_P ? pack_half2_rn(p[nt][0], p[nt][1]) : pack_bf16x2(p[nt][0], p[nt][1]));
     pf[nt][1] = transpose8(HALF_P ? pack_half2_rn(p[nt][2], p[nt][3]) : pack_bf16x2(p[nt][2], p[nt][3]));
   }
 }
 
-// 16 cached e4m3 rows (the first `rows` real).
-template <int NT>
+// The exponent of an E8M0 byte as a float (NaN for 255).
+__device__ __forceinline__ float e8m0_exponent(uint32_t s) {
+  return s == 255u ? NAN : __uint_as_float(0x4b000000u | s) - (8388608.f + 127.f);
+}
+
+// 16 cached e4m3 rows; TAIL: only the first `rows` are real, what follows them is stale.
+template <int NT, bool TAIL>
 __device__ __forceinline__ void tree_tile_e4m3(TreeState<true, NT>& st, const uint8_t* stage, int h, int lane, int rows) {
   using SL = TreeStage<true>;
   const int g = lane >> 2, t = lane & 3;
-  float s[NT][4];
+  const uint8_t* kr = stage + g * SL::kKStride + h * kHeadDim + t * 32;
+  const uint8_t* sc = stage + SL::kScales + g * kKvHeads + h;
+  const uint32_t s0 = sc[0], s1 = sc[8 * kKvHeads], e0 = sc[16 * kKvHeads], e1 = sc[24 * kKvHeads];
+  float acc[NT][4];
   {
-    const uint8_t* kr = stage + g * SL::kKStride + h * kHeadDim + t * 32;
     uint4 w[4];
     w[0] = *reinterpret_cast<const uint4*>(kr);
-    w[1] = *reinterpret_cast<const uint4*>(kr + 16);
-    w[2] = *reinterpret_cast<const uint4*>(kr + 8 * SL::kKStride);
+    w[1] = *reinterpret_cast<const uint4*>(kr + 8 * SL::kKStride);
+    w[2] = *reinterpret_cast<const uint4*>(kr + 16);
     w[3] = *reinterpret_cast<const uint4*>(kr + 8 * SL::kKStride + 16);
-    float acc[2][NT][4] = {};
+    float part[2][NT][4] = {};
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-      const uint32_t r0 = word4(w[x >> 2], x & 3), r1 = word4(w[2 + (x >> 2)], x & 3);
-      const uint32_t af[4] = {e4m3x2_to_half2(r0), e4m3x2_to_half2(r1), e4m3x2_to_half2(r0 >> 16),
-                              e4m3x2_to_half2(r1 >> 16)};
+      uint32_t af[4];
+      e4m3x4_to_half2(word4(w[2 * (x >> 2)], x & 3), af[0], af[2]);
+      e4m3x4_to_half2(word4(w[2 * (x >> 2) + 1], x & 3), af[1], af[3]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma16816(acc[x & 1][nt], af, st.q[nt][x][0], st.q[nt][x][1], __half());
+      for (int nt = 0; nt < NT; ++nt) mma16816(part[x & 1][nt], af, st.q[nt][x][0], st.q[nt][x][1], __half());
     }
-    const float k0 = e8m0_to_float(stage[SL::kScales + g * kKvHeads + h]);
-    const float k1 = e8m0_to_float(stage[SL::kScales + (g + 8) * kKvHeads + h]);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        s[nt][k] = (acc[0][nt][k] + acc[1][nt][k]) * ((k < 2 ? k0 : k1) * st.cf[nt][k & 1]);
+      for (int k = 0; k < 4; ++k) acc[nt][k] = part[0][nt][k] + part[1][nt][k];
   }
-  const uint32_t e0 = stage[SL::kScales + (kTreeRows + g) * kKvHeads + h];
-  const uint32_t e1 = stage[SL::kScales + (kTreeRows + g + 8) * kKvHeads + h];
-  const float ev0 = e0 == 255u ? NAN : static_cast<float>(e0) - 127.f;
-  const float ev1 = e1 == 255u ? NAN : static_cast<float>(e1) - 127.f;
   uint4 v[4];   // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 16 g .. + 15
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     v[k] = *reinterpret_cast<const uint4*>(stage + SL::kV + (2 * t + (k & 1) + 8 * (k >> 1)) * SL::kVStride +
                                            h * kHeadDim + g * 16);
-  float e[2] = {ev0, ev1};
-  if (rows < kTreeRows) {   // the rows behind the last token are stale: no score, no scale, no value
+  float ev0 = e8m0_exponent(e0), ev1 = e8m0_exponent(e1);
+  uint32_t hide[NT];
+  if (TAIL) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (g + 8 * (k >> 1) >= rows) s[nt][k] = -INFINITY;
-    if (g >= rows) e[0] = 0.f;
-    if (g + 8 >= rows) e[1] = 0.f;
+    for (int nt = 0; nt < NT; ++nt) hide[nt] = (g >= rows ? 1u : 0u) | (g + 8 >= rows ? 2u : 0u);
+    if (g >= rows) ev0 = 0.f;
+    if (g + 8 >= rows) ev1 = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (2 * t + (k & 1) + 8 * (k >> 1) >= rows) v[k] = make_uint4(0, 0, 0, 0);
   }
   uint32_t pf[NT][2];
   float p[NT][4];
-  tree_softmax<true, NT, true>(st, s, e[0], e[1], pf, p);
+  tree_softmax<true, NT, true, TAIL>(st, acc, e8m0_to_float(s0), e8m0_to_float(s1), ev0, ev1, hide, pf, p);
 #pragma unroll
   for (int mt = 0; mt < 8; ++mt) {
     const uint32_t sel = (mt & 1) ? 0x7362u : 0x5140u;   // the two dims' bytes of both keys: (dim 0: k, k'), (dim 1: k, k')
-    const uint32_t x = __byte_perm(word4(v[0], mt >> 1), word4(v[1], mt >> 1), sel);
-    const uint32_t y = __byte_perm(word4(v[2], mt >> 1), word4(v[3], mt >> 1), sel);
-    const uint32_t af[4] = {e4m3x2_to_half2(x), e4m3x2_to_half2(x >> 16), e4m3x2_to_half2(y), e4m3x2_to_half2(y >> 16)};
+    uint32_t af[4];
+    e4m3x4_to_half2(__byte_perm(word4(v[0], mt >> 1), word4(v[1], mt >> 1), sel), af[0], af[1]);
+    e4m3x4_to_half2(__byte_perm(word4(v[2], mt >> 1), word4(v[3], mt >> 1), sel), af[2], af[3]);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) mma16816(st.o[nt][mt], af, pf[nt][0], pf[nt][1], __half());
   }
@@ -292,9 +313,9 @@ __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {   // infinities 
   return w;
 }
 
-// A tile of bf16 rows: 16 cached ones, or drafted ones (DRAFT: 16, or 8 in the e4m3 kernel's stages), the first `rows`
-// real; see[nt]: bit j set when the lane's token of tile nt sees row j (DRAFT).
-template <bool FP8, int NT, bool DRAFT>
+// A tile of bf16 rows: 16 cached ones (TAIL: the first `rows` real, what follows them stale), or drafted ones (DRAFT: 16,
+// or 8 in the e4m3 kernel's stages, the first `rows` real; see[nt]: bit j set when the lane's token of tile nt sees row j).
+template <bool FP8, int NT, bool TAIL, bool DRAFT>
 __device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uint8_t* stage, int h, int lane, int rows,
                                                const uint32_t (&see)[NT]) {
   using SL = TreeStage<FP8>;
@@ -302,10 +323,10 @@ __device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uin
   constexpr int kKS = DRAFT ? SL::kDraftKStride : SL::kKStride, kVS = DRAFT ? SL::kDraftVStride : SL::kVStride;
   static_assert(DRAFT || !FP8, "an e4m3 cache's rows have their own tile");
   const int g = lane >> 2, t = lane & 3;
-  float s[NT][4];
+  float acc[NT][4];
   {
     const uint8_t* kr = stage + g * kKS + h * kHeadBytes;
-    float acc[2][NT][4] = {};
+    float part[2][NT][4] = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int off = 2 * key_dim<FP8>(t, 2 * i);   // eight dims: k-steps 2i and 2i + 1
@@ -323,14 +344,14 @@ __device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uin
             b0 = pack_bf16x2(f0.x, f0.y);
             b1 = pack_bf16x2(f1.x, f1.y);
           }
-          mma16816(acc[x][nt], af, b0, b1, __nv_bfloat16());
+          mma16816(part[x][nt], af, b0, b1, __nv_bfloat16());
         }
       }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s[nt][k] = (acc[0][nt][k] + acc[1][nt][k]) * st.cf[nt][k & 1];
+      for (int k = 0; k < 4; ++k) acc[nt][k] = part[0][nt][k] + part[1][nt][k];
   }
   uint4 v[4][2];   // keys 2t, 2t + 1, 2t + 8, 2t + 9: the lane's 16 dims
 #pragma unroll
@@ -342,14 +363,15 @@ __device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uin
       v[k][i] = key < kKeys ? *reinterpret_cast<const uint4*>(vr + 2 * row_dim<FP8>(g, 4 * i)) : make_uint4(0, 0, 0, 0);
   }
   bool odd = false;   // DRAFT: a value that must not meet a zero probability
-  if (DRAFT || rows < kTreeRows) {
+  uint32_t hide[NT];
+  if (DRAFT || TAIL) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      hide[nt] = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int key = g + 8 * (k >> 1);
-        if (key >= rows || (DRAFT && !((see[nt] >> key) & 1u))) s[nt][k] = -INFINITY;
-      }
+      for (int r = 0; r < 2; ++r)
+        if (g + 8 * r >= rows || (DRAFT && !((see[nt] >> (g + 8 * r)) & 1u))) hide[nt] |= 1u << r;
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const bool real = 2 * t + (k & 1) + 8 * (k >> 1) < rows;
@@ -367,7 +389,7 @@ __device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uin
   }
   uint32_t pf[NT][2];
   float p[NT][4];
-  tree_softmax<FP8, NT, false>(st, s, 0.f, 0.f, pf, p);
+  tree_softmax<FP8, NT, false, DRAFT || TAIL>(st, acc, 1.f, 1.f, 0.f, 0.f, hide, pf, p);
 #pragma unroll
   for (int mt = 0; mt < 8; ++mt) {
     const uint32_t a0 = word4(v[0][mt >> 2], mt & 3), a1 = word4(v[1][mt >> 2], mt & 3);
@@ -420,16 +442,10 @@ __device__ __forceinline__ void tree_finish(const TreeArgs& a, const TreeItem& i
     float r[2], mx[2], l[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      if (FP8) {
-        mx[k] = max_over_rows(st.ms[nt][k]);
-        const float ref = mx[k] == -INFINITY ? 0.f : mx[k];
-        l[k] = sum_over_rows(st.l[nt][k] * exp2f(st.ms[nt][k] - ref));
-        r[k] = st.m[nt][k] == -INFINITY ? 1.f : exp2f(st.m[nt][k] - ref);
-      } else {
-        mx[k] = st.m[nt][k];
-        l[k] = sum_over_rows(st.l[nt][k]);
-        r[k] = 1.f;
-      }
+      l[k] = sum_over_rows(st.l[nt][k]);
+      mx[k] = FP8 ? -st.ns[nt][k] : -st.nm[nt][k];
+      // outputs relative to the maximum that l is relative to
+      r[k] = FP8 && st.nm[nt][k] != INFINITY && st.ns[nt][k] != INFINITY ? exp2f(st.ns[nt][k] - st.nm[nt][k]) : 1.f;
       if (slot < 0) r[k] = (padded || l[k] == 0.f) ? 0.f : r[k] / l[k];
     }
     if (tok >= a.tokens) continue;
@@ -470,22 +486,32 @@ __device__ __forceinline__ void tree_finish(const TreeArgs& a, const TreeItem& i
 // cache also the row's eight scales. The addresses of the next chunk are looked up before the wait for a free stage.
 template <bool FP8, int TOK, int STAGES>
 __device__ __forceinline__ void tree_produce(const TreeArgs& a, const TreePlan& P, uint8_t* stages, uint64_t* full,
-                                             uint64_t* empty, volatile int* abort_flag, int lane) {
+                                             uint64_t* empty, int lane) {
   using SL = TreeStage<FP8>;
-  const int row = lane & 15, which = lane >> 4;
+  const int row = lane & 15, which = lane >> 4, n = static_cast<int>(P.c1 - P.c0);
   int w = P.w;
-  long long first = P.first;
   TreeItem it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, w);
-  long long k = 0;
-  for (long long i = P.c0; i < P.c1; ++i, ++k) {
-    while (i >= first + it.n) {
-      first += it.n;
-      it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, ++w);
-    }
-    const int j = static_cast<int>(i - first);
-    const bool draft = j >= it.nc;
-    const int r0 = draft ? (j - it.nc) * SL::kDraftRows : j * kTreeRows;
-    const int rows = draft ? min(SL::kDraftRows, it.drafts - r0) : min(kTreeRows, it.len - r0);
+  int j = static_cast<int>(P.c0 - P.first);   // chunk of the item
+  int page[1], rows = 0, r0 = 0;
+  bool draft = false;
+  auto warm = [&]() {   // a new item's queries into the L2 cache
+    const int toks = min(TOK, a.tokens - it.tok0);
+    for (int x = lane; x < toks * 32; x += 32)
+      prefetch_l2(a.q + static_cast<long long>(it.seat) * a.q_seat + static_cast<long long>(it.tok0 + (x >> 5)) * a.q_tok + (x & 31) * 64);
+  };
+  auto look_up = [&]() {   // asks for the table entries of chunk j of item w
+    draft = j >= it.nc;
+    r0 = draft ? (j - it.nc) * SL::kDraftRows : j * kTreeRows;
+    rows = draft ? min(SL::kDraftRows, it.drafts - r0) : min(kTreeRows, it.len - r0);
+    tree_pages<1, 1>(a, it.seat, r0 + row, draft ? 0 : it.len, page);
+  };
+  warm();
+  look_up();
+  int k = 0;
+  bool ok = true;
+  for (; k < n; ++k) {
+    const int stage = k % STAGES;
+    uint8_t* base = stages + stage * SL::kBytes;
     const uint8_t* src = nullptr;
     long long prow = 0;
     if (row < rows) {
@@ -493,40 +519,49 @@ __device__ __forceinline__ void tree_produce(const TreeArgs& a, const TreePlan& 
         src = reinterpret_cast<const uint8_t*>((which ? a.v_new : a.k_new) + static_cast<long long>(it.seat) * a.kv_seat +
                                                static_cast<long long>(r0 + row) * a.kv_tok);
       } else {
-        prow = tree_pool_row(a, it.seat, r0 + row);
+        prow = tree_row(a, page[0], r0 + row, it.len);
         src = static_cast<const uint8_t*>(which ? a.v_pool : a.k_pool) + prow * SL::kRow;
       }
     }
-    const int stage = static_cast<int>(k % STAGES);
-    uint8_t* base = stages + stage * SL::kBytes;
-    if (k >= STAGES && !mbar_wait_bounded(&empty[stage], static_cast<uint32_t>((k / STAGES - 1) & 1))) {
-      atomicOr(a.status, kStatusWaitTimeout);
-      *abort_flag = 1;
+    const bool was_draft = draft;
+    const int was_rows = rows;
+    if (k + 1 < n) {   // the next chunk's entries travel while this one waits for its stage
+      if (++j >= it.n) {
+        do it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, ++w);
+        while (it.n == 0);
+        j = 0;
+        warm();
+      }
+      look_up();
     }
-    if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
+    if (k >= STAGES && !tree_wait(&empty[stage], static_cast<uint32_t>((k / STAGES - 1) & 1))) {
+      atomicOr(a.status, kStatusWaitTimeout);
+      ok = false;
+    }
+    if (__any_sync(0xffffffffu, !ok)) break;
     fence_proxy_async_smem();
-    if (lane == 0) mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(2 * rows * (draft ? kRowBytes : SL::kRow)));
+    if (lane == 0)
+      mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(2 * was_rows * (was_draft ? kRowBytes : SL::kRow)));
     __syncwarp();
     if (src != nullptr) {
-      const int stride = draft ? (which ? SL::kDraftVStride : SL::kDraftKStride) : (which ? SL::kVStride : SL::kKStride);
-      bulk_g2s(base + which * SL::kV + row * stride, src, draft ? kRowBytes : SL::kRow, &full[stage]);
-      if (FP8 && !draft)
+      const int stride = was_draft ? (which ? SL::kDraftVStride : SL::kDraftKStride) : (which ? SL::kVStride : SL::kKStride);
+      bulk_g2s(base + which * SL::kV + row * stride, src, was_draft ? kRowBytes : SL::kRow, &full[stage]);
+      if (FP8 && !was_draft)
         cp_async8(base + SL::kScales + (which * kTreeRows + row) * kKvHeads,
                   (which ? a.v_scale : a.k_scale) + prow * kKvHeads);
     }
     if (FP8) cp_async_arrive(&full[stage]);
   }
-  // the last chunks issued may still be landing when a consumer has given up: wait for them (bounded)
-  if (*abort_flag != 0)
-    for (long long j = k > STAGES ? k - STAGES : 0; j < k; ++j)
-      mbar_wait_bounded(&full[j % STAGES], static_cast<uint32_t>((j / STAGES) & 1), 100000000ull);
+  // the last chunks issued may still be landing when this warp gives up: wait for them (bounded)
+  if (k < n)
+    for (int x = max(k - STAGES, 0); x < k; ++x)
+      mbar_wait_bounded(&full[x % STAGES], static_cast<uint32_t>((x / STAGES) & 1), 100000000ull);
 }
 
 template <bool FP8, int NT, int STAGES>
 struct TreeSmem {
   static constexpr int kBars = STAGES * TreeStage<FP8>::kBytes;
-  static constexpr int kAbort = kBars + 2 * STAGES * 8;
-  static constexpr int kBytes = kAbort + 16;
+  static constexpr int kBytes = kBars + 2 * STAGES * 8;
 };
 
 template <bool FP8, int NT, int STAGES, int MIN_CTAS>
@@ -537,7 +572,6 @@ __global__ void __launch_bounds__(kTreeThreads, MIN_CTAS) paged_tree_kernel(cons
   extern __shared__ __align__(128) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::kBars);
   uint64_t* empty = full + STAGES;
-  volatile int* abort_flag = reinterpret_cast<int*>(smem + SM::kAbort);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be scheduled; it waits for this grid
   if (tid == 0) {
@@ -545,7 +579,6 @@ __global__ void __launch_bounds__(kTreeThreads, MIN_CTAS) paged_tree_kernel(cons
       mbar_init(&full[s], FP8 ? 33 : 1);
       mbar_init(&empty[s], kTreeConsumers);
     }
-    *abort_flag = 0;
     a.ws_span[blockIdx.x] = make_int2(-1, 0);
     fence_mbar_init();
   }
@@ -553,39 +586,41 @@ __global__ void __launch_bounds__(kTreeThreads, MIN_CTAS) paged_tree_kernel(cons
   if (!tree_plan<TOK, kTreeRows, SL::kDraftRows, kTreeThreads>(a, P, blockIdx.x, gridDim.x, 0, kQHeads)) return;   // its barriers published the barrier init
 
   if (warp == kTreeConsumers) {
-    tree_produce<FP8, TOK, STAGES>(a, P, smem, full, empty, abort_flag, lane);
+    tree_produce<FP8, TOK, STAGES>(a, P, smem, full, empty, lane);
     return;
   }
-  const int h = warp, t = lane & 3, c = static_cast<int>(blockIdx.x);
+  const int h = warp, t = lane & 3, c = static_cast<int>(blockIdx.x), n = static_cast<int>(P.c1 - P.c0);
   TreeState<FP8, NT> st;
-  int w = P.w;
-  long long first = P.first, i = P.c0, k = 0;
+  int w = P.w, k = 0;
+  long long first = P.first;
   bool ok = true;
-  while (i < P.c1 && ok) {
-    TreeItem it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, w);
-    while (i >= first + it.n) {
+  TreeItem it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, w);
+  while (k < n) {
+    while (P.c0 + k >= first + it.n) {
       first += it.n;
       it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, ++w);
     }
     tree_begin<FP8, NT>(a, it, h, lane, st);
-    const long long end = first + it.n < P.c1 ? first + it.n : P.c1;
-    for (; i < end; ++i, ++k) {
-      const int stage = static_cast<int>(k % STAGES);
-      if (!mbar_wait_bounded(&full[stage], static_cast<uint32_t>((k / STAGES) & 1))) {
+    const int end = static_cast<int>(min(first + it.n, P.c1) - P.c0);
+    int j = static_cast<int>(P.c0 + k - first);
+    for (; k < end; ++k, ++j) {
+      const int stage = k % STAGES;
+      if (!tree_wait(&full[stage], static_cast<uint32_t>((k / STAGES) & 1))) {
         atomicOr(a.status, kStatusWaitTimeout);
-        *abort_flag = 1;
-      }
-      if (__any_sync(0xffffffffu, *abort_flag != 0)) {
         ok = false;
-        break;
       }
+      if (__any_sync(0xffffffffu, !ok)) break;
       const uint8_t* base = smem + stage * SL::kBytes;
-      const int j = static_cast<int>(i - first);
       uint32_t see[NT] = {};
       if (j < it.nc) {
-        const int rows = min(kTreeRows, it.len - j * kTreeRows);
-        if constexpr (FP8) tree_tile_e4m3<NT>(st, base, h, lane, rows);
-        else tree_tile_bf16<false, NT, false>(st, base, h, lane, rows, see);
+        const int rows = it.len - j * kTreeRows;
+        if constexpr (FP8) {
+          if (rows >= kTreeRows) tree_tile_e4m3<NT, false>(st, base, h, lane, kTreeRows);
+          else tree_tile_e4m3<NT, true>(st, base, h, lane, rows);
+        } else {
+          if (rows >= kTreeRows) tree_tile_bf16<false, NT, false, false>(st, base, h, lane, kTreeRows, see);
+          else tree_tile_bf16<false, NT, true, false>(st, base, h, lane, rows, see);
+        }
       } else {
         const int r0 = (j - it.nc) * SL::kDraftRows;
 #pragma unroll
@@ -595,20 +630,18 @@ __global__ void __launch_bounds__(kTreeThreads, MIN_CTAS) paged_tree_kernel(cons
             see[nt] = static_cast<uint32_t>(
                 static_cast<unsigned long long>(a.mask[static_cast<long long>(it.seat) * a.mask_seat + tok]) >> r0);
         }
-        tree_tile_bf16<FP8, NT, true>(st, base, h, lane, min(SL::kDraftRows, it.drafts - r0), see);
+        tree_tile_bf16<FP8, NT, false, true>(st, base, h, lane, min(SL::kDraftRows, it.drafts - r0), see);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[stage]);
     }
-    if (!ok) break;
+    if (k < end) break;   // a wait gave up
     // slot 2c + 1 holds the item that starts here and goes on, 2c the one that came in from the CTA before
     const bool from_before = first < P.c0, goes_on = first + it.n > P.c1;
     tree_finish<FP8, NT>(a, it, h, lane, st, from_before ? 2 * c : (goes_on ? 2 * c + 1 : -1));
-    if (!from_before && goes_on && h == 0 && lane == 0) {
-      a.ws_span[c] = make_int2(w, tree_last_share(P, first + it.n - 1));
-    }
+    if (!from_before && goes_on && h == 0 && lane == 0) a.ws_span[c] = make_int2(w, tree_last_share(P, first + it.n - 1));
   }
-  if (!ok && lane == 0)
+  if (k < n && lane == 0)
     for (int s = 0; s < STAGES; ++s)
       mbar_wait_bounded(&full[(k + s) % STAGES], static_cast<uint32_t>(((k + s) / STAGES) & 1), 100000000ull);
 }

@@ -130,7 +130,6 @@ __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async8_at(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // Byte offset of 16-byte unit c (0..15) of a row in an operand tile whose dim halves are `half` bytes apart.
 __device__ __forceinline__ uint32_t tc_unit(int row, int c, int half) {
@@ -166,8 +165,8 @@ __device__ __forceinline__ int tc_chunk(const TcCursor& c, int k) { return c.j0 
 
 // Four e4m3 bytes times f as two packed bf16 words, exact.
 __device__ __forceinline__ uint2 dequant4(uint32_t w, float2 f) {
-  const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
-  const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
+  uint32_t lo, hi;
+  e4m3x4_to_half2(w, lo, hi);
   const float2 x = __fmul2_rn(__half22float2(*reinterpret_cast<const __half2*>(&lo)), f);
   const float2 y = __fmul2_rn(__half22float2(*reinterpret_cast<const __half2*>(&hi)), f);
   return make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(y.x, y.y));
