@@ -17,41 +17,64 @@
 // one that spans CTAs leaves an fp32 partial (output, maximum, sum) per CTA, which a second small kernel adds in CTA
 // order (deterministic; it is launched with programmatic stream serialisation, so its start-up hides under the first).
 //
-// Bound: HBM. A token row holds all 8 KV heads in 2048 (1024 for e4m3) contiguous bytes. One producer warp brings the
-// rows of a chunk into a ring of shared-memory stages, a lane per row and one bulk copy each, so any page size and page
-// boundary works; eight consumer warps take one KV head each. Rows are padded by 16 (64) bytes so that the fragment
-// loads of the matrix instructions are free of bank conflicts.
+// Bound: HBM. A token row holds all 8 KV heads in 2048 (1024 for e4m3) contiguous bytes. One producer warp fills a ring of
+// shared-memory stages by TMA: R rows of all heads in one box (R = 16, or the largest power of two that divides the page
+// size, so a box never leaves its page), laid out [head or half head][R rows][128 bytes] with the 128-byte swizzle, which
+// makes the fragment loads of the matrix instructions free of bank conflicts. (One bulk copy per row and lane into padded
+// rows cost the producer 66 cycles each, 32 a chunk: 189 us on 576 seats, e4m3.) Eight consumer warps take one KV head each.
 // Scores S^T = K.Q^T and outputs O^T = V^T.P^T use mma.sync m16n8k16 with the 16 keys (dims) as the rows of A and the
 // 2 heads x 4 tokens as the 8 columns of B: with so few query columns the legacy tensor path is far below its limit.
+#include <cuda.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
+#include <cstring>
+
+#include "tensor_map.cuh"
 #include "tree_common.cuh"
 
 namespace q3 {
 
 namespace {
 
-constexpr int kTreeConsumers = kKvHeads;                  // one warp per KV head
-constexpr int kTreeThreads = (kTreeConsumers + 1) * 32;   // and a producer warp
 constexpr int kTreeRows = 16;                             // cached rows per chunk
 
-// Stage layout. bf16: K rows 2112 bytes apart (four 16-byte units more than 2048), V rows 2064. e4m3: K and V rows
-// 1040 apart, then the scales [16][8] of K and of V; drafted rows (bf16, eight per chunk) use the same bytes, 2064
-// apart.
+// Stage layout: K, V, then (e4m3) the scales [16][8] of K and of V. Cached rows as described above; drafted rows (bf16, 16
+// or, in the e4m3 kernel's stages, 8 per chunk) plainly, 2048 bytes each.
 template <bool FP8>
 struct TreeStage {
   static constexpr int kRow = FP8 ? 1024 : 2048;
-  static constexpr int kKStride = FP8 ? 1040 : 2112;
-  static constexpr int kVStride = FP8 ? 1040 : 2064;
-  static constexpr int kV = kTreeRows * kKStride;
-  static constexpr int kScales = kV + kTreeRows * kVStride;
-  static constexpr int kBytes = kScales + (FP8 ? 2 * kTreeRows * kKvHeads : 0);
+  static constexpr int kV = kTreeRows * kRow;
+  static constexpr int kScales = 2 * kV;
+  static constexpr int kBytes = kScales + (FP8 ? 1024 : 0);
   static constexpr int kDraftRows = FP8 ? 8 : 16;
-  static constexpr int kDraftKStride = FP8 ? 2064 : 2112;
-  static constexpr int kDraftVStride = 2064;
-  static_assert(kDraftRows * kDraftKStride <= kV && kV + kDraftRows * kDraftVStride <= kScales && kBytes % 16 == 0,
-                "drafted rows fit their stage");
+  static_assert(kDraftRows * kRowBytes <= kV && kBytes % 1024 == 0, "drafted rows fit their stage");
+};
+
+// Where a consumer lane's 16-byte pieces lie in a stage: K row g (unit 2t of its head's 128 bytes, or of both halves), V
+// rows 2t and 2t + 1 (unit g); rows 8 further are `eight` bytes further. The swizzle xors a 128-byte line's units with the
+// line's number.
+template <bool FP8>
+struct TreeLane {
+  uint32_t k[FP8 ? 1 : 2], v[2][FP8 ? 1 : 2], eight;
+  __device__ __forceinline__ void init(int R, int h, int g, int t) {
+    auto at = [&](int r, int half, int unit) -> uint32_t {
+      const uint32_t line = (r / R * R * TreeStage<FP8>::kRow + (FP8 ? h : 2 * h + half) * R * 128 + r % R * 128) >> 7;
+      return line * 128 + ((unit ^ (line & 7)) << 4);
+    };
+#pragma unroll
+    for (int i = 0; i < (FP8 ? 1 : 2); ++i) {
+      k[i] = at(g, i, 2 * t);
+      v[0][i] = TreeStage<FP8>::kV + at(2 * t, i, g);
+      v[1][i] = TreeStage<FP8>::kV + at(2 * t + 1, i, g);
+    }
+    eight = R == kTreeRows ? 1024 : 8 * TreeStage<FP8>::kRow;
+  }
+};
+
+struct TreeParams {
+  TreeArgs a;
+  CUtensorMap k, v;   // the pools as [heads or half heads][rows][128 bytes]
+  int box_rows;
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
@@ -111,7 +134,7 @@ struct TreeState {
 
 template <bool FP8>
 __device__ __forceinline__ int key_dim(int t, int s) {
-  return FP8 ? 32 * t + 4 * s : 32 * (s >> 1) + 8 * t + 4 * (s & 1);
+  return FP8 ? 32 * t + 4 * s : 64 * (s >> 2) + 16 * t + 4 * (s & 3);
 }
 template <bool FP8>
 __device__ __forceinline__ int row_dim(int g, int mt) {
@@ -119,13 +142,13 @@ __device__ __forceinline__ int row_dim(int g, int mt) {
 }
 
 template <bool FP8, int NT>
-__device__ __forceinline__ void tree_begin(const TreeArgs& a, const TreeItem& it, int h, int lane, TreeState<FP8, NT>& st) {
+__device__ __forceinline__ void tree_begin(const TreeArgs& a, int seat, int tok0, int h, int lane, TreeState<FP8, NT>& st) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int tok = it.tok0 + 4 * nt + (g >> 1);
+    const int tok = tok0 + 4 * nt + (g >> 1);
     const bool have = tok < a.tokens;
-    const __nv_bfloat16* src = a.q + static_cast<long long>(it.seat) * a.q_seat + static_cast<long long>(have ? tok : 0) * a.q_tok +
+    const __nv_bfloat16* src = a.q + static_cast<long long>(seat) * a.q_seat + static_cast<long long>(have ? tok : 0) * a.q_tok +
                                (2 * h + (g & 1)) * kHeadDim;
     uint32_t top = 0;
 #pragma unroll
@@ -250,19 +273,20 @@ __device__ __forceinline__ float e8m0_exponent(uint32_t s) {
 
 // 16 cached e4m3 rows; TAIL: only the first `rows` are real, what follows them is stale.
 template <int NT, bool TAIL>
-__device__ __forceinline__ void tree_tile_e4m3(TreeState<true, NT>& st, const uint8_t* stage, int h, int lane, int rows) {
+__device__ __forceinline__ void tree_tile_e4m3(TreeState<true, NT>& st, const uint8_t* stage, const TreeLane<true>& at, int h,
+                                               int lane, int rows) {
   using SL = TreeStage<true>;
   const int g = lane >> 2, t = lane & 3;
-  const uint8_t* kr = stage + g * SL::kKStride + h * kHeadDim + t * 32;
+  const uint8_t *kr = stage + at.k[0], *kx = stage + (at.k[0] ^ 16);
   const uint8_t* sc = stage + SL::kScales + g * kKvHeads + h;
   const uint32_t s0 = sc[0], s1 = sc[8 * kKvHeads], e0 = sc[16 * kKvHeads], e1 = sc[24 * kKvHeads];
   float acc[NT][4];
   {
     uint4 w[4];
     w[0] = *reinterpret_cast<const uint4*>(kr);
-    w[1] = *reinterpret_cast<const uint4*>(kr + 8 * SL::kKStride);
-    w[2] = *reinterpret_cast<const uint4*>(kr + 16);
-    w[3] = *reinterpret_cast<const uint4*>(kr + 8 * SL::kKStride + 16);
+    w[1] = *reinterpret_cast<const uint4*>(kr + at.eight);
+    w[2] = *reinterpret_cast<const uint4*>(kx);
+    w[3] = *reinterpret_cast<const uint4*>(kx + at.eight);
     float part[2][NT][4] = {};
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
@@ -277,11 +301,6 @@ __device__ __forceinline__ void tree_tile_e4m3(TreeState<true, NT>& st, const ui
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[nt][k] = part[0][nt][k] + part[1][nt][k];
   }
-  uint4 v[4];   // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 16 g .. + 15
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    v[k] = *reinterpret_cast<const uint4*>(stage + SL::kV + (2 * t + (k & 1) + 8 * (k >> 1)) * SL::kVStride +
-                                           h * kHeadDim + g * 16);
   float ev0 = e8m0_exponent(e0), ev1 = e8m0_exponent(e1);
   uint32_t hide[NT];
   if (TAIL) {
@@ -289,13 +308,20 @@ __device__ __forceinline__ void tree_tile_e4m3(TreeState<true, NT>& st, const ui
     for (int nt = 0; nt < NT; ++nt) hide[nt] = (g >= rows ? 1u : 0u) | (g + 8 >= rows ? 2u : 0u);
     if (g >= rows) ev0 = 0.f;
     if (g + 8 >= rows) ev1 = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (2 * t + (k & 1) + 8 * (k >> 1) >= rows) v[k] = make_uint4(0, 0, 0, 0);
   }
   uint32_t pf[NT][2];
   float p[NT][4];
   tree_softmax<true, NT, true, TAIL>(st, acc, e8m0_to_float(s0), e8m0_to_float(s1), ev0, ev1, hide, pf, p);
+  asm volatile("" ::: "memory");   // V is loaded now: held over the softmax it would not fit the registers
+  uint4 v[4];   // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 16 g .. + 15
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    v[k] = *reinterpret_cast<const uint4*>(stage + at.v[k & 1][0] + (k >> 1) * at.eight);
+  if (TAIL) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (2 * t + (k & 1) + 8 * (k >> 1) >= rows) v[k] = make_uint4(0, 0, 0, 0);
+  }
 #pragma unroll
   for (int mt = 0; mt < 8; ++mt) {
     const uint32_t sel = (mt & 1) ? 0x7362u : 0x5140u;   // the two dims' bytes of both keys: (dim 0: k, k'), (dim 1: k, k')
@@ -316,22 +342,23 @@ __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {   // infinities 
 // A tile of bf16 rows: 16 cached ones (TAIL: the first `rows` real, what follows them stale), or drafted ones (DRAFT: 16,
 // or 8 in the e4m3 kernel's stages, the first `rows` real; see[nt]: bit j set when the lane's token of tile nt sees row j).
 template <bool FP8, int NT, bool TAIL, bool DRAFT>
-__device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uint8_t* stage, int h, int lane, int rows,
+__device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uint8_t* stage, const TreeLane<FP8>& at, int h,
+                                               int lane, int rows,
                                                const uint32_t (&see)[NT]) {
   using SL = TreeStage<FP8>;
   constexpr int kKeys = FP8 ? 8 : 16;
-  constexpr int kKS = DRAFT ? SL::kDraftKStride : SL::kKStride, kVS = DRAFT ? SL::kDraftVStride : SL::kVStride;
   static_assert(DRAFT || !FP8, "an e4m3 cache's rows have their own tile");
   const int g = lane >> 2, t = lane & 3;
   float acc[NT][4];
   {
-    const uint8_t* kr = stage + g * kKS + h * kHeadBytes;
     float part[2][NT][4] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int off = 2 * key_dim<FP8>(t, 2 * i);   // eight dims: k-steps 2i and 2i + 1
-      const uint4 w0 = *reinterpret_cast<const uint4*>(kr + off);
-      const uint4 w1 = kKeys == 16 ? *reinterpret_cast<const uint4*>(kr + 8 * kKS + off) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) {   // eight dims: k-steps 2i and 2i + 1
+      const uint8_t* kr;
+      if constexpr (DRAFT) kr = stage + g * kRowBytes + h * kHeadBytes + 2 * key_dim<FP8>(t, 2 * i);
+      else kr = stage + (at.k[i >> 1] ^ (16 * (i & 1)));
+      const uint4 w0 = *reinterpret_cast<const uint4*>(kr);
+      const uint4 w1 = kKeys == 16 ? *reinterpret_cast<const uint4*>(kr + (DRAFT ? 8 * kRowBytes : at.eight)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const uint32_t af[4] = {x ? w0.z : w0.x, x ? w1.z : w1.x, x ? w0.w : w0.y, x ? w1.w : w1.y};
@@ -357,10 +384,13 @@ __device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uin
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int key = 2 * t + (k & 1) + 8 * (k >> 1);
-    const uint8_t* vr = stage + SL::kV + key * kVS + h * kHeadBytes;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      v[k][i] = key < kKeys ? *reinterpret_cast<const uint4*>(vr + 2 * row_dim<FP8>(g, 4 * i)) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* vr;
+      if constexpr (DRAFT) vr = stage + SL::kV + key * kRowBytes + h * kHeadBytes + 2 * row_dim<FP8>(g, 4 * i);
+      else vr = stage + at.v[k & 1][i] + (k >> 1) * at.eight;
+      v[k][i] = key < kKeys ? *reinterpret_cast<const uint4*>(vr) : make_uint4(0, 0, 0, 0);
+    }
   }
   bool odd = false;   // DRAFT: a value that must not meet a zero probability
   uint32_t hide[NT];
@@ -403,7 +433,7 @@ __device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uin
     // a drafted row holds an infinity or NaN: only the tokens that see the row take it (0 * inf would reach the others)
 #pragma unroll 1
     for (int j = 0; j < rows; ++j) {
-      const uint8_t* vr = stage + SL::kV + j * kVS + h * kHeadBytes;
+      const uint8_t* vr = stage + SL::kV + j * kRowBytes + h * kHeadBytes;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int src = 4 * (j & 7) + t;
@@ -429,15 +459,14 @@ __device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uin
 }
 
 // End of an item's chunks in this CTA. slot < 0: the item is complete and its rows are written; else its partial goes
-// to that workspace slot: outputs [8 heads][2 TOK columns][128] fp32 and (maximum, sum) pairs.
+// to that workspace slot: outputs [8 heads][cols][128] fp32 and (maximum, sum) pairs, the warp's columns from col0 on.
 template <bool FP8, int NT>
-__device__ __forceinline__ void tree_finish(const TreeArgs& a, const TreeItem& it, int h, int lane, TreeState<FP8, NT>& st,
-                                            int slot) {
-  constexpr int kCols = 8 * NT;
+__device__ __forceinline__ void tree_finish(const TreeArgs& a, const TreeItem& it, int tok0, int cols, int col0, int h, int lane,
+                                            TreeState<FP8, NT>& st, int slot) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int tok = it.tok0 + 4 * nt + t;
+    const int tok = tok0 + 4 * nt + t;
     const bool padded = a.draft_lens != nullptr && tok >= it.drafts;
     float r[2], mx[2], l[2];
 #pragma unroll
@@ -470,7 +499,7 @@ __device__ __forceinline__ void tree_finish(const TreeArgs& a, const TreeItem& i
     } else {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const long long col = (static_cast<long long>(slot) * kKvHeads + h) * kCols + 8 * nt + 2 * t + k;
+        const long long col = (static_cast<long long>(slot) * kKvHeads + h) * cols + col0 + 8 * nt + 2 * t + k;
         float* dst = a.ws_o + col * kHeadDim;
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt)
@@ -482,13 +511,16 @@ __device__ __forceinline__ void tree_finish(const TreeArgs& a, const TreeItem& i
   }
 }
 
-// The producer warp: lanes 0..15 bring the chunk's K rows, lanes 16..31 its V rows, one bulk copy each; with an e4m3
-// cache also the row's eight scales. The addresses of the next chunk are looked up before the wait for a free stage.
+// The producer warp: lane b < 16 / R brings box b of the chunk's K rows (and their scales), lane 16 + b of its V rows. The
+// table entries of the next chunk are asked for before the wait for a free stage. Drafted rows: a lane and a bulk copy each.
 template <bool FP8, int TOK, int STAGES>
-__device__ __forceinline__ void tree_produce(const TreeArgs& a, const TreePlan& P, uint8_t* stages, uint64_t* full,
+__device__ __forceinline__ void tree_produce(const TreeParams& p, const TreePlan& P, uint8_t* stages, uint64_t* full,
                                              uint64_t* empty, int lane) {
   using SL = TreeStage<FP8>;
-  const int row = lane & 15, which = lane >> 4, n = static_cast<int>(P.c1 - P.c0);
+  const TreeArgs& a = p.a;
+  const int which = lane >> 4, n = static_cast<int>(P.c1 - P.c0), R = p.box_rows;
+  const int row = (lane & 15) * R;              // cached rows: first of the lane's box (of 16: none past them)
+  const CUtensorMap* map = which ? &p.v : &p.k;
   int w = P.w;
   TreeItem it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, w);
   int j = static_cast<int>(P.c0 - P.first);   // chunk of the item
@@ -503,7 +535,7 @@ __device__ __forceinline__ void tree_produce(const TreeArgs& a, const TreePlan& 
     draft = j >= it.nc;
     r0 = draft ? (j - it.nc) * SL::kDraftRows : j * kTreeRows;
     rows = draft ? min(SL::kDraftRows, it.drafts - r0) : min(kTreeRows, it.len - r0);
-    tree_pages<1, 1>(a, it.seat, r0 + row, draft ? 0 : it.len, page);
+    tree_pages<1, 1>(a, it.seat, r0 + row, draft || row >= kTreeRows ? 0 : it.len, page);
   };
   warm();
   look_up();
@@ -513,15 +545,13 @@ __device__ __forceinline__ void tree_produce(const TreeArgs& a, const TreePlan& 
     const int stage = k % STAGES;
     uint8_t* base = stages + stage * SL::kBytes;
     const uint8_t* src = nullptr;
-    long long prow = 0;
-    if (row < rows) {
-      if (draft) {
+    int prow = -1;
+    if (draft) {
+      if ((lane & 15) < rows)
         src = reinterpret_cast<const uint8_t*>((which ? a.v_new : a.k_new) + static_cast<long long>(it.seat) * a.kv_seat +
-                                               static_cast<long long>(r0 + row) * a.kv_tok);
-      } else {
-        prow = tree_row(a, page[0], r0 + row, it.len);
-        src = static_cast<const uint8_t*>(which ? a.v_pool : a.k_pool) + prow * SL::kRow;
-      }
+                                               static_cast<long long>(r0 + (lane & 15)) * a.kv_tok);
+    } else if (row < rows) {
+      prow = static_cast<int>(tree_row(a, page[0], r0 + row, it.len));
     }
     const bool was_draft = draft;
     const int was_rows = rows;
@@ -540,17 +570,23 @@ __device__ __forceinline__ void tree_produce(const TreeArgs& a, const TreePlan& 
     }
     if (__any_sync(0xffffffffu, !ok)) break;
     fence_proxy_async_smem();
-    if (lane == 0)
-      mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(2 * was_rows * (was_draft ? kRowBytes : SL::kRow)));
-    __syncwarp();
-    if (src != nullptr) {
-      const int stride = was_draft ? (which ? SL::kDraftVStride : SL::kDraftKStride) : (which ? SL::kVStride : SL::kKStride);
-      bulk_g2s(base + which * SL::kV + row * stride, src, was_draft ? kRowBytes : SL::kRow, &full[stage]);
-      if (FP8 && !was_draft)
-        cp_async8(base + SL::kScales + (which * kTreeRows + row) * kKvHeads,
-                  (which ? a.v_scale : a.k_scale) + prow * kKvHeads);
+    if (lane == 0) {
+      const int boxes = (was_rows + R - 1) / R;   // cached: whole boxes, with their scales unless those come row by row
+      mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(was_draft ? 2 * was_rows * kRowBytes
+                                                                : 2 * boxes * R * (SL::kRow + (FP8 && R > 1 ? kKvHeads : 0))));
     }
-    if (FP8) cp_async_arrive(&full[stage]);
+    __syncwarp();
+    if (src != nullptr) bulk_g2s(base + which * SL::kV + (lane & 15) * kRowBytes, src, kRowBytes, &full[stage]);
+    if (prow >= 0) {
+      tma_load_3d(smem_addr(base) + which * SL::kV + row * SL::kRow, map, 0, prow, 0, smem_addr(&full[stage]));
+      if (FP8) {
+        uint8_t* dst = base + SL::kScales + (which * kTreeRows + row) * kKvHeads;
+        const uint8_t* sc = (which ? a.v_scale : a.k_scale) + static_cast<long long>(prow) * kKvHeads;
+        if (R > 1) bulk_g2s(dst, sc, R * kKvHeads, &full[stage]);
+        else cp_async8(dst, sc);
+      }
+    }
+    if (FP8 && R == 1) cp_async_arrive(&full[stage]);
   }
   // the last chunks issued may still be landing when this warp gives up: wait for them (bounded)
   if (k < n)
@@ -558,49 +594,76 @@ __device__ __forceinline__ void tree_produce(const TreeArgs& a, const TreePlan& 
       mbar_wait_bounded(&full[x % STAGES], static_cast<uint32_t>((x / STAGES) & 1), 100000000ull);
 }
 
-template <bool FP8, int NT, int STAGES>
-struct TreeSmem {
-  static constexpr int kBars = STAGES * TreeStage<FP8>::kBytes;
-  static constexpr int kBytes = kBars + 2 * STAGES * 8;
+// One CTA per SM: STREAMS shares of the chunk list, each with a ring of STAGES stages, a producer warp (of warpgroup 0, the
+// others of which leave) and 8 WPH consumer warps; the WPH warps of a head take four tokens each of a group of 4 WPH. With
+// 16 consumer warps (640 threads at 96 registers) warpgroup 0 goes down to 32 registers and the consumers up to 112:
+// 128 x 32 + 512 x 112 = 640 x 96.
+template <bool FP8, int STREAMS, int WPH, int STAGES>
+struct TreeShape {
+  static constexpr int kConsumers = kKvHeads * WPH * STREAMS, kThreads = 128 + 32 * kConsumers;
+  static constexpr bool kMoveRegs = kConsumers == 16;
+  static constexpr int kLaunchRegs = 96, kProducerRegs = 32, kConsumerRegs = 112;
+  static_assert(kConsumers == 8 || 128 * kProducerRegs + 512 * kConsumerRegs == 640 * kLaunchRegs, "the register split");
+  static constexpr int kTok = 4 * WPH;
+  static constexpr int kStream = STAGES * TreeStage<FP8>::kBytes;
+  static constexpr int kBars = STREAMS * kStream;            // per stream: full[STAGES], empty[STAGES]
+  static constexpr int kBytes = kBars + STREAMS * 2 * STAGES * 8;
+  static constexpr int kAlloc = kBytes + 1024;               // slack to align the base to 1024 B (swizzle atoms)
+  static_assert(kAlloc + 1024 <= 232448, "shared memory");
 };
 
-template <bool FP8, int NT, int STAGES, int MIN_CTAS>
-__global__ void __launch_bounds__(kTreeThreads, MIN_CTAS) paged_tree_kernel(const TreeArgs a) {
+template <bool FP8, bool DRAFTS, int STREAMS, int WPH, int STAGES>
+__global__ void __launch_bounds__(TreeShape<FP8, STREAMS, WPH, STAGES>::kThreads, 1)
+    paged_tree_kernel(const __grid_constant__ TreeParams p) {
   using SL = TreeStage<FP8>;
-  using SM = TreeSmem<FP8, NT, STAGES>;
-  constexpr int TOK = 4 * NT;
-  extern __shared__ __align__(128) uint8_t smem[];
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::kBars);
-  uint64_t* empty = full + STAGES;
+  using SH = TreeShape<FP8, STREAMS, WPH, STAGES>;
+  const TreeArgs& a = p.a;
+  extern __shared__ __align__(1024) uint8_t tree_raw[];
+  uint8_t* smem = tree_raw + ((1024u - (smem_addr(tree_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int mine = warp < 4 ? min(warp, STREAMS - 1) : (warp - 4) / (kKvHeads * WPH);   // the warp's stream
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be scheduled; it waits for this grid
   if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], FP8 ? 33 : 1);
-      mbar_init(&empty[s], kTreeConsumers);
+    for (int s = 0; s < STREAMS; ++s) {
+      uint64_t* b = reinterpret_cast<uint64_t*>(smem + SH::kBars) + 2 * STAGES * s;
+      for (int i = 0; i < STAGES; ++i) {
+        mbar_init(&b[i], FP8 && p.box_rows == 1 ? 33 : 1);   // + each lane's scales when they come row by row
+        mbar_init(&b[STAGES + i], kKvHeads * WPH);
+      }
+      a.ws_span[STREAMS * blockIdx.x + s] = make_int2(-1, 0);
     }
-    a.ws_span[blockIdx.x] = make_int2(-1, 0);
     fence_mbar_init();
   }
   TreePlan P;
-  if (!tree_plan<TOK, kTreeRows, SL::kDraftRows, kTreeThreads>(a, P, blockIdx.x, gridDim.x, 0, kQHeads)) return;   // its barriers published the barrier init
+  if (!tree_plan<SH::kTok, kTreeRows, SL::kDraftRows, SH::kThreads, STREAMS>(a, P, STREAMS * blockIdx.x, STREAMS * gridDim.x,
+                                                                             mine, 0, kQHeads))
+    return;   // its barriers published the barrier init
+  uint8_t* stages = smem + mine * SH::kStream;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + SH::kBars) + 2 * STAGES * mine;
+  uint64_t* empty = full + STAGES;
+  const int n = static_cast<int>(P.c1 - P.c0);
 
-  if (warp == kTreeConsumers) {
-    tree_produce<FP8, TOK, STAGES>(a, P, smem, full, empty, lane);
+  if (warp < 4) {
+    if constexpr (SH::kMoveRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::kProducerRegs));
+    if (warp < STREAMS && n > 0) tree_produce<FP8, SH::kTok, STAGES>(p, P, stages, full, empty, lane);
     return;
   }
-  const int h = warp, t = lane & 3, c = static_cast<int>(blockIdx.x), n = static_cast<int>(P.c1 - P.c0);
-  TreeState<FP8, NT> st;
+  if constexpr (SH::kMoveRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::kConsumerRegs));
+  const int h = (warp - 4) % kKvHeads, sub = (warp - 4) / kKvHeads % WPH, t = lane & 3, c = STREAMS * static_cast<int>(blockIdx.x) + mine;
+  TreeState<FP8, 1> st;
+  TreeLane<FP8> at;
+  at.init(p.box_rows, h, lane >> 2, t);
   int w = P.w, k = 0;
   long long first = P.first;
   bool ok = true;
-  TreeItem it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, w);
+  TreeItem it = tree_item<SH::kTok, kTreeRows, SL::kDraftRows>(a, w);
   while (k < n) {
     while (P.c0 + k >= first + it.n) {
       first += it.n;
-      it = tree_item<TOK, kTreeRows, SL::kDraftRows>(a, ++w);
+      it = tree_item<SH::kTok, kTreeRows, SL::kDraftRows>(a, ++w);
     }
-    tree_begin<FP8, NT>(a, it, h, lane, st);
+    const int tok0 = it.tok0 + 4 * sub;   // this warp's four tokens
+    tree_begin<FP8, 1>(a, it.seat, tok0, h, lane, st);
     const int end = static_cast<int>(min(first + it.n, P.c1) - P.c0);
     int j = static_cast<int>(P.c0 + k - first);
     for (; k < end; ++k, ++j) {
@@ -610,110 +673,87 @@ __global__ void __launch_bounds__(kTreeThreads, MIN_CTAS) paged_tree_kernel(cons
         ok = false;
       }
       if (__any_sync(0xffffffffu, !ok)) break;
-      const uint8_t* base = smem + stage * SL::kBytes;
-      uint32_t see[NT] = {};
-      if (j < it.nc) {
+      const uint8_t* base = stages + stage * SL::kBytes;
+      uint32_t see[1] = {0};
+      if (!DRAFTS || j < it.nc) {
         const int rows = it.len - j * kTreeRows;
         if constexpr (FP8) {
-          if (rows >= kTreeRows) tree_tile_e4m3<NT, false>(st, base, h, lane, kTreeRows);
-          else tree_tile_e4m3<NT, true>(st, base, h, lane, rows);
+          if (rows >= kTreeRows) tree_tile_e4m3<1, false>(st, base, at, h, lane, kTreeRows);
+          else tree_tile_e4m3<1, true>(st, base, at, h, lane, rows);
         } else {
-          if (rows >= kTreeRows) tree_tile_bf16<false, NT, false, false>(st, base, h, lane, kTreeRows, see);
-          else tree_tile_bf16<false, NT, true, false>(st, base, h, lane, rows, see);
+          if (rows >= kTreeRows) tree_tile_bf16<false, 1, false, false>(st, base, at, h, lane, kTreeRows, see);
+          else tree_tile_bf16<false, 1, true, false>(st, base, at, h, lane, rows, see);
         }
-      } else {
+      } else if constexpr (DRAFTS) {
         const int r0 = (j - it.nc) * SL::kDraftRows;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int tok = it.tok0 + 4 * nt + t;
-          if (tok < it.drafts)
-            see[nt] = static_cast<uint32_t>(
-                static_cast<unsigned long long>(a.mask[static_cast<long long>(it.seat) * a.mask_seat + tok]) >> r0);
-        }
-        tree_tile_bf16<FP8, NT, false, true>(st, base, h, lane, min(SL::kDraftRows, it.drafts - r0), see);
+        if (tok0 + t < it.drafts)
+          see[0] = static_cast<uint32_t>(
+              static_cast<unsigned long long>(a.mask[static_cast<long long>(it.seat) * a.mask_seat + tok0 + t]) >> r0);
+        tree_tile_bf16<FP8, 1, false, true>(st, base, at, h, lane, min(SL::kDraftRows, it.drafts - r0), see);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[stage]);
     }
     if (k < end) break;   // a wait gave up
-    // slot 2c + 1 holds the item that starts here and goes on, 2c the one that came in from the CTA before
+    // slot 2c + 1 holds the item that starts here and goes on, 2c the one that came in from the share before
     const bool from_before = first < P.c0, goes_on = first + it.n > P.c1;
-    tree_finish<FP8, NT>(a, it, h, lane, st, from_before ? 2 * c : (goes_on ? 2 * c + 1 : -1));
-    if (!from_before && goes_on && h == 0 && lane == 0) a.ws_span[c] = make_int2(w, tree_last_share(P, first + it.n - 1));
+    tree_finish<FP8, 1>(a, it, tok0, 8 * WPH, 8 * sub, h, lane, st, from_before ? 2 * c : (goes_on ? 2 * c + 1 : -1));
+    if (!from_before && goes_on && h == 0 && sub == 0 && lane == 0)
+      a.ws_span[c] = make_int2(w, tree_last_share(P, first + it.n - 1));
   }
   if (k < n && lane == 0)
     for (int s = 0; s < STAGES; ++s)
       mbar_wait_bounded(&full[(k + s) % STAGES], static_cast<uint32_t>(((k + s) / STAGES) & 1), 100000000ull);
 }
 
-// Adds the partials of the item that starts in CTA c and goes on (if there is one) for KV head h: CTA (c, h).
-// cols = 2 heads x TOK tokens, eight to a CTA (blockIdx.z); each column's 128 dims in a warp, and with fewer columns than
-// warps the partials of a column are shared out over several warps.
+// Adds the partials of the item that starts in share c and goes on (if there is one), for eight (head, column) pairs: a warp
+// each, four dims a lane. Columns: 2 heads x the item's tokens. Warp-wide maximum and weights first (32 partials at a time),
+// so that the outputs' loads do not wait for anything.
 constexpr int kMergeWarps = 8;
 
 __global__ void __launch_bounds__(kMergeWarps * 32) paged_tree_merge_kernel(const TreeArgs a, int tok_per_group) {
-  __shared__ float4 part[kMergeWarps][32];
-  __shared__ float part_l[kMergeWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x, lane = threadIdx.x & 31, pair = blockIdx.y * kMergeWarps + (threadIdx.x >> 5);
   const int2 span = __ldcg(&a.ws_span[c]);
   if (span.x < 0) return;
   const int seat = span.x / a.groups, tok0 = (span.x - seat * a.groups) * tok_per_group;
+  const int live = 2 * min(tok_per_group, a.tokens - tok0), h = pair / live, col = pair - h * live;
+  if (h >= kKvHeads) return;
   const int cols = 2 * tok_per_group, parts = span.y - c + 1;
-  const int col0 = blockIdx.z * kMergeWarps, live = min(2 * min(tok_per_group, a.tokens - tok0) - col0, kMergeWarps);
-  if (live <= 0) return;
-  int drafts = a.tokens;
-  if (a.draft_lens != nullptr) drafts = a.draft_lens[seat];
-  int share = 1;                                     // warps per column: the largest power of two that leaves none over
-  while (share * 2 * live <= kMergeWarps) share *= 2;
-  const int per = kMergeWarps / share;               // columns at a time
-  {
-    const int col = col0 + warp % per, sub = warp / per;
-    const bool mine = warp % per < live;
-    // partial x of the column: slot 2c + 1 for x = 0, then slot 2(c + x)
-    auto at = [&](int x) {
-      return (static_cast<long long>(x == 0 ? 2 * c + 1 : 2 * (c + x)) * kKvHeads + h) * cols + col;
-    };
-    float M = -INFINITY;
-    if (mine)
-      for (int x = lane; x < parts; x += 32) M = fmaxf(M, __ldcg(a.ws_ml + 2 * at(x)));
-    M = warp_max(M);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float4 o = make_float4(0, 0, 0, 0);
-    float l = 0.f;
-    if (mine) {
-#pragma unroll 4
-      for (int x = sub; x < parts; x += share) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + 2 * at(x)));
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(a.ws_o + at(x) * kHeadDim) + lane);
-        const float f = exp2f(ml.x - ref);
-        l += ml.y * f;
-        o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
-      }
+  // partial x of the column: slot 2c + 1 for x = 0, then slot 2(c + x)
+  auto at = [&](int x) {
+    return (static_cast<long long>(x == 0 ? 2 * c + 1 : 2 * (c + x)) * kKvHeads + h) * cols + col;
+  };
+  float M = -INFINITY;
+  for (int x = lane; x < parts; x += 32) M = fmaxf(M, __ldcg(a.ws_ml + 2 * at(x)));
+  M = warp_max(M);
+  const float ref = M == -INFINITY ? 0.f : M;
+  float4 o = make_float4(0, 0, 0, 0);
+  float l = 0.f;
+  for (int x0 = 0; x0 < parts; x0 += 32) {
+    float w = 0.f;
+    if (x0 + lane < parts) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + 2 * at(x0 + lane)));
+      w = exp2f(ml.x - ref);
+      l += ml.y * w;
     }
-    if (share > 1) {
-      part[warp][lane] = o;
-      if (lane == 0) part_l[warp] = l;
-      __syncthreads();
-      if (sub == 0) {
-        for (int x = 1; x < share; ++x) {
-          const float4 v = part[warp + x * per][lane];
-          o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
-          l += part_l[warp + x * per];
-        }
-      }
-      __syncthreads();
-    }
-    if (mine && sub == 0) {
-      const int tok = tok0 + (col >> 1);
-      const bool none = l == 0.f || tok >= drafts;
-      const float r = 1.f / l;
-      __nv_bfloat16* dst = a.out + static_cast<long long>(seat) * a.out_seat + static_cast<long long>(tok) * a.out_tok +
-                           (2 * h + (col & 1)) * kHeadDim;
-      *(reinterpret_cast<uint2*>(dst) + lane) =
-          none ? make_uint2(0, 0) : float4_to_bf16x4(make_float4(o.x * r, o.y * r, o.z * r, o.w * r));
+    const int n = min(32, parts - x0);
+#pragma unroll 8
+    for (int x = 0; x < n; ++x) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.ws_o + at(x0 + x) * kHeadDim) + lane);
+      const float f = __shfl_sync(0xffffffffu, w, x);
+      o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
     }
   }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+  const int tok = tok0 + (col >> 1);
+  const bool none = l == 0.f || (a.draft_lens != nullptr && tok >= a.draft_lens[seat]);
+  const float r = 1.f / l;
+  __nv_bfloat16* dst = a.out + static_cast<long long>(seat) * a.out_seat + static_cast<long long>(tok) * a.out_tok +
+                       (2 * h + (col & 1)) * kHeadDim;
+  *(reinterpret_cast<uint2*>(dst) + lane) =
+      none ? make_uint2(0, 0) : float4_to_bf16x4(make_float4(o.x * r, o.y * r, o.z * r, o.w * r));
 }
 
 struct TreeConfig {
@@ -721,29 +761,56 @@ struct TreeConfig {
   int tok, shares;       // tokens per group; shares of the chunk list
 };
 
-// Up to 8 tokens: the kernel above, a group of 4 (one 8-column tile) or 8 (two), as many shares as CTAs fit. More: the
-// tcgen05 kernel, whose time does not grow with the tokens, one share per 8 SMs (a CTA per KV head). Its row maximum
-// takes the scale for positive; other scales run here in groups of 8 that each read the cache.
+// Up to 8 tokens: the kernel above, a group of 4 (one warp per head) or 8 (two). More: the tcgen05 kernel, whose time does
+// not grow with the tokens, one share per 8 SMs (a CTA per KV head). Its row maximum takes the scale for positive; other
+// scales run here in groups of 8 that each read the cache.
 TreeConfig tree_config(bool fp8, int tokens, float scale, int num_sms) {
   if (tokens > 8 && scale > 0.f) return {true, tokens, max(1, num_sms / kKvHeads)};
   const int tok = tokens <= 4 ? 4 : 8;
   return {false, tok, fp8 && tok == 4 ? 2 * num_sms : num_sms};
 }
 
-template <bool FP8, int NT, int STAGES, int MIN_CTAS>
-cudaError_t launch_tree_main(const TreeArgs& a, int grid, cudaStream_t stream) {
-  using SM = TreeSmem<FP8, NT, STAGES>;
-  auto kern = paged_tree_kernel<FP8, NT, STAGES, MIN_CTAS>;
+// A pool as [heads (bf16: half heads)][rows][128 bytes]; box = all heads x box_rows rows, 128-byte swizzle.
+template <bool FP8>
+bool make_pool_map(CUtensorMap* m, const void* base, long long rows, int box_rows) {
+  const EncodeTiled enc = tensor_map_encoder();
+  if (!enc || rows > (1ll << 31) - 1) return false;
+  const cuuint32_t parts = FP8 ? kKvHeads : 2 * kKvHeads, elems = FP8 ? 128 : 64;
+  const cuuint64_t dims[3] = {elems, static_cast<cuuint64_t>(rows), parts};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(TreeStage<FP8>::kRow), 128};
+  const cuuint32_t box[3] = {elems, static_cast<cuuint32_t>(box_rows), parts};
+  const cuuint32_t estr[3] = {1u, 1u, 1u};
+  return enc(m, FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// With the moved registers the launch is refused unless the kernel was built at exactly kLaunchRegs: a setmaxnreg.inc that
+// cannot be met would wait forever.
+template <bool FP8, bool DRAFTS, int STREAMS, int WPH, int STAGES>
+cudaError_t launch_tree_main(const TreeArgs& a, int shares, cudaStream_t stream) {
+  using SH = TreeShape<FP8, STREAMS, WPH, STAGES>;
+  auto kern = paged_tree_kernel<FP8, DRAFTS, STREAMS, WPH, STAGES>;
   static thread_local int configured_device = -1;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (configured_device != dev) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kBytes);
+    cudaFuncAttributes fa;
+    if ((e = cudaFuncGetAttributes(&fa, kern)) != cudaSuccess) return e;
+    if (SH::kMoveRegs && fa.numRegs != SH::kLaunchRegs) return cudaErrorInvalidConfiguration;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SH::kAlloc);
     if (e != cudaSuccess) return e;
     configured_device = dev;
   }
-  kern<<<grid, kTreeThreads, SM::kBytes, stream>>>(a);
+  TreeParams p;
+  memset(&p, 0, sizeof(p));
+  p.a = a;
+  p.box_rows = min(a.page_size & -a.page_size, kTreeRows);
+  const long long rows = static_cast<long long>(a.num_pages) * a.page_size;
+  if (!make_pool_map<FP8>(&p.k, a.k_pool, rows, p.box_rows) || !make_pool_map<FP8>(&p.v, a.v_pool, rows, p.box_rows))
+    return cudaErrorInvalidValue;
+  kern<<<shares / STREAMS, SH::kThreads, SH::kAlloc, stream>>>(p);
   return cudaGetLastError();
 }
 
@@ -768,16 +835,18 @@ cudaError_t launch_paged_tree(const TreeArgs& a, const TreeWorkspace& w, cudaStr
   const bool fp8 = a.k_scale != nullptr;
   cudaError_t e;
   if (w.tc) e = launch_paged_tree_tc(a, w.shares, stream);
-  else if (fp8 && w.tok == 4) e = launch_tree_main<true, 1, 3, 2>(a, w.shares, stream);
-  else if (fp8) e = launch_tree_main<true, 2, 6, 1>(a, w.shares, stream);
-  else if (w.tok == 4) e = launch_tree_main<false, 1, 3, 1>(a, w.shares, stream);
-  else e = launch_tree_main<false, 2, 3, 1>(a, w.shares, stream);
+  else if (fp8 && a.k_new == nullptr && w.tok == 4) e = launch_tree_main<true, false, 2, 1, 3>(a, w.shares, stream);
+  else if (fp8 && w.tok == 4) e = launch_tree_main<true, true, 2, 1, 3>(a, w.shares, stream);
+  else if (fp8) e = launch_tree_main<true, true, 1, 2, 6>(a, w.shares, stream);
+  else if (w.tok == 4) e = launch_tree_main<false, true, 1, 1, 3>(a, w.shares, stream);
+  else e = launch_tree_main<false, true, 1, 2, 3>(a, w.shares, stream);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(w.shares, kKvHeads, (2 * w.tok + kMergeWarps - 1) / kMergeWarps);
+  const int pairs = kKvHeads * 2 * min(w.tok, a.tokens);
+  lc.gridDim = dim3(w.shares, (pairs + kMergeWarps - 1) / kMergeWarps);
   lc.blockDim = dim3(kMergeWarps * 32);
   lc.stream = stream;
   lc.attrs = &at;

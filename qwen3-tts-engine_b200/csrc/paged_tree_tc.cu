@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc
     fence_mbar_init();
   }
   TreePlan P;
-  if (!tree_plan<kTcTok, kTcRows, kTcTok, SM::kThreads>(a, P, share, shares, 2 * h, 2)) return;   // nothing allocated yet
+  if (!tree_plan<kTcTok, kTcRows, kTcTok, SM::kThreads, 1>(a, P, share, shares, 0, 2 * h, 2)) return;   // nothing allocated yet
   if (warp == SM::kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                  "r"(kTcTmemCols));

@@ -38,14 +38,15 @@ struct TreePlan {
   int Ge, w;             // shares that have chunks; the item that holds chunk c0
 };
 
-// Share c of G of the chunk list, by all THREADS threads of the CTA. Items without chunks (nothing to attend, or padded
-// tokens alone) get zero rows here, for the CTA's heads [head0, head0 + heads). Returns false when the share is empty.
-template <int TOK, int ROWS, int DROWS, int THREADS>
-__device__ __forceinline__ bool tree_plan(const TreeArgs& a, TreePlan& P, int c, int G, int head0, int heads) {
+// Shares c .. c + NS - 1 of G of the chunk list, by all THREADS threads of the CTA; P receives share c + mine. Items
+// without chunks (nothing to attend, or padded tokens alone) get zero rows here, for the CTA's heads [head0, head0 + heads).
+// Returns false when all the shares are empty; one of several is empty when P.c0 == P.c1.
+template <int TOK, int ROWS, int DROWS, int THREADS, int NS>
+__device__ __forceinline__ bool tree_plan(const TreeArgs& a, TreePlan& P, int c, int G, int mine, int head0, int heads) {
   constexpr int kWarps = THREADS / 32;
   __shared__ long long sums[kWarps];
-  __shared__ long long found_first;
-  __shared__ int found_item;
+  __shared__ long long found_first[NS];
+  __shared__ int found_item[NS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, W = a.B * a.groups;
   long long local = 0;
   for (int w0 = warp * 32; w0 < W; w0 += THREADS) {   // uniform in a warp
@@ -59,7 +60,7 @@ __device__ __forceinline__ bool tree_plan(const TreeArgs& a, TreePlan& P, int c,
            (a.draft_lens != nullptr && a.draft_lens[it.seat] != it.drafts)))
         atomicOr(a.status, kStatusBadLength);
     }
-    for (unsigned zero = __ballot_sync(0xffffffffu, w < W && it.n == 0 && w % G == c); zero != 0; zero &= zero - 1) {
+    for (unsigned zero = __ballot_sync(0xffffffffu, w < W && it.n == 0 && w % G >= c && w % G < c + NS); zero != 0; zero &= zero - 1) {
       const int z = w0 + __ffs(zero) - 1, seat = z / a.groups, tok0 = (z - seat * a.groups) * TOK;
       const int per = heads * (kHeadDim / 8), n = min(TOK, a.tokens - tok0) * per;
       for (int i = lane; i < n; i += 32) {
@@ -78,9 +79,9 @@ __device__ __forceinline__ bool tree_plan(const TreeArgs& a, TreePlan& P, int c,
   for (int k = 0; k < kWarps; ++k) N += sums[k];
   P.N = N;
   P.Ge = static_cast<int>(N < G ? N : G);
-  if (c >= P.Ge) return false;
-  P.c0 = N * c / P.Ge;
-  P.c1 = N * (c + 1) / P.Ge;
+  const int active = min(P.Ge - c, NS);
+  if (active <= 0) return false;
+  const long long last = N * (c + active - 1) / P.Ge;   // where the last active share starts
   long long base = 0;
   for (int w0 = 0; w0 < W; w0 += THREADS) {
     const int w = w0 + tid;
@@ -101,16 +102,23 @@ __device__ __forceinline__ bool tree_plan(const TreeArgs& a, TreePlan& P, int c,
       total += sums[k];
     }
     incl += before;
-    if (n > 0 && incl - n <= P.c0 && P.c0 < incl) {
-      found_item = w;
-      found_first = incl - n;
+#pragma unroll
+    for (int v = 0; v < NS; ++v) {
+      const long long c0 = N * (c + v) / P.Ge;
+      if (v < active && n > 0 && incl - n <= c0 && c0 < incl) {
+        found_item[v] = w;
+        found_first[v] = incl - n;
+      }
     }
     base += total;
-    if (base > P.c0) break;   // uniform
+    if (base > last) break;   // uniform
   }
   __syncthreads();
-  P.w = found_item;
-  P.first = found_first;
+  const int v = min(mine, active - 1);
+  P.c0 = N * (c + v) / P.Ge;
+  P.c1 = mine < active ? N * (c + v + 1) / P.Ge : P.c0;
+  P.w = found_item[v];
+  P.first = found_first[v];
   return true;
 }
 
