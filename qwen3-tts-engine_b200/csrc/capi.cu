@@ -836,8 +836,8 @@ size_t q3_paged_tree_workspace_bytes(int32_t batch, int32_t tokens, int32_t quan
   int dev = 0;
   if (batch < 0 || tokens < 1 || tokens > q3::kTreeMaxTokens || current_device(&dev) != Q3_OK) return 0;
   // the larger of the two kernels' (which one runs depends on the scale's sign too)
-  const size_t x = q3::tree_workspace(quantised != 0, tokens, 1.f, sm_count(dev)).bytes;
-  const size_t y = q3::tree_workspace(quantised != 0, tokens, -1.f, sm_count(dev)).bytes;
+  const size_t x = q3::tree_workspace(quantised != 0, batch, tokens, 1.f, sm_count(dev)).bytes;
+  const size_t y = q3::tree_workspace(quantised != 0, batch, tokens, -1.f, sm_count(dev)).bytes;
   return x > y ? x : y;
 }
 
@@ -869,7 +869,7 @@ int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_
     return Q3_ERR_ALIGNMENT;
   int dev = 0;
   if ((rc = current_device(&dev)) != Q3_OK) return rc;
-  const q3::TreeWorkspace w = q3::tree_workspace(p->k_scale != nullptr, p->tokens, p->softmax_scale, sm_count(dev));
+  const q3::TreeWorkspace w = q3::tree_workspace(p->k_scale != nullptr, p->batch, p->tokens, p->softmax_scale, sm_count(dev));
   if (!workspace || workspace_bytes < w.bytes || !aligned(workspace, 256)) return Q3_ERR_WORKSPACE;
   q3::TreeArgs a{};
   if ((rc = status_ptr(dev, &a.status)) != Q3_OK) return rc;
@@ -906,7 +906,8 @@ int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_
   a.out_seat = p->out_seat_stride;
   a.out_tok = p->out_token_stride;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  a.ws_span = reinterpret_cast<int2*>(ws + w.span);
+  a.ws_span = reinterpret_cast<int4*>(ws + w.span);
+  a.span_by_item = w.span_by_item;
   a.ws_ml = reinterpret_cast<float*>(ws + w.ml);
   a.ws_o = reinterpret_cast<float*>(ws + w.o);
   return record(q3::launch_paged_tree(a, w, static_cast<cudaStream_t>(stream)));

@@ -621,6 +621,10 @@ __global__ void __launch_bounds__(TreeShape<FP8, STREAMS, WPH, STAGES>::kThreads
   extern __shared__ __align__(1024) uint8_t tree_raw[];
   uint8_t* smem = tree_raw + ((1024u - (smem_addr(tree_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    prefetch_map(&p.k);
+    prefetch_map(&p.v);
+  }
   const int mine = warp < 4 ? min(warp, STREAMS - 1) : (warp - 4) / (kKvHeads * WPH);   // the warp's stream
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be scheduled; it waits for this grid
   if (tid == 0) {
@@ -630,7 +634,7 @@ __global__ void __launch_bounds__(TreeShape<FP8, STREAMS, WPH, STAGES>::kThreads
         mbar_init(&b[i], FP8 && p.box_rows == 1 ? 33 : 1);   // + each lane's scales when they come row by row
         mbar_init(&b[STAGES + i], kKvHeads * WPH);
       }
-      a.ws_span[STREAMS * blockIdx.x + s] = make_int2(-1, 0);
+      tree_no_span(a, STREAMS * blockIdx.x + s);
     }
     fence_mbar_init();
   }
@@ -698,62 +702,91 @@ __global__ void __launch_bounds__(TreeShape<FP8, STREAMS, WPH, STAGES>::kThreads
     // slot 2c + 1 holds the item that starts here and goes on, 2c the one that came in from the share before
     const bool from_before = first < P.c0, goes_on = first + it.n > P.c1;
     tree_finish<FP8, 1>(a, it, tok0, 8 * WPH, 8 * sub, h, lane, st, from_before ? 2 * c : (goes_on ? 2 * c + 1 : -1));
-    if (!from_before && goes_on && h == 0 && sub == 0 && lane == 0)
-      a.ws_span[c] = make_int2(w, tree_last_share(P, first + it.n - 1));
+    if (!from_before && h == 0 && sub == 0 && lane == 0)
+      tree_span(a, w, c, goes_on ? tree_last_share(P, first + it.n - 1) : c);
   }
   if (k < n && lane == 0)
     for (int s = 0; s < STAGES; ++s)
       mbar_wait_bounded(&full[(k + s) % STAGES], static_cast<uint32_t>(((k + s) / STAGES) & 1), 100000000ull);
 }
 
-// Adds the partials of the item that starts in share c and goes on (if there is one), for eight (head, column) pairs: a warp
-// each, four dims a lane. Columns: 2 heads x the item's tokens. Warp-wide maximum and weights first (32 partials at a time),
-// so that the outputs' loads do not wait for anything.
+// Adds the partials of the items that span shares. Columns: (head, 2 heads x token); 128 dims of a column are four per lane
+// of a warp. WIDE: few items of many partials each; one column per CTA, the partials shared out over its eight warps.
+// Otherwise a warp takes four columns, so that eight loads are in flight with two partials.
 constexpr int kMergeWarps = 8;
 
-__global__ void __launch_bounds__(kMergeWarps * 32) paged_tree_merge_kernel(const TreeArgs a, int tok_per_group) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x, lane = threadIdx.x & 31, pair = blockIdx.y * kMergeWarps + (threadIdx.x >> 5);
-  const int2 span = __ldcg(&a.ws_span[c]);
-  if (span.x < 0) return;
-  const int seat = span.x / a.groups, tok0 = (span.x - seat * a.groups) * tok_per_group;
-  const int live = 2 * min(tok_per_group, a.tokens - tok0), h = pair / live, col = pair - h * live;
-  if (h >= kKvHeads) return;
-  const int cols = 2 * tok_per_group, parts = span.y - c + 1;
-  // partial x of the column: slot 2c + 1 for x = 0, then slot 2(c + x)
-  auto at = [&](int x) {
-    return (static_cast<long long>(x == 0 ? 2 * c + 1 : 2 * (c + x)) * kKvHeads + h) * cols + col;
-  };
-  float M = -INFINITY;
-  for (int x = lane; x < parts; x += 32) M = fmaxf(M, __ldcg(a.ws_ml + 2 * at(x)));
-  M = warp_max(M);
-  const float ref = M == -INFINITY ? 0.f : M;
-  float4 o = make_float4(0, 0, 0, 0);
-  float l = 0.f;
-  for (int x0 = 0; x0 < parts; x0 += 32) {
-    float w = 0.f;
-    if (x0 + lane < parts) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + 2 * at(x0 + lane)));
-      w = exp2f(ml.x - ref);
-      l += ml.y * w;
-    }
-    const int n = min(32, parts - x0);
-#pragma unroll 8
-    for (int x = 0; x < n; ++x) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.ws_o + at(x0 + x) * kHeadDim) + lane);
-      const float f = __shfl_sync(0xffffffffu, w, x);
-      o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
-    }
+// Running (maximum, sum, output) of one column.
+struct MergeState {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float pm, float pl, const float4& v) {
+    const float mn = fmaxf(m, pm), ref = mn == -INFINITY ? 0.f : mn;
+    const float f = exp2f(m - ref), g = exp2f(pm - ref);
+    m = mn;
+    l = l * f + pl * g;
+    o.x = o.x * f + v.x * g; o.y = o.y * f + v.y * g; o.z = o.z * f + v.z * g; o.w = o.w * f + v.w * g;
   }
+};
+
+template <bool WIDE>
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_tree_merge_kernel(const TreeArgs a, int tok_per_group) {
+  constexpr int kCols = WIDE ? 1 : 4, kBatch = 8 / kCols;   // columns per warp; partials asked for at a time
+  __shared__ float4 part_o[WIDE ? kMergeWarps : 1][32];
+  __shared__ float2 part_ml[WIDE ? kMergeWarps : 1];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int4 span = __ldcg(&a.ws_span[blockIdx.x]);
+  if (span.x < 0) return;
+  const int seat = span.x / a.groups, tok0 = (span.x - seat * a.groups) * tok_per_group, c = span.y, parts = span.z - c + 1;
+  const int live = 2 * min(tok_per_group, a.tokens - tok0), cols = 2 * tok_per_group, pairs = kKvHeads * live;
+  const int pair0 = WIDE ? blockIdx.y : (blockIdx.y * kMergeWarps + warp) * kCols;
+  if (pair0 >= pairs) return;   // uniform in the CTA when WIDE
+  long long at[kCols];          // the columns in slot 0
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-  const int tok = tok0 + (col >> 1);
-  const bool none = l == 0.f || (a.draft_lens != nullptr && tok >= a.draft_lens[seat]);
-  const float r = 1.f / l;
-  __nv_bfloat16* dst = a.out + static_cast<long long>(seat) * a.out_seat + static_cast<long long>(tok) * a.out_tok +
-                       (2 * h + (col & 1)) * kHeadDim;
-  *(reinterpret_cast<uint2*>(dst) + lane) =
-      none ? make_uint2(0, 0) : float4_to_bf16x4(make_float4(o.x * r, o.y * r, o.z * r, o.w * r));
+  for (int i = 0; i < kCols; ++i) {
+    const int pair = min(pair0 + i, pairs - 1), h = pair / live;
+    at[i] = static_cast<long long>(h) * cols + (pair - h * live);
+  }
+  const long long slot_cols = static_cast<long long>(kKvHeads) * cols;
+  MergeState st[kCols];
+  for (int x0 = WIDE ? warp * kBatch : 0; x0 < parts; x0 += (WIDE ? kMergeWarps : 1) * kBatch) {
+    float4 v[kBatch][kCols];
+    float2 ml[kBatch][kCols];
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x) {   // partial x: slot 2c + 1 for x = 0, then slot 2 (c + x)
+      const int y = min(x0 + x, parts - 1);
+      const long long slot = (y == 0 ? 2 * c + 1 : 2 * (c + y)) * slot_cols;
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) {
+        v[x][i] = __ldcg(reinterpret_cast<const float4*>(a.ws_o + (slot + at[i]) * kHeadDim) + lane);
+        ml[x][i] = __ldcg(reinterpret_cast<const float2*>(a.ws_ml) + slot + at[i]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x)
+#pragma unroll
+      for (int i = 0; i < kCols; ++i)
+        if (x0 + x < parts) st[i].add(ml[x][i].x, ml[x][i].y, v[x][i]);
+  }
+  if (WIDE) {
+    part_o[warp][lane] = st[0].o;
+    if (lane == 0) part_ml[warp] = make_float2(st[0].m, st[0].l);
+    __syncthreads();
+    if (warp != 0) return;
+    for (int x = 1; x < kMergeWarps; ++x) st[0].add(part_ml[x].x, part_ml[x].y, part_o[x][lane]);
+  }
+  const int drafts = a.draft_lens != nullptr ? a.draft_lens[seat] : a.tokens;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    if (pair0 + i >= pairs) break;
+    const int h = (pair0 + i) / live, col = pair0 + i - h * live, tok = tok0 + (col >> 1);
+    const bool none = st[i].l == 0.f || tok >= drafts;
+    const float r = 1.f / st[i].l;
+    __nv_bfloat16* dst = a.out + static_cast<long long>(seat) * a.out_seat + static_cast<long long>(tok) * a.out_tok +
+                         (2 * h + (col & 1)) * kHeadDim;
+    *(reinterpret_cast<uint2*>(dst) + lane) =
+        none ? make_uint2(0, 0) : float4_to_bf16x4(make_float4(st[i].o.x * r, st[i].o.y * r, st[i].o.z * r, st[i].o.w * r));
+  }
 }
 
 struct TreeConfig {
@@ -816,16 +849,17 @@ cudaError_t launch_tree_main(const TreeArgs& a, int shares, cudaStream_t stream)
 
 }  // namespace
 
-TreeWorkspace tree_workspace(bool fp8, int tokens, float scale, int num_sms) {
+TreeWorkspace tree_workspace(bool fp8, int batch, int tokens, float scale, int num_sms) {
   TreeWorkspace w;
   const TreeConfig cfg = tree_config(fp8, tokens, scale, num_sms);
   w.tc = cfg.tc;
   w.tok = cfg.tok;
   w.shares = cfg.shares;
   w.groups = (tokens + cfg.tok - 1) / cfg.tok;
+  w.span_by_item = static_cast<long long>(batch) * w.groups <= w.shares;
   const size_t cols = 2ull * w.shares * kKvHeads * 2 * cfg.tok;   // two slots per share
   w.span = 0;
-  w.ml = (static_cast<size_t>(w.shares) * sizeof(int2) + 255) / 256 * 256;
+  w.ml = (static_cast<size_t>(w.shares) * sizeof(int4) + 255) / 256 * 256;
   w.o = w.ml + (cols * 2 * sizeof(float) + 255) / 256 * 256;
   w.bytes = w.o + cols * kHeadDim * sizeof(float);
   return w;
@@ -845,13 +879,16 @@ cudaError_t launch_paged_tree(const TreeArgs& a, const TreeWorkspace& w, cudaStr
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t lc = {};
-  const int pairs = kKvHeads * 2 * min(w.tok, a.tokens);
-  lc.gridDim = dim3(w.shares, (pairs + kMergeWarps - 1) / kMergeWarps);
+  // with six shares and more per item the wide form (9 seats of up to 40000 rows: 13 -> 4 us)
+  const int pairs = kKvHeads * 2 * min(w.tok, a.tokens), items = a.B * a.groups;
+  const bool wide = w.span_by_item && w.shares >= 6 * items;
+  lc.gridDim = dim3(w.span_by_item ? items : w.shares, wide ? pairs : (pairs + 4 * kMergeWarps - 1) / (4 * kMergeWarps));
   lc.blockDim = dim3(kMergeWarps * 32);
   lc.stream = stream;
   lc.attrs = &at;
   lc.numAttrs = 1;
-  return cudaLaunchKernelEx(&lc, paged_tree_merge_kernel, a, w.tok);
+  return wide ? cudaLaunchKernelEx(&lc, paged_tree_merge_kernel<true>, a, w.tok)
+              : cudaLaunchKernelEx(&lc, paged_tree_merge_kernel<false>, a, w.tok);
 }
 
 }  // namespace q3

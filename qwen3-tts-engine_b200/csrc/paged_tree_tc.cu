@@ -425,6 +425,10 @@ __global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int h = blockIdx.x & 7, share = blockIdx.x >> 3, shares = gridDim.x >> 3;
   const int live_warps = (2 * a.tokens + 31) / 32;
+  if (tid == 32) {
+    prefetch_map(&p.k);
+    prefetch_map(&p.v);
+  }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be scheduled; it waits for this grid
   if (tid == 0) {
     for (int i = 0; i < kSt; ++i) {
@@ -443,7 +447,7 @@ __global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc
     *abort_flag = 0;
     for (int i = 0; i < SM::kCopyWarps; ++i) issued[i] = 0;
     for (int i = 0; i < kTcOddSlots; ++i) odd[i] = 0;
-    if (h == 0) a.ws_span[share] = make_int2(-1, 0);
+    if (h == 0) tree_no_span(a, share);
     fence_mbar_init();
   }
   TreePlan P;
@@ -639,8 +643,8 @@ __global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc
         __syncwarp();   // the TMEM loads are the whole warp's
       }
       if (slot >= 0 && mine) *reinterpret_cast<float2*>(a.ws_ml + 2 * col) = make_float2(m_run, l_run);
-      if (slot == 2 * share + 1 && h == 0 && tid == 0)
-        a.ws_span[share] = make_int2(cur.w, tree_last_share(P, cur.first + cur.it.n - 1));
+      if (!from_before && h == 0 && tid == 0)
+        tree_span(a, cur.w, share, goes_on ? tree_last_share(P, cur.first + cur.it.n - 1) : share);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[SM::kOFree]);

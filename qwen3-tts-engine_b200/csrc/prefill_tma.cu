@@ -76,10 +76,6 @@ struct PfTmaParams {
   int pool_maps;     // tkp / tvp are valid
 };
 
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
-}
-
 // Shared -> global tensor store (a page-aligned box of new K or V rows into the pool), in this thread's bulk group.
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(

@@ -123,7 +123,9 @@ struct TreeArgs {
   float scale_log2;
   __nv_bfloat16* out;              // [B, tokens, 16, 128]
   long long out_seat, out_tok;
-  int2* ws_span;                   // [shares] (item that starts in the share and goes on, its last share), item -1: none
+  int4* ws_span;                   // [shares] items that span shares: (item or -1, first share, last share), one place per
+                                   // item (span_by_item: as many items as shares at most) or per share (where it starts)
+  int span_by_item;
   float* ws_ml;                    // [2 shares slots][8 heads][2 tok columns] (maximum, sum)
   float* ws_o;                     // the same columns' [128] fp32 outputs
   uint32_t* status;
@@ -131,9 +133,10 @@ struct TreeArgs {
 struct TreeWorkspace {
   bool tc;                         // the tcgen05 kernel (paged_tree_tc.cu)
   int tok, groups, shares;         // tokens per group, groups per seat, shares of the chunk list
+  int span_by_item;
   size_t span, ml, o, bytes;       // byte offsets, total
 };
-TreeWorkspace tree_workspace(bool fp8, int tokens, float scale, int num_sms);
+TreeWorkspace tree_workspace(bool fp8, int batch, int tokens, float scale, int num_sms);
 cudaError_t launch_paged_tree(const TreeArgs& a, const TreeWorkspace& w, cudaStream_t stream);
 cudaError_t launch_paged_tree_tc(const TreeArgs& a, int shares, cudaStream_t stream);
 

@@ -26,6 +26,10 @@ inline EncodeTiled tensor_map_encoder() {
   return fn;
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 // Tiled 3-D load of one box into shared memory at dst (shared-space address), completion counted on bar.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(

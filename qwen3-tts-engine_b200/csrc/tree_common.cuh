@@ -68,8 +68,10 @@ __device__ __forceinline__ bool tree_plan(const TreeArgs& a, TreePlan& P, int c,
                            static_cast<long long>(tok0 + i / per) * a.out_tok + head0 * kHeadDim;
         reinterpret_cast<uint4*>(o)[i % per] = make_uint4(0, 0, 0, 0);
       }
+      if (a.span_by_item && head0 == 0 && lane == 0) a.ws_span[z] = make_int4(-1, 0, 0, 0);
     }
   }
+  const long long own = local;   // one item per thread at most: its chunks
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) local += __shfl_xor_sync(0xffffffffu, local, o);
   if (lane == 0) sums[warp] = local;
@@ -85,7 +87,7 @@ __device__ __forceinline__ bool tree_plan(const TreeArgs& a, TreePlan& P, int c,
   long long base = 0;
   for (int w0 = 0; w0 < W; w0 += THREADS) {
     const int w = w0 + tid;
-    const int n = w < W ? tree_item<TOK, ROWS, DROWS>(a, w).n : 0;
+    const int n = W <= THREADS ? static_cast<int>(own) : (w < W ? tree_item<TOK, ROWS, DROWS>(a, w).n : 0);
     long long incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -120,6 +122,16 @@ __device__ __forceinline__ bool tree_plan(const TreeArgs& a, TreePlan& P, int c,
   P.w = found_item[v];
   P.first = found_first[v];
   return true;
+}
+
+// Nothing starts in share c and goes on, so far (records per share; records per item are all written as items end).
+__device__ __forceinline__ void tree_no_span(const TreeArgs& a, int c) {
+  if (!a.span_by_item) a.ws_span[c] = make_int4(-1, 0, 0, 0);
+}
+// Item w starts in share c; last: its last share.
+__device__ __forceinline__ void tree_span(const TreeArgs& a, int w, int c, int last) {
+  if (a.span_by_item) a.ws_span[w] = make_int4(last > c ? w : -1, c, last, 0);
+  else if (last > c) a.ws_span[c] = make_int4(w, c, last, 0);
 }
 
 // The last share of an item whose last chunk is e: the largest c with N * c / Ge <= e.
