@@ -3,22 +3,28 @@
 //
 // One CTA = (share of the chunk list, KV head h). Accumulator row r = 2 token + (q head & 1): the up to 128 rows of a seat
 // share every K/V tile, so the cache is read once however many tokens were drafted. Tiles of 64 keys:
-//   S = Q K^T      M = 128 rows, N = 64 keys:  A = Q, B = K from shared memory (128-byte swizzle)
+//   S = Q K^T      M = 128 rows, N = 64 keys:  A = Q from TMEM, B = K from shared memory (128-byte swizzle)
 //   O += P V       M = 128, N = 128 dims:      A = P (bf16) from TMEM, B = V from shared memory
 // The 8 CTAs of a share walk the same keys at the same time, one head each, so the 256 (128) contiguous bytes a CTA
 // takes of a token row join the other heads' in the DRAM page. Warps:
-//   copies (4/3)  bring the head's part of 64 token rows by TMA tensor copies of 128 bytes x R rows, R the largest
+//   copies (3/1)  bring the head's part of 64 token rows by TMA tensor copies of 128 bytes x R rows, R the largest
 //                 power of two up to 64 that divides the page size (a box never leaves its page), with the table
 //                 entries looked up a tile ahead. bf16 rows land swizzled, as operands. e4m3 rows (and their scales)
 //                 land in a ring of raw tiles. (Four-row gathers serve any page the same way but took 66 cycles each,
 //                 64 of them a tile: 341 us on 24 seats x 64 tokens x 1000 to 8000 rows.) Issuing a tile's copies
 //                 takes a warp longer than the tile's bytes take HBM, so the warps take tiles in turn.
-//   loaders (4/8) turn raw e4m3 tiles into bf16 operands, exactly (four significant bits times a power of two); write Q of
-//                 a new seat and the drafted rows (the last tile of a seat); zero V rows past a seat's last token.
-//   MMA (1)       lane 0 issues S(t+1) before P(t) V(t), so the tensor core works while the softmax does.
-//   softmax (4)   thread r owns row r: online softmax with a lazy maximum (O is rescaled in TMEM when it grows by more
-//                 than 2^8), P(t) as bf16 into TMEM over S(t); at a seat's end O to the output, or as a partial to the
-//                 workspace. Warps without live rows have no part in any of it.
+//   loaders (4/6) turn raw e4m3 tiles into operands: K as fp16 (exact; its scale goes to the scores, Q is then fp16 too,
+//                 scaled by a power of two per row), V as bf16 (exact: four significant bits times a power of two, so
+//                 that no range is lost next to the probabilities); write the drafted rows (the last tile of a seat); zero V
+//                 rows past a seat's last token.
+//   MMA (1)       one thread issues S(t+1) before P(t) V(t), so the tensor core works while the softmax does.
+//   softmax (2 x 4) set t & 1 takes tile t: thread r of a set owns row r: online softmax with a lazy maximum (the set's O is
+//                 rescaled in TMEM when it grows by more than 2^8), P(t) as bf16 into TMEM over S(t). Each set has an O,
+//                 maximum and sum of its own, so that the sets never wait for one another within a seat (one set alone
+//                 took 2000 cycles a tile, most of them latency, where HBM takes 1424); at a seat's end both add the two
+//                 up, half of the dims each, to the output or as a partial to the workspace. They also write Q into TMEM
+//                 (with Q in shared memory an S took 600 cycles: the tensor core reads 6 KB per 16 dims instead of 2).
+//                 Warps without live rows have no part in any of it.
 // An infinity or NaN in a drafted V row would reach rows that do not see it as 0 * inf: the loaders write zero in its
 // place and raise a flag, and the rows that do see it get it back at the end.
 //
@@ -40,38 +46,41 @@ namespace {
 
 constexpr int kTcRows = 64;                     // keys per tile (cached rows, or all drafted rows)
 constexpr int kTcTok = kTreeMaxTokens;          // tokens per item: the whole draft
-constexpr int kTcTmemCols = 256;
-constexpr uint32_t kTcOCol = 128;               // S(t), P(t) at column 64 * (t & 1); O at 128
-constexpr int kTcOddSlots = 8;
-constexpr int kTcLoaderWarp = 4;                // after the softmax warps 0-3
+constexpr int kTcTmemCols = 512;
+// S(t), P(t) at column 64 (t & 1); O of set s at 128 + 128 s; Q of item i at 384 + 64 (i & 1)
+constexpr uint32_t kTcOCol = 128, kTcQCol = 384;
+constexpr int kTcOddSlots = 16;                 // more than the stages: see where it is read
+constexpr int kTcLoaderWarp = 8;                // after the softmax warps 0-7
 
-// LARGE: more than 32 tokens. Q takes 256 bytes per accumulator row of live warps (the rows after them are whatever
-// follows in shared memory: they only reach rows nobody reads); what it leaves goes to the rings.
-template <bool FP8, bool LARGE>
+template <bool FP8>
 struct TcSmem {
-  static constexpr int kLoaders = FP8 ? 8 : 4;               // loader warps
-  static constexpr int kCopyWarps = FP8 ? 3 : 4;
-  static constexpr int kMmaWarp = kTcLoaderWarp + kLoaders, kCopyWarp = kMmaWarp + 1;
+  static constexpr int kLoaders = FP8 ? 4 : 4;               // loader warps
+  static constexpr int kCopyWarps = FP8 ? 2 : 2;             // 16 warps: 128 registers each
+  static constexpr int kMmaWarp = kTcLoaderWarp + kLoaders, kCopyWarp = kMmaWarp + 2;
   static constexpr int kThreads = (kCopyWarp + kCopyWarps) * 32;
-  static constexpr int kStages = FP8 ? (LARGE ? 3 : 4) : (LARGE ? 5 : 6);   // operand tiles
-  static constexpr int kRawSlots = FP8 ? 3 : 0;
+  static constexpr int kStages = FP8 ? 4 : 6;                // operand tiles
+  static constexpr int kRawSlots = FP8 ? 5 : 0;
   static constexpr int kCopySlots = FP8 ? kRawSlots : kStages;   // tiles the copies fill
-  static constexpr int kQBytes = LARGE ? 32768 : 16384, kTile = 16384, kHalf = 8192;
-  static constexpr int kQ = 0;                               // two Q buffers: [2 dim halves][128 or 64 rows][128 B]
-  static constexpr int kKv = 2 * kQBytes;                    // stage s: K then V, [2 dim halves][64 keys][128 B] each
+  static constexpr int kTile = 16384, kHalf = 8192;
+  static constexpr int kKv = 0;                              // stage s: K then V, [2 dim halves][64 keys][128 B] each
   static constexpr int kRaw = kKv + kStages * 2 * kTile;     // raw e4m3: K then V [64 rows][128 B], scales [2][64][8]
   static constexpr int kRawBytes = 2 * kTcRows * kHeadDim + 2 * kTcRows * kKvHeads;
-  static constexpr int kBars = kRaw + kRawSlots * kRawBytes;
+  static constexpr int kKeyScale = kRaw + kRawSlots * kRawBytes;   // e4m3: per stage, the score factor of each key (fp32)
+  static constexpr int kRowScale = kKeyScale + (FP8 ? kStages * kTcRows * 4 : 0);   // score factor of Q's rows, by item & 3
+  static constexpr int kMl = kRowScale + 4 * 128 * 4;        // (maximum, sum) of each set's rows, by item & 1
+  static constexpr int kBars = kMl + 2 * 2 * 128 * 8;
   static constexpr int kFull = 0, kEmpty = kStages, kCopied = 2 * kStages, kRawFree = kCopied + kCopySlots,
-                       kSFull = kRawFree + kRawSlots, kPFull = kSFull + 2, kPvDone = kPFull + 2, kOFree = kPvDone + 2,
-                       kFinal = kOFree + 1, kNumBars = kFinal + 1;
+                       kSFull = kRawFree + kRawSlots, kPFull = kSFull + 2, kPvDone = kPFull + 2, kQFull = kPvDone + 2,
+                       kOFree = kQFull + 2, kSets = kOFree + 1, kFinal = kSets + 4, kNumBars = kFinal + 2;
   static constexpr int kTmemSlot = kBars + 8 * kNumBars;
   static constexpr int kAbort = kTmemSlot + 4;
   static constexpr int kIssued = kAbort + 4;                 // per copy warp, 1 + its last tile issued (abort path)
   static constexpr int kOdd = kIssued + 4 * kCopyWarps;
   static constexpr int kBytes = kOdd + 4 * kTcOddSlots;
   static constexpr int kAlloc = kBytes + 1024;               // slack to align the base to 1024 B (swizzle atoms)
-  static_assert(kAlloc <= 232448 && kRawBytes % 1024 == 0, "shared memory");
+  // 1 KB of static shared memory (the plan's) and 1 KB the system keeps come on top
+  static_assert(kAlloc + 1024 <= 232448 && kRawBytes % 1024 == 0 && kKeyScale % 16 == 0 && kMl % 8 == 0 && kBars % 8 == 0,
+                "shared memory");
 };
 
 struct TcParams {
@@ -108,18 +117,26 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
   return true;
 }
 
-// The MMAs without the optional mask of output lanes.
-__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+// D += A B with A in TMEM, issued by the lane whose `leader` is not 0. The whole warp runs the code around it, so that
+// addresses and descriptors stay in uniform registers (inside a branch for one lane an MMA took 70 cycles to issue).
+__device__ __forceinline__ void tc_mma_tmem_a(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)));
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
+      : "memory");
 }
-__device__ __forceinline__ void tc_mma_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void tc_commit(uint32_t leader, uint32_t bar) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)));
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t tc_elect() {
+  uint32_t x;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(x));
+  return x;
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -182,10 +199,10 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
 // Lane l looks after rows 4 (l & 15) .. + 3 of a tile, of K (l < 16) or V, and copies the boxes that start there. With
 // boxes of four rows or more those rows are neighbours in the pool: one table entry, one box at most. All of a tile's
 // addresses are ready before its slot is waited for.
-template <bool FP8, bool LARGE>
+template <bool FP8>
 __device__ __forceinline__ void tc_copies(const TcParams& p, const TreePlan& P, TcCursor cur, uint8_t* smem, uint64_t* bars,
                                           volatile int* abort_flag, volatile int* issued, int h, int cw, int lane) {
-  using SM = TcSmem<FP8, LARGE>;
+  using SM = TcSmem<FP8>;
   const TreeArgs& a = p.a;
   const int n = static_cast<int>(P.c1 - P.c0), which = lane >> 4, r0 = 4 * (lane & 15);
   const CUtensorMap* map = which ? &p.v : &p.k;
@@ -279,11 +296,37 @@ __device__ __forceinline__ void tc_copies(const TcParams& p, const TreePlan& P, 
   }
 }
 
+// bf16 values as fp16 ones times a power of two. top: the largest magnitude's bf16 bits; up: 2^(14 - e), which brings it to
+// [2^14, 2^15); down: 2^(e - 14).
+__device__ __forceinline__ void half_scale(uint32_t top, float& up, float& down) {
+  const int e = max(static_cast<int>(top >> 7) - 127, -112);
+  up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
+  down = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+}
+__device__ __forceinline__ uint32_t vec_top(uint32_t m, const uint4& w) {   // packed maxima of magnitudes
+  m = __vmaxu2(__vmaxu2(m, w.x & 0x7fff7fffu), w.y & 0x7fff7fffu);
+  return __vmaxu2(__vmaxu2(m, w.z & 0x7fff7fffu), w.w & 0x7fff7fffu);
+}
+// The largest magnitude of a row whose vectors lie in lanes `from`, 2 from, .. `to` apart.
+__device__ __forceinline__ uint32_t row_top(const uint4& w, int from, int to) {
+  uint32_t m = vec_top(0u, w);
+  for (int o = from; o <= to; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return max(m & 0xffffu, m >> 16);
+}
+__device__ __forceinline__ uint32_t to_half2(uint32_t w, float up) {
+  const float2 x = bf16x2_to_float2(w);
+  const __half2 h = __floats2half2_rn(x.x * up, x.y * up);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint4 to_half(const uint4& w, float up) {
+  return make_uint4(to_half2(w.x, up), to_half2(w.y, up), to_half2(w.z, up), to_half2(w.w, up));
+}
+
 // ------------------------------------------------------------------ the loader warps
-template <bool FP8, bool LARGE>
+template <bool FP8>
 struct TcLoader {
-  using SM = TcSmem<FP8, LARGE>;
-  static constexpr int kThreads = SM::kLoaders * 32, kRowStep = kThreads / 16;   // 16 threads per row of 256 bytes
+  using SM = TcSmem<FP8>;
+  static constexpr int kThreads = 128, kRowStep = kThreads / 16;   // the first four warps: 16 threads per row of 256 bytes
   const TreeArgs& a;
   const TreePlan& P;
   uint32_t sbase;
@@ -292,31 +335,21 @@ struct TcLoader {
   volatile int* abort_flag;
   int h, tid;
 
-  // Everything of tile k that the copies do not write, then the tile is handed to the tensor core. last0, last1: the
-  // last tiles of the item before and of the one before that (-1: none).
-  __device__ __forceinline__ bool tile(int k, TcCursor& c, int& last0, int& last1, volatile int* odd) {
+  // Everything of tile k that the copies do not write, then the tile is handed to the tensor core.
+  __device__ __forceinline__ bool tile(int k, TcCursor& c, volatile int* odd) {
     const int stage = k % SM::kStages;
-    const bool starts = tc_seek(a, P, c, k) || k == 0;
+    tc_seek(a, P, c, k);
     const int j = tc_chunk(c, k);
     const uint32_t dst = sbase + SM::kKv + static_cast<uint32_t>(stage) * 2 * SM::kTile;
     if (k >= SM::kStages && !wait(SM::kEmpty + stage, (k / SM::kStages - 1) & 1)) return false;
-    if (starts) {
-      // the Q buffer's last user is two items back; once its stage has been handed out again it is done
-      last1 = last0;
-      last0 = k - 1;
-      if (last1 >= 0 && k < last1 + SM::kStages && !wait(SM::kEmpty + last1 % SM::kStages, (last1 / SM::kStages) & 1))
-        return false;
-      load_q(c.it.seat, sbase + SM::kQ + (c.index & 1) * SM::kQBytes);
-    }
     const int real = c.it.len - j * kTcRows;   // cached tiles: rows that hold a token
-    bool wrote = starts;
+    bool wrote = FP8;
     if (FP8) {
       const int slot = k % (SM::kRawSlots + !FP8);
       if (!wait(SM::kCopied + slot, (k / (SM::kRawSlots + !FP8)) & 1)) return false;
-      if (j < c.it.nc) convert(smem + SM::kRaw + slot * SM::kRawBytes, dst, real);
+      if (j < c.it.nc) convert(smem + SM::kRaw + slot * SM::kRawBytes, dst, key_scale(stage), real);
       __syncwarp();
       if ((tid & 31) == 0) mbar_arrive(&bars[SM::kRawFree + slot]);
-      wrote = true;
     } else if (j < c.it.nc && real < kTcRows) {
       // whatever lies in the rows behind the last token, their probability 0 must meet a 0
       if (!wait(SM::kCopied + stage, (k / SM::kStages) & 1)) return false;
@@ -324,8 +357,8 @@ struct TcLoader {
         st_shared16(dst + SM::kTile + tc_unit(real + (i >> 4), i & 15, SM::kHalf), make_uint4(0, 0, 0, 0));
       wrote = true;
     }
-    if (j >= c.it.nc) {
-      if (load_draft(c.it, dst)) odd[c.index % kTcOddSlots] = c.index + 1;
+    if (j >= c.it.nc && tid < kThreads) {
+      if (load_draft(c.it, dst, key_scale(stage))) odd[c.index % kTcOddSlots] = c.index + 1;
       wrote = true;
     }
     if (wrote) fence_proxy_async_smem();   // this thread's writes before the tensor core reads
@@ -334,24 +367,47 @@ struct TcLoader {
     return true;
   }
 
-  // A raw e4m3 tile as bf16 operands; rows past `real` as zeros. 8 threads per row, 16 values each.
-  __device__ __forceinline__ void convert(const uint8_t* raw, uint32_t dst, int real) {
+  __device__ __forceinline__ float* key_scale(int stage) const {
+    return reinterpret_cast<float*>(smem + SM::kKeyScale) + stage * kTcRows;
+  }
+
+  // A raw e4m3 tile as operands, K fp16 and V bf16; V rows past `real` as zeros. 8 threads per row, 16 values each.
+  __device__ __forceinline__ void convert(const uint8_t* raw, uint32_t dst, float* scale, int real) {
+    constexpr int kAll = SM::kLoaders * 32, kPer = kTcRows * 8 / kAll, kStep = kAll / 8;
     const int u = tid & 7;
+    // dims 16u .. + 15 are units 2u and 2u + 1; the lanes of the second half write the odd unit first (banks)
+    const bool swap = u >= 4;
+    const uint8_t* scales = raw + 2 * kTcRows * kHeadDim + h;
+    uint4 k[kPer], v[kPer];
+    uint32_t s[kPer];
 #pragma unroll
-    for (int x = 0; x < 2 * kTcRows * 8 / kThreads; ++x) {
-      const int i = (tid >> 3) + (kThreads / 8) * x, which = i / kTcRows, r = i % kTcRows;
-      uint4 w = *reinterpret_cast<const uint4*>(raw + i * kHeadDim + u * 16);
-      const float s = e8m0_to_float(raw[2 * kTcRows * kHeadDim + i * kKvHeads + h]);
-      const float2 f = make_float2(s, s);
-      const uint2 p0 = dequant4(w.x, f), p1 = dequant4(w.y, f), p2 = dequant4(w.z, f), p3 = dequant4(w.w, f);
-      uint4 lo = make_uint4(p0.x, p0.y, p1.x, p1.y), hi = make_uint4(p2.x, p2.y, p3.x, p3.y);
-      if (r >= real) lo = hi = make_uint4(0, 0, 0, 0);
-      const uint32_t t = dst + which * SM::kTile;
-      // dims 16u .. + 15 are units 2u and 2u + 1; the lanes of the second half write the odd unit first (banks)
-      const bool swap = u >= 4;
-      st_shared16(t + tc_unit(r, 2 * u + swap, SM::kHalf), swap ? hi : lo);
-      st_shared16(t + tc_unit(r, 2 * u + !swap, SM::kHalf), swap ? lo : hi);
+    for (int x = 0; x < kPer; ++x) {
+      const int r = (tid >> 3) + kStep * x;
+      k[x] = *reinterpret_cast<const uint4*>(raw + r * kHeadDim + u * 16);
+      v[x] = *reinterpret_cast<const uint4*>(raw + (kTcRows + r) * kHeadDim + u * 16);
+      s[x] = scales[(kTcRows + r) * kKvHeads];
     }
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) {
+      const int r = (tid >> 3) + kStep * x;
+      const uint32_t first = dst + tc_unit(r, 2 * u + swap, SM::kHalf);
+      uint4 lo, hi;
+      e4m3x4_to_half2(k[x].x, lo.x, lo.y);
+      e4m3x4_to_half2(k[x].y, lo.z, lo.w);
+      e4m3x4_to_half2(k[x].z, hi.x, hi.y);
+      e4m3x4_to_half2(k[x].w, hi.z, hi.w);
+      st_shared16(first, swap ? hi : lo);
+      st_shared16(first ^ 16u, swap ? lo : hi);
+      const float sc = e8m0_to_float(s[x]);
+      const float2 f = make_float2(sc, sc);
+      const uint2 p0 = dequant4(v[x].x, f), p1 = dequant4(v[x].y, f), p2 = dequant4(v[x].z, f), p3 = dequant4(v[x].w, f);
+      lo = make_uint4(p0.x, p0.y, p1.x, p1.y);
+      hi = make_uint4(p2.x, p2.y, p3.x, p3.y);
+      if (r >= real) lo = hi = make_uint4(0, 0, 0, 0);
+      st_shared16(first + SM::kTile, swap ? hi : lo);
+      st_shared16((first ^ 16u) + SM::kTile, swap ? lo : hi);
+    }
+    if (tid < kTcRows) scale[tid] = e8m0_to_float(scales[tid * kKvHeads]);
   }
 
   __device__ __forceinline__ bool wait(int bar, uint32_t parity) {
@@ -359,28 +415,9 @@ struct TcLoader {
     tw_fail(a.status, abort_flag);
     return false;
   }
-  __device__ __forceinline__ void load_q(int seat, uint32_t dst) {
-    const int u = tid & 15, rows = (2 * a.tokens + 31) / 32 * 32;   // rows of live warps
-    for (int r0 = 0; r0 < rows; r0 += 4 * kRowStep) {
-      uint4 v[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int r = r0 + (tid >> 4) + kRowStep * x;
-        v[x] = make_uint4(0, 0, 0, 0);
-        if (r < 2 * a.tokens)
-          v[x] = __ldg(reinterpret_cast<const uint4*>(a.q + static_cast<long long>(seat) * a.q_seat +
-                                                      static_cast<long long>(r >> 1) * a.q_tok +
-                                                      (2 * h + (r & 1)) * kHeadDim) + u);
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int r = r0 + (tid >> 4) + kRowStep * x;
-        if (r < SM::kQBytes / 256) st_shared16(dst + tc_unit(r, u, SM::kQBytes / 2), v[x]);
-      }
-    }
-  }
-  // The drafted rows as one tile; true when a V value was an infinity or NaN.
-  __device__ __forceinline__ bool load_draft(const TreeItem& it, uint32_t dst) {
+  // The drafted rows as one tile; true when a V value was an infinity or NaN. FP8: K as fp16 with a power of two per key, as
+  // Q is (exact unless an element is 2^28 below the row's largest).
+  __device__ __forceinline__ bool load_draft(const TreeItem& it, uint32_t dst, float* scale) {
     const int u = tid & 15;
     bool odd = false;
 #pragma unroll
@@ -401,6 +438,12 @@ struct TcLoader {
         const uint32_t at = tc_unit((tid >> 4) + kRowStep * (x0 + x), u, SM::kHalf);
         const uint4 f = make_uint4(finite_or_zero(v[x].x), finite_or_zero(v[x].y), finite_or_zero(v[x].z), finite_or_zero(v[x].w));
         odd |= f.x != v[x].x || f.y != v[x].y || f.z != v[x].z || f.w != v[x].w;
+        if (FP8) {
+          float up, down;
+          half_scale(row_top(k[x], 1, 8), up, down);
+          k[x] = to_half(k[x], up);
+          if (u == 0) scale[(tid >> 4) + kRowStep * (x0 + x)] = down;
+        }
         st_shared16(dst + at, k[x]);
         st_shared16(dst + SM::kTile + at, f);
       }
@@ -409,9 +452,9 @@ struct TcLoader {
   }
 };
 
-template <bool FP8, bool LARGE>
-__global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc_kernel(const __grid_constant__ TcParams p) {
-  using SM = TcSmem<FP8, LARGE>;
+template <bool FP8>
+__global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel(const __grid_constant__ TcParams p) {
+  using SM = TcSmem<FP8>;
   const TreeArgs& a = p.a;
   constexpr int kSt = SM::kStages;
   extern __shared__ __align__(1024) uint8_t tc_raw[];
@@ -424,7 +467,7 @@ __global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc
   const uint32_t sbase = smem_addr(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int h = blockIdx.x & 7, share = blockIdx.x >> 3, shares = gridDim.x >> 3;
-  const int live_warps = (2 * a.tokens + 31) / 32;
+  const int live_warps = (2 * a.tokens + 31) / 32;              // of each softmax set
   if (tid == 32) {
     prefetch_map(&p.k);
     prefetch_map(&p.v);
@@ -441,9 +484,11 @@ __global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc
       mbar_init(&bars[SM::kSFull + i], 1);
       mbar_init(&bars[SM::kPFull + i], live_warps);
       mbar_init(&bars[SM::kPvDone + i], 1);
+      mbar_init(&bars[SM::kQFull + i], live_warps);
     }
-    mbar_init(&bars[SM::kOFree], live_warps);
-    mbar_init(&bars[SM::kFinal], 1);
+    mbar_init(&bars[SM::kOFree], 2 * live_warps);
+    for (int i = 0; i < 4; ++i) mbar_init(&bars[SM::kSets + i], 2);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars[SM::kFinal + i], 1);
     *abort_flag = 0;
     for (int i = 0; i < SM::kCopyWarps; ++i) issued[i] = 0;
     for (int i = 0; i < kTcOddSlots; ++i) odd[i] = 0;
@@ -466,77 +511,141 @@ __global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc
   tc_enter(P, cur);
 
   if (warp >= SM::kCopyWarp) {
-    tc_copies<FP8, LARGE>(p, P, cur, smem, bars, abort_flag, issued, h, warp - SM::kCopyWarp, lane);
+    tc_copies<FP8>(p, P, cur, smem, bars, abort_flag, issued, h, warp - SM::kCopyWarp, lane);
   } else if (warp >= kTcLoaderWarp && warp < SM::kMmaWarp) {
-    TcLoader<FP8, LARGE> ld{a, P, sbase, smem, bars, abort_flag, h, tid - 32 * kTcLoaderWarp};
-    int last0 = -1, last1 = -1;
+    TcLoader<FP8> ld{a, P, sbase, smem, bars, abort_flag, h, tid - 32 * kTcLoaderWarp};
     for (int k = 0; k < n; ++k)
-      if (!ld.tile(k, cur, last0, last1, odd)) break;
-  } else if (warp == SM::kMmaWarp) {
-    // one thread: S(k), then P(k - 1) V(k - 1)
-    if (lane == 0) {
-      constexpr uint32_t kIdescQK = umma_idesc_bf16(128, kTcRows, 0, 0), kIdescPV = umma_idesc_bf16(128, kHeadDim, 0, 1);
-      const uint64_t dq = sw128_desc(sbase + SM::kQ, 1024, 16), dk = sw128_desc(sbase + SM::kKv, 1024, 16);
-      const uint64_t dv = sw128_desc(sbase + SM::kKv + SM::kTile, 1024, SM::kHalf);
-      bool ok = true;
-      TcCursor pv = cur;
-      auto wait = [&](int bar, int phase) { return tc_wait(&bars[bar], static_cast<uint32_t>(phase & 1), abort_flag); };
-      for (int k = 0; k <= n && ok; ++k) {
-        if (k < n) {
-          const int stage = k % kSt;
-          tc_seek(a, P, cur, k);
-          ok = wait(SM::kFull + stage, k / kSt) && (FP8 || wait(SM::kCopied + stage, k / kSt)) &&
-               (k < 2 || wait(SM::kPvDone + (k & 1), (k - 2) >> 1));   // P(k - 2) lay where S(k) goes
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t q = dq + (cur.index & 1) * (SM::kQBytes >> 4), kk = dk + stage * (2 * SM::kTile >> 4);
-          const uint32_t t_s = tmem + 64u * static_cast<uint32_t>(k & 1);
+      if (!ld.tile(k, cur, odd)) break;
+  } else if (warp == SM::kMmaWarp || warp == SM::kMmaWarp + 1) {
+    // two warps: S(k) and P(k) V(k), each tile after tile
+    const bool scores = warp == SM::kMmaWarp;
+    const uint32_t leader = tc_elect(), bar0 = smem_addr(bars);
+    // operand format bits 7 and 10: bf16; clear: fp16
+    constexpr uint32_t kIdescQK = umma_idesc_bf16(128, kTcRows, 0, 0) & (FP8 ? ~((1u << 7) | (1u << 10)) : ~0u);
+    constexpr uint32_t kIdescPV = umma_idesc_bf16(128, kHeadDim, 0, 1);
+    const uint64_t dk = sw128_desc(sbase + SM::kKv, 1024, 16);
+    const uint64_t dv = sw128_desc(sbase + SM::kKv + SM::kTile, 1024, SM::kHalf);
+    bool ok = true;
+    auto wait = [&](int bar, int phase) {
+      return __all_sync(0xffffffffu, tc_wait(&bars[bar], static_cast<uint32_t>(phase & 1), abort_flag));
+    };
+    int stage = 0, lap = 0;
+    for (int k = 0; k < n; ++k) {
+      if (scores) {
+        const bool starts = tc_seek(a, P, cur, k) || k == 0;
+        ok = (!starts || wait(SM::kQFull + (cur.index & 1), cur.index >> 1)) && wait(SM::kFull + stage, lap) &&
+             (FP8 || wait(SM::kCopied + stage, lap)) &&
+             (k < 2 || wait(SM::kPvDone + (k & 1), (k - 2) >> 1));   // P(k - 2) lay where S(k) goes
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t kk = dk + stage * (2 * SM::kTile >> 4);
+        const uint32_t t_s = tmem + 64u * static_cast<uint32_t>(k & 1), t_q = tmem + kTcQCol + 64u * static_cast<uint32_t>(cur.index & 1);
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks)
-            tc_mma(t_s, q + ((ks >> 2) * (SM::kQBytes / 2) + (ks & 3) * 32) / 16,
-                   kk + ((ks >> 2) * SM::kHalf + (ks & 3) * 32) / 16, kIdescQK, ks > 0);
-          umma_commit(&bars[SM::kSFull + (k & 1)]);
-        }
-        if (k > 0) {
-          const int p = k - 1, stage = p % kSt, b = p & 1;
-          const bool next = tc_seek(a, P, pv, p), starts = next || p == 0;
-          ok = wait(SM::kPFull + b, p >> 1) &&
-               (!next || wait(SM::kOFree, pv.index - 1));   // the last item's O has been read
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t v = dv + stage * (2 * SM::kTile >> 4);
+        for (int ks = 0; ks < 8; ++ks)
+          tc_mma_tmem_a(leader, t_s, t_q + 8u * ks, kk + ((ks >> 2) * SM::kHalf + (ks & 3) * 32) / 16, kIdescQK, ks > 0);
+        tc_commit(leader, bar0 + 8 * (SM::kSFull + (k & 1)));
+      } else {
+        const int b = k & 1;
+        const bool next = tc_seek(a, P, cur, k);
+        ok = wait(SM::kPFull + b, k >> 1) && (!next || wait(SM::kOFree, cur.index - 1)) &&   // the last item's O has been read
+             wait(SM::kFull + stage, lap) && (FP8 || wait(SM::kCopied + stage, lap));
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t v = dv + stage * (2 * SM::kTile >> 4);
+        const uint32_t more = k < cur.begin + 2 ? 0u : 1u;   // 0: a set's first tile of the item
 #pragma unroll
-          for (int ks = 0; ks < kTcRows / 16; ++ks)
-            tc_mma_tmem_a(tmem + kTcOCol, tmem + 64u * b + 8u * ks, v + ks * (2048 / 16), kIdescPV, !starts || ks > 0);
-          umma_commit(&bars[SM::kEmpty + stage]);
-          umma_commit(&bars[SM::kPvDone + b]);
-        }
+        for (int ks = 0; ks < kTcRows / 16; ++ks)
+          tc_mma_tmem_a(leader, tmem + kTcOCol + 128u * b, tmem + 64u * b + 8u * ks, v + ks * (2048 / 16), kIdescPV, more | ks);
+        tc_commit(leader, bar0 + 8 * (SM::kEmpty + stage));
+        tc_commit(leader, bar0 + 8 * (SM::kPvDone + b));
       }
-      if (!ok) tw_fail(a.status, abort_flag);
+      if (++stage == kSt) {
+        stage = 0;
+        ++lap;
+      }
     }
-    __syncwarp();
-  } else if (warp < live_warps) {
-    const int r = tid, tok = r >> 1;
-    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    if (!ok && lane == 0) tw_fail(a.status, abort_flag);
+  } else if (warp < kTcLoaderWarp && (warp & 3) < live_warps) {
+    const int set = warp >> 2, r = tid & 127, tok = r >> 1;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    float* row_scale = reinterpret_cast<float*>(smem + SM::kRowScale);
+    float2* set_ml = reinterpret_cast<float2*>(smem + SM::kMl);
     int k = 0;
     bool ok = true;
+    auto wait = [&](int bar, int phase) {
+      return __all_sync(0xffffffffu, tc_wait(&bars[bar], static_cast<uint32_t>(phase & 1), abort_flag));
+    };
+    // Row r of a seat's Q into the TMEM buffer of item `index`. The buffer's last user is two items back: a set gets to write
+    // it when it has read a score of the item between.
+    auto write_q = [&](int seat, int index) {
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<long long>(seat) * a.q_seat + static_cast<long long>(tok) * a.q_tok +
+                                                       (2 * h + (r & 1)) * kHeadDim);
+      const bool mine = r < 2 * a.tokens;
+      float up = 1.f, down = 1.f;
+      if (FP8) {
+        uint32_t top = 0;
+        if (mine)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = vec_top(top, __ldg(src + i));
+        half_scale(max(top & 0xffffu, top >> 16), up, down);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (mine) v = __ldg(src + 8 * half + i);
+          if (FP8) v = to_half(v, up);
+          w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+        __syncwarp();
+        tmem_st32u(tmem + kTcQCol + 64u * static_cast<uint32_t>(index & 1) + 32u * half + lane_base, w);
+      }
+      row_scale[(index & 3) * 128 + r] = down * a.scale_log2;
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[SM::kQFull + (index & 1)]);
+    };
+    TcCursor nxt = cur;
+    if (set == 0) write_q(cur.it.seat, 0);
     while (k < n && ok) {
       tc_seek(a, P, cur, k);
-      const int end = cur.end;
+      const int begin = cur.begin, end = cur.end;
+      const int q_at = max(begin, end - 2);   // the tile at which its set writes the next seat's Q
       unsigned long long see = 0;
       if (tok < cur.it.drafts)
         see = static_cast<unsigned long long>(a.mask[static_cast<long long>(cur.it.seat) * a.mask_seat + tok]) &
               (~0ull >> (64 - cur.it.drafts));
       float m_run = -INFINITY, l_run = 0.f;
-      for (const int k0 = k; k < end; ++k) {
-        const int b = k & 1, j = tc_chunk(cur, k);
-        ok = __all_sync(0xffffffffu, tc_wait(&bars[SM::kSFull + b], (k >> 1) & 1, abort_flag));
+      ok = wait(SM::kQFull + (cur.index & 1), cur.index >> 1);   // for the row's factor
+      const float factor = row_scale[(cur.index & 3) * 128 + r];
+      const int k0 = begin + ((begin ^ set) & 1);                  // the set's first tile
+      for (k = k0; k < end && ok; k += 2) {
+        const int j = tc_chunk(cur, k);
+        if (k == q_at && end < n) {
+          tc_seek(a, P, nxt, end);
+          write_q(nxt.it.seat, nxt.index);
+        }
+        ok = wait(SM::kSFull + set, k >> 1) && (!FP8 || wait(SM::kFull + k % kSt, k / kSt));   // (the keys' scales)
         if (!ok) break;
         tc_fence_after();
         float sv[2][32];
-        tmem_ld32(tmem + 64u * b + lane_base, sv[0]);
-        tmem_ld32(tmem + 64u * b + 32u + lane_base, sv[1]);
+        tmem_ld32(tmem + 64u * set + lane_base, sv[0]);
+        tmem_ld32(tmem + 64u * set + 32u + lane_base, sv[1]);
         tc_wait_ld();
+        if (FP8) {
+          const float4* ks = reinterpret_cast<const float4*>(smem + SM::kKeyScale) + k % kSt * (kTcRows / 4);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float4 f = ks[i];
+            float* x = &sv[i >> 3][4 * (i & 7)];
+            const float2 p = __fmul2_rn(make_float2(x[0], x[1]), make_float2(f.x, f.y));
+            const float2 q = __fmul2_rn(make_float2(x[2], x[3]), make_float2(f.z, f.w));
+            x[0] = p.x; x[1] = p.y; x[2] = q.x; x[3] = q.y;
+          }
+        }
         if (j >= cur.it.nc) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
@@ -556,12 +665,12 @@ __global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 32; ++i) cm[i & 3] = fmaxf(cm[i & 3], sv[u][i]);
-        const float cmax = fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3])) * a.scale_log2;   // the scale is positive
+        const float cmax = fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3])) * factor;   // the scale is positive
         const bool grow = cmax > m_run + 8.f || (m_run == -INFINITY && cmax > -INFINITY);
         const float m_new = grow ? cmax : m_run;
         const float alpha = grow ? ex2_approx(m_run - m_new) : 1.f;
         const float mm = m_new == -INFINITY ? 0.f : m_new;
-        const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(-mm, -mm);
+        const float2 sc2 = make_float2(factor, factor), nm2 = make_float2(-mm, -mm);
         float2 ls2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t pk[32];
 #pragma unroll
@@ -576,46 +685,70 @@ __global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc
         const float2 ls = __fadd2_rn(__fadd2_rn(ls2[0], ls2[1]), __fadd2_rn(ls2[2], ls2[3]));
         l_run = l_run * alpha + (ls.x + ls.y);
         m_run = m_new;
-        if (k > k0 && __any_sync(0xffffffffu, alpha != 1.f)) {   // the item's first tile starts O from zero
-          ok = __all_sync(0xffffffffu, tc_wait(&bars[SM::kPvDone + ((k - 1) & 1)], ((k - 1) >> 1) & 1, abort_flag));
-          if (!ok) break;
-          tc_fence_after();
+        if (k > k0 && __any_sync(0xffffffffu, alpha != 1.f)) {   // a set's first tile of an item starts its O from zero
+          // the set's last P V is done: S(k) was issued after it
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             float ov[32];
-            tmem_ld32(tmem + kTcOCol + lane_base + c * 32, ov);
+            tmem_ld32(tmem + kTcOCol + 128u * set + lane_base + c * 32, ov);
             tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) ov[i] *= alpha;
-            tmem_st32(tmem + kTcOCol + lane_base + c * 32, ov);
+            tmem_st32(tmem + kTcOCol + 128u * set + lane_base + c * 32, ov);
           }
           tc_wait_st();
         }
-        tmem_st32u(tmem + 64u * b + lane_base, pk);
+        tmem_st32u(tmem + 64u * set + lane_base, pk);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[SM::kPFull + b]);
+        if (lane == 0) mbar_arrive(&bars[SM::kPFull + set]);
       }
-      if (ok) ok = __all_sync(0xffffffffu, tc_wait(&bars[SM::kPvDone + ((k - 1) & 1)], ((k - 1) >> 1) & 1, abort_flag));
+      k = end;
+      if (!ok) break;
+      // ---- the item's end: the sets exchange (maximum, sum) and wait for the last P V of both
+      set_ml[((cur.index & 1) * 2 + set) * 128 + r] = make_float2(m_run, l_run);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[SM::kSets + (warp & 3)]);
+      ok = wait(SM::kSets + (warp & 3), cur.index) && wait(SM::kPvDone + ((end - 1) & 1), (end - 1) >> 1) &&
+           (end - begin < 2 || wait(SM::kPvDone + (end & 1), (end - 2) >> 1));
       if (!ok) break;
       tc_fence_after();
-      // ---- the item's rows: written when it is complete here, else left as a partial (slot 2 share + 1: it starts here
-      // and goes on; 2 share: it came in from the share before)
+      const float2 other = set_ml[((cur.index & 1) * 2 + (set ^ 1)) * 128 + r];
+      const float2 ml0 = set ? other : make_float2(m_run, l_run), ml1 = set ? make_float2(m_run, l_run) : other;
+      const bool have0 = end - begin > 1 || (begin & 1) == 0, have1 = end - begin > 1 || (begin & 1) == 1;
+      const float M = fmaxf(ml0.x, ml1.x), ref = M == -INFINITY ? 0.f : M;
+      const float f0 = have0 ? exp2f(ml0.x - ref) : 0.f, f1 = have1 ? exp2f(ml1.x - ref) : 0.f;
+      const float l = ml0.y * f0 + ml1.y * f1;   // an absent set's sum is 0
+      // written when the item is complete here, else left as a partial (slot 2 share + 1: it starts here and goes on;
+      // 2 share: it came in from the share before)
       const bool from_before = cur.first < P.c0, goes_on = cur.first + cur.it.n > P.c1;
       const int slot = from_before ? 2 * share : (goes_on ? 2 * share + 1 : -1);
       const bool mine = r < 2 * a.tokens;
-      const bool none = l_run == 0.f || (a.draft_lens != nullptr && tok >= cur.it.drafts);
-      const float inv = none ? 0.f : 1.f / l_run;
+      const bool none = l == 0.f || (a.draft_lens != nullptr && tok >= cur.it.drafts);
+      const float inv = none ? 0.f : 1.f / l;
       const unsigned long long fix = !goes_on && odd[cur.index % kTcOddSlots] == cur.index + 1 ? see : 0ull;
       const long long col = (static_cast<long long>(max(slot, 0)) * kKvHeads + h) * (2 * a.tokens) + r;
       __nv_bfloat16* dst = a.out + static_cast<long long>(cur.it.seat) * a.out_seat +
                            static_cast<long long>(mine ? tok : 0) * a.out_tok + (2 * h + (r & 1)) * kHeadDim;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 2 * set; c < 2 * set + 2; ++c) {
         float ov[32];
-        tmem_ld32(tmem + kTcOCol + lane_base + c * 32, ov);
-        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) ov[i] = 0.f;
+        if (have0) {
+          tmem_ld32(tmem + kTcOCol + lane_base + c * 32, ov);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ov[i] *= f0;
+        }
+        if (have1) {
+          float o1[32];
+          tmem_ld32(tmem + kTcOCol + 128u + lane_base + c * 32, o1);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ov[i] = fmaf(o1[i], f1, ov[i]);
+        }
         for (unsigned long long v = fix; v != 0; v &= v - 1) {   // infinities and NaN of drafted rows this row sees
           const __nv_bfloat16* src = a.v_new + static_cast<long long>(cur.it.seat) * a.kv_seat +
                                      static_cast<long long>(__ffsll(v) - 1) * a.kv_tok + h * kHeadDim + c * 32;
@@ -642,7 +775,7 @@ __global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc
         }
         __syncwarp();   // the TMEM loads are the whole warp's
       }
-      if (slot >= 0 && mine) *reinterpret_cast<float2*>(a.ws_ml + 2 * col) = make_float2(m_run, l_run);
+      if (slot >= 0 && mine && set == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * col) = make_float2(M, l);
       if (!from_before && h == 0 && tid == 0)
         tree_span(a, cur.w, share, goes_on ? tree_last_share(P, cur.first + cur.it.n - 1) : share);
       tc_fence_before();
@@ -655,9 +788,9 @@ __global__ void __launch_bounds__(TcSmem<FP8, LARGE>::kThreads, 1) paged_tree_tc
   // ------------------------------------------------------------------ teardown
   tc_fence_before();
   __syncthreads();
-  if (*abort_flag && tid == SM::kMmaWarp * 32) {   // let MMAs and copies in flight finish (bounded)
-    umma_commit(&bars[SM::kFinal]);
-    mbar_wait_bounded(&bars[SM::kFinal], 0, 200000000ull);
+  if (*abort_flag && (warp == SM::kMmaWarp || warp == SM::kMmaWarp + 1) && tc_elect()) {   // let what is in flight finish (bounded)
+    umma_commit(&bars[SM::kFinal + warp - SM::kMmaWarp]);
+    mbar_wait_bounded(&bars[SM::kFinal + warp - SM::kMmaWarp], 0, 200000000ull);
     int top = 0;
     for (int i = 0; i < SM::kCopyWarps; ++i) top = max(top, issued[i]);
     for (int k = max(top - SM::kCopySlots - SM::kCopyWarps, 0); k < top; ++k)
@@ -685,15 +818,15 @@ bool make_pool_map(CUtensorMap* m, const void* base, long long rows, int box_row
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool FP8, bool LARGE>
+template <bool FP8>
 cudaError_t launch_tc(const TreeArgs& a, int grid, cudaStream_t stream) {
-  auto kern = paged_tree_tc_kernel<FP8, LARGE>;
+  auto kern = paged_tree_tc_kernel<FP8>;
   static thread_local int configured_device = -1;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (configured_device != dev) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<FP8, LARGE>::kAlloc);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<FP8>::kAlloc);
     if (e != cudaSuccess) return e;
     configured_device = dev;
   }
@@ -705,17 +838,14 @@ cudaError_t launch_tc(const TreeArgs& a, int grid, cudaStream_t stream) {
   if (p.box_rows > kTcRows) p.box_rows = kTcRows;
   if (!make_pool_map<FP8>(&p.k, a.k_pool, rows, p.box_rows) || !make_pool_map<FP8>(&p.v, a.v_pool, rows, p.box_rows))
     return cudaErrorInvalidValue;
-  kern<<<grid, TcSmem<FP8, LARGE>::kThreads, TcSmem<FP8, LARGE>::kAlloc, stream>>>(p);
+  kern<<<grid, TcSmem<FP8>::kThreads, TcSmem<FP8>::kAlloc, stream>>>(p);
   return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_paged_tree_tc(const TreeArgs& a, int shares, cudaStream_t stream) {
-  const bool large = a.tokens > 32;
-  const int grid = shares * kKvHeads;
-  if (a.k_scale != nullptr) return large ? launch_tc<true, true>(a, grid, stream) : launch_tc<true, false>(a, grid, stream);
-  return large ? launch_tc<false, true>(a, grid, stream) : launch_tc<false, false>(a, grid, stream);
+  return a.k_scale != nullptr ? launch_tc<true>(a, shares * kKvHeads, stream) : launch_tc<false>(a, shares * kKvHeads, stream);
 }
 
 }  // namespace q3
