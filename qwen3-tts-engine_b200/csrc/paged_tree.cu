@@ -794,11 +794,12 @@ struct TreeConfig {
   int tok, shares;       // tokens per group; shares of the chunk list
 };
 
-// Up to 8 tokens: the kernel above, a group of 4 (one warp per head) or 8 (two). More: the tcgen05 kernel, whose time does
-// not grow with the tokens, one share per 8 SMs (a CTA per KV head). Its row maximum takes the scale for positive; other
-// scales run here in groups of 8 that each read the cache.
+// Few tokens: the kernel above, in groups of 4 (one warp per head) or 8 (two) that each read the cache. More: the tcgen05
+// kernel, whose time hardly grows with the tokens, one share per 8 SMs (a CTA per KV head). 96 seats of 1200 to 2400 rows:
+// bf16, 8 tokens 130 us here, 9 tokens 204 here and 181 there; e4m3, 16 tokens 224 here and 250 there, 17 tokens 319 and
+// 254. The tcgen05 kernel takes the row maximum before it scales, so a scale that is not positive runs here too.
 TreeConfig tree_config(bool fp8, int tokens, float scale, int num_sms) {
-  if (tokens > 8 && scale > 0.f) return {true, tokens, max(1, num_sms / kKvHeads)};
+  if (tokens > (fp8 ? 16 : 8) && scale > 0.f) return {true, tokens, max(1, num_sms / kKvHeads)};
   const int tok = tokens <= 4 ? 4 : 8;
   return {false, tok, fp8 && tok == 4 ? 2 * num_sms : num_sms};
 }

@@ -1,4 +1,4 @@
-// Attention of 9 to 64 drafted tokens per seat over a paged K/V cache (bf16 or e4m3), on the 5th-generation tensor
+// Attention of many drafted tokens (up to 64) per seat over a paged K/V cache (bf16 or e4m3), on the 5th-generation tensor
 // cores (tcgen05 + TMEM), sm_100a. The mathematics, the contract and the chunk list are those of paged_tree.cu.
 //
 // One CTA = (share of the chunk list, KV head h). Accumulator row r = 2 token + (q head & 1): the up to 128 rows of a seat
@@ -13,10 +13,8 @@
 //                 land in a ring of raw tiles. (Four-row gathers serve any page the same way but took 66 cycles each,
 //                 64 of them a tile: 341 us on 24 seats x 64 tokens x 1000 to 8000 rows.) Issuing a tile's copies
 //                 takes a warp longer than the tile's bytes take HBM, so the warps take tiles in turn.
-//   loaders (4/6) turn raw e4m3 tiles into operands: K as fp16 (exact; its scale goes to the scores, Q is then fp16 too,
-//                 scaled by a power of two per row), V as bf16 (exact: four significant bits times a power of two, so
-//                 that no range is lost next to the probabilities); write the drafted rows (the last tile of a seat); zero V
-//                 rows past a seat's last token.
+//   loaders (4/8) turn raw e4m3 tiles into bf16 operands (exact: four significant bits times a power of two); write the
+//                 drafted rows (the last tile of a seat); zero V rows past a seat's last token.
 //   MMA (1)       one thread issues S(t+1) before P(t) V(t), so the tensor core works while the softmax does.
 //   softmax (2 x 4) set t & 1 takes tile t: thread r of a set owns row r: online softmax with a lazy maximum (the set's O is
 //                 rescaled in TMEM when it grows by more than 2^8), P(t) as bf16 into TMEM over S(t). Each set has an O,
@@ -54,8 +52,8 @@ constexpr int kTcLoaderWarp = 8;                // after the softmax warps 0-7
 
 template <bool FP8>
 struct TcSmem {
-  static constexpr int kLoaders = FP8 ? 4 : 4;               // loader warps
-  static constexpr int kCopyWarps = FP8 ? 2 : 2;             // 16 warps: 128 registers each
+  static constexpr int kLoaders = FP8 ? 8 : 4;               // loader warps
+  static constexpr int kCopyWarps = 2;                       // 16 warps of 128 registers; e4m3: 20 of 96
   static constexpr int kMmaWarp = kTcLoaderWarp + kLoaders, kCopyWarp = kMmaWarp + 2;
   static constexpr int kThreads = (kCopyWarp + kCopyWarps) * 32;
   static constexpr int kStages = FP8 ? 4 : 6;                // operand tiles
@@ -65,9 +63,7 @@ struct TcSmem {
   static constexpr int kKv = 0;                              // stage s: K then V, [2 dim halves][64 keys][128 B] each
   static constexpr int kRaw = kKv + kStages * 2 * kTile;     // raw e4m3: K then V [64 rows][128 B], scales [2][64][8]
   static constexpr int kRawBytes = 2 * kTcRows * kHeadDim + 2 * kTcRows * kKvHeads;
-  static constexpr int kKeyScale = kRaw + kRawSlots * kRawBytes;   // e4m3: per stage, the score factor of each key (fp32)
-  static constexpr int kRowScale = kKeyScale + (FP8 ? kStages * kTcRows * 4 : 0);   // score factor of Q's rows, by item & 3
-  static constexpr int kMl = kRowScale + 4 * 128 * 4;        // (maximum, sum) of each set's rows, by item & 1
+  static constexpr int kMl = kRaw + kRawSlots * kRawBytes;   // (maximum, sum) of each set's rows, by item & 1
   static constexpr int kBars = kMl + 2 * 2 * 128 * 8;
   static constexpr int kFull = 0, kEmpty = kStages, kCopied = 2 * kStages, kRawFree = kCopied + kCopySlots,
                        kSFull = kRawFree + kRawSlots, kPFull = kSFull + 2, kPvDone = kPFull + 2, kQFull = kPvDone + 2,
@@ -79,7 +75,7 @@ struct TcSmem {
   static constexpr int kBytes = kOdd + 4 * kTcOddSlots;
   static constexpr int kAlloc = kBytes + 1024;               // slack to align the base to 1024 B (swizzle atoms)
   // 1 KB of static shared memory (the plan's) and 1 KB the system keeps come on top
-  static_assert(kAlloc + 1024 <= 232448 && kRawBytes % 1024 == 0 && kKeyScale % 16 == 0 && kMl % 8 == 0 && kBars % 8 == 0,
+  static_assert(kAlloc + 1024 <= 232448 && kRawBytes % 1024 == 0 && kMl % 8 == 0 && kBars % 8 == 0,
                 "shared memory");
 };
 
@@ -115,6 +111,16 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
   while (!poll())
     if (*abort_flag || global_timer_ns() - t0 > 2000000000ull) return false;
   return true;
+}
+
+// 16 consecutive 32-bit columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
 }
 
 // D += A B with A in TMEM, issued by the lane whose `leader` is not 0. The whole warp runs the code around it, so that
@@ -296,32 +302,6 @@ __device__ __forceinline__ void tc_copies(const TcParams& p, const TreePlan& P, 
   }
 }
 
-// bf16 values as fp16 ones times a power of two. top: the largest magnitude's bf16 bits; up: 2^(14 - e), which brings it to
-// [2^14, 2^15); down: 2^(e - 14).
-__device__ __forceinline__ void half_scale(uint32_t top, float& up, float& down) {
-  const int e = max(static_cast<int>(top >> 7) - 127, -112);
-  up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
-  down = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
-}
-__device__ __forceinline__ uint32_t vec_top(uint32_t m, const uint4& w) {   // packed maxima of magnitudes
-  m = __vmaxu2(__vmaxu2(m, w.x & 0x7fff7fffu), w.y & 0x7fff7fffu);
-  return __vmaxu2(__vmaxu2(m, w.z & 0x7fff7fffu), w.w & 0x7fff7fffu);
-}
-// The largest magnitude of a row whose vectors lie in lanes `from`, 2 from, .. `to` apart.
-__device__ __forceinline__ uint32_t row_top(const uint4& w, int from, int to) {
-  uint32_t m = vec_top(0u, w);
-  for (int o = from; o <= to; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return max(m & 0xffffu, m >> 16);
-}
-__device__ __forceinline__ uint32_t to_half2(uint32_t w, float up) {
-  const float2 x = bf16x2_to_float2(w);
-  const __half2 h = __floats2half2_rn(x.x * up, x.y * up);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint4 to_half(const uint4& w, float up) {
-  return make_uint4(to_half2(w.x, up), to_half2(w.y, up), to_half2(w.z, up), to_half2(w.w, up));
-}
-
 // ------------------------------------------------------------------ the loader warps
 template <bool FP8>
 struct TcLoader {
@@ -347,7 +327,7 @@ struct TcLoader {
     if (FP8) {
       const int slot = k % (SM::kRawSlots + !FP8);
       if (!wait(SM::kCopied + slot, (k / (SM::kRawSlots + !FP8)) & 1)) return false;
-      if (j < c.it.nc) convert(smem + SM::kRaw + slot * SM::kRawBytes, dst, key_scale(stage), real);
+      if (j < c.it.nc) convert(smem + SM::kRaw + slot * SM::kRawBytes, dst, real);
       __syncwarp();
       if ((tid & 31) == 0) mbar_arrive(&bars[SM::kRawFree + slot]);
     } else if (j < c.it.nc && real < kTcRows) {
@@ -358,7 +338,7 @@ struct TcLoader {
       wrote = true;
     }
     if (j >= c.it.nc && tid < kThreads) {
-      if (load_draft(c.it, dst, key_scale(stage))) odd[c.index % kTcOddSlots] = c.index + 1;
+      if (load_draft(c.it, dst)) odd[c.index % kTcOddSlots] = c.index + 1;
       wrote = true;
     }
     if (wrote) fence_proxy_async_smem();   // this thread's writes before the tensor core reads
@@ -367,47 +347,32 @@ struct TcLoader {
     return true;
   }
 
-  __device__ __forceinline__ float* key_scale(int stage) const {
-    return reinterpret_cast<float*>(smem + SM::kKeyScale) + stage * kTcRows;
-  }
-
-  // A raw e4m3 tile as operands, K fp16 and V bf16; V rows past `real` as zeros. 8 threads per row, 16 values each.
-  __device__ __forceinline__ void convert(const uint8_t* raw, uint32_t dst, float* scale, int real) {
-    constexpr int kAll = SM::kLoaders * 32, kPer = kTcRows * 8 / kAll, kStep = kAll / 8;
+  // A raw e4m3 tile as bf16 operands; rows past `real` as zeros. 8 threads per row, 16 values each.
+  __device__ __forceinline__ void convert(const uint8_t* raw, uint32_t dst, int real) {
+    constexpr int kAll = SM::kLoaders * 32, kPer = 2 * kTcRows * 8 / kAll, kStep = kAll / 8;
     const int u = tid & 7;
     // dims 16u .. + 15 are units 2u and 2u + 1; the lanes of the second half write the odd unit first (banks)
     const bool swap = u >= 4;
-    const uint8_t* scales = raw + 2 * kTcRows * kHeadDim + h;
-    uint4 k[kPer], v[kPer];
+    uint4 w[kPer];
     uint32_t s[kPer];
 #pragma unroll
-    for (int x = 0; x < kPer; ++x) {
-      const int r = (tid >> 3) + kStep * x;
-      k[x] = *reinterpret_cast<const uint4*>(raw + r * kHeadDim + u * 16);
-      v[x] = *reinterpret_cast<const uint4*>(raw + (kTcRows + r) * kHeadDim + u * 16);
-      s[x] = scales[(kTcRows + r) * kKvHeads];
+    for (int x = 0; x < kPer; ++x) {   // rows 0 .. 63 are K's, 64 .. 127 V's
+      const int i = (tid >> 3) + kStep * x;
+      w[x] = *reinterpret_cast<const uint4*>(raw + i * kHeadDim + u * 16);
+      s[x] = raw[2 * kTcRows * kHeadDim + i * kKvHeads + h];
     }
 #pragma unroll
     for (int x = 0; x < kPer; ++x) {
-      const int r = (tid >> 3) + kStep * x;
-      const uint32_t first = dst + tc_unit(r, 2 * u + swap, SM::kHalf);
-      uint4 lo, hi;
-      e4m3x4_to_half2(k[x].x, lo.x, lo.y);
-      e4m3x4_to_half2(k[x].y, lo.z, lo.w);
-      e4m3x4_to_half2(k[x].z, hi.x, hi.y);
-      e4m3x4_to_half2(k[x].w, hi.z, hi.w);
-      st_shared16(first, swap ? hi : lo);
-      st_shared16(first ^ 16u, swap ? lo : hi);
+      const int i = (tid >> 3) + kStep * x, r = i % kTcRows;
       const float sc = e8m0_to_float(s[x]);
       const float2 f = make_float2(sc, sc);
-      const uint2 p0 = dequant4(v[x].x, f), p1 = dequant4(v[x].y, f), p2 = dequant4(v[x].z, f), p3 = dequant4(v[x].w, f);
-      lo = make_uint4(p0.x, p0.y, p1.x, p1.y);
-      hi = make_uint4(p2.x, p2.y, p3.x, p3.y);
+      const uint2 p0 = dequant4(w[x].x, f), p1 = dequant4(w[x].y, f), p2 = dequant4(w[x].z, f), p3 = dequant4(w[x].w, f);
+      uint4 lo = make_uint4(p0.x, p0.y, p1.x, p1.y), hi = make_uint4(p2.x, p2.y, p3.x, p3.y);
       if (r >= real) lo = hi = make_uint4(0, 0, 0, 0);
-      st_shared16(first + SM::kTile, swap ? hi : lo);
-      st_shared16((first ^ 16u) + SM::kTile, swap ? lo : hi);
+      const uint32_t first = dst + i / kTcRows * SM::kTile + tc_unit(r, 2 * u + swap, SM::kHalf);
+      st_shared16(first, swap ? hi : lo);
+      st_shared16(first ^ 16u, swap ? lo : hi);
     }
-    if (tid < kTcRows) scale[tid] = e8m0_to_float(scales[tid * kKvHeads]);
   }
 
   __device__ __forceinline__ bool wait(int bar, uint32_t parity) {
@@ -415,9 +380,8 @@ struct TcLoader {
     tw_fail(a.status, abort_flag);
     return false;
   }
-  // The drafted rows as one tile; true when a V value was an infinity or NaN. FP8: K as fp16 with a power of two per key, as
-  // Q is (exact unless an element is 2^28 below the row's largest).
-  __device__ __forceinline__ bool load_draft(const TreeItem& it, uint32_t dst, float* scale) {
+  // The drafted rows as one tile; true when a V value was an infinity or NaN.
+  __device__ __forceinline__ bool load_draft(const TreeItem& it, uint32_t dst) {
     const int u = tid & 15;
     bool odd = false;
 #pragma unroll
@@ -438,12 +402,6 @@ struct TcLoader {
         const uint32_t at = tc_unit((tid >> 4) + kRowStep * (x0 + x), u, SM::kHalf);
         const uint4 f = make_uint4(finite_or_zero(v[x].x), finite_or_zero(v[x].y), finite_or_zero(v[x].z), finite_or_zero(v[x].w));
         odd |= f.x != v[x].x || f.y != v[x].y || f.z != v[x].z || f.w != v[x].w;
-        if (FP8) {
-          float up, down;
-          half_scale(row_top(k[x], 1, 8), up, down);
-          k[x] = to_half(k[x], up);
-          if (u == 0) scale[(tid >> 4) + kRowStep * (x0 + x)] = down;
-        }
         st_shared16(dst + at, k[x]);
         st_shared16(dst + SM::kTile + at, f);
       }
@@ -520,8 +478,7 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
     // two warps: S(k) and P(k) V(k), each tile after tile
     const bool scores = warp == SM::kMmaWarp;
     const uint32_t leader = tc_elect(), bar0 = smem_addr(bars);
-    // operand format bits 7 and 10: bf16; clear: fp16
-    constexpr uint32_t kIdescQK = umma_idesc_bf16(128, kTcRows, 0, 0) & (FP8 ? ~((1u << 7) | (1u << 10)) : ~0u);
+    constexpr uint32_t kIdescQK = umma_idesc_bf16(128, kTcRows, 0, 0);
     constexpr uint32_t kIdescPV = umma_idesc_bf16(128, kHeadDim, 0, 1);
     const uint64_t dk = sw128_desc(sbase + SM::kKv, 1024, 16);
     const uint64_t dv = sw128_desc(sbase + SM::kKv + SM::kTile, 1024, SM::kHalf);
@@ -568,7 +525,6 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
   } else if (warp < kTcLoaderWarp && (warp & 3) < live_warps) {
     const int set = warp >> 2, r = tid & 127, tok = r >> 1;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    float* row_scale = reinterpret_cast<float*>(smem + SM::kRowScale);
     float2* set_ml = reinterpret_cast<float2*>(smem + SM::kMl);
     int k = 0;
     bool ok = true;
@@ -581,14 +537,6 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
       const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<long long>(seat) * a.q_seat + static_cast<long long>(tok) * a.q_tok +
                                                        (2 * h + (r & 1)) * kHeadDim);
       const bool mine = r < 2 * a.tokens;
-      float up = 1.f, down = 1.f;
-      if (FP8) {
-        uint32_t top = 0;
-        if (mine)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) top = vec_top(top, __ldg(src + i));
-        half_scale(max(top & 0xffffu, top >> 16), up, down);
-      }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t w[32];
@@ -596,13 +544,11 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
         for (int i = 0; i < 8; ++i) {
           uint4 v = make_uint4(0, 0, 0, 0);
           if (mine) v = __ldg(src + 8 * half + i);
-          if (FP8) v = to_half(v, up);
           w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
         }
         __syncwarp();
         tmem_st32u(tmem + kTcQCol + 64u * static_cast<uint32_t>(index & 1) + 32u * half + lane_base, w);
       }
-      row_scale[(index & 3) * 128 + r] = down * a.scale_log2;
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -619,8 +565,6 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
         see = static_cast<unsigned long long>(a.mask[static_cast<long long>(cur.it.seat) * a.mask_seat + tok]) &
               (~0ull >> (64 - cur.it.drafts));
       float m_run = -INFINITY, l_run = 0.f;
-      ok = wait(SM::kQFull + (cur.index & 1), cur.index >> 1);   // for the row's factor
-      const float factor = row_scale[(cur.index & 3) * 128 + r];
       const int k0 = begin + ((begin ^ set) & 1);                  // the set's first tile
       for (k = k0; k < end && ok; k += 2) {
         const int j = tc_chunk(cur, k);
@@ -628,63 +572,70 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
           tc_seek(a, P, nxt, end);
           write_q(nxt.it.seat, nxt.index);
         }
-        ok = wait(SM::kSFull + set, k >> 1) && (!FP8 || wait(SM::kFull + k % kSt, k / kSt));   // (the keys' scales)
+        ok = wait(SM::kSFull + set, k >> 1);
         if (!ok) break;
         tc_fence_after();
-        float sv[2][32];
-        tmem_ld32(tmem + 64u * set + lane_base, sv[0]);
-        tmem_ld32(tmem + 64u * set + 32u + lane_base, sv[1]);
-        tc_wait_ld();
-        if (FP8) {
-          const float4* ks = reinterpret_cast<const float4*>(smem + SM::kKeyScale) + k % kSt * (kTcRows / 4);
+        const bool draft = j >= cur.it.nc;
+        const int real = draft ? kTcRows : cur.it.len - j * kTcRows;
+        const uint32_t t_s = tmem + 64u * set + lane_base;
+        // 32 products, -inf where the row does not see the key
+        auto scores = [&](float (&x)[32], int half) {
+          tmem_ld32(t_s + 32u * half, x);
+          tc_wait_ld();
+          if (draft) {
+            const uint32_t bits = static_cast<uint32_t>(see >> (32 * half));
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float4 f = ks[i];
-            float* x = &sv[i >> 3][4 * (i & 7)];
-            const float2 p = __fmul2_rn(make_float2(x[0], x[1]), make_float2(f.x, f.y));
-            const float2 q = __fmul2_rn(make_float2(x[2], x[3]), make_float2(f.z, f.w));
-            x[0] = p.x; x[1] = p.y; x[2] = q.x; x[3] = q.y;
+            for (int i = 0; i < 32; ++i) x[i] = ((bits >> i) & 1u) ? x[i] : -INFINITY;
+          } else if (real < kTcRows) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = half * 32 + i < real ? x[i] : -INFINITY;
           }
+        };
+        auto largest = [](const float (&x)[32]) {
+          float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) m[i & 3] = fmaxf(m[i & 3], x[i]);
+          return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        };
+        // e4m3: 96 registers hold one half of a row at a time, so its scores are read twice
+        float sv[FP8 ? 1 : 2][32];
+        float cmax;
+        if constexpr (FP8) {
+          scores(sv[0], 0);
+          cmax = largest(sv[0]);
+          scores(sv[0], 1);
+          cmax = fmaxf(cmax, largest(sv[0]));
+        } else {
+          scores(sv[0], 0);
+          scores(sv[1], 1);
+          cmax = fmaxf(largest(sv[0]), largest(sv[1]));
         }
-        if (j >= cur.it.nc) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t bits = static_cast<uint32_t>(see >> (32 * u));
-#pragma unroll
-            for (int i = 0; i < 32; ++i) sv[u][i] = ((bits >> i) & 1u) ? sv[u][i] : -INFINITY;
-          }
-        } else if (cur.it.len - j * kTcRows < kTcRows) {
-          const int real = cur.it.len - j * kTcRows;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) sv[u][i] = u * 32 + i < real ? sv[u][i] : -INFINITY;
-        }
-        float cm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) cm[i & 3] = fmaxf(cm[i & 3], sv[u][i]);
-        const float cmax = fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3])) * factor;   // the scale is positive
+        cmax *= a.scale_log2;   // which is positive
         const bool grow = cmax > m_run + 8.f || (m_run == -INFINITY && cmax > -INFINITY);
         const float m_new = grow ? cmax : m_run;
         const float alpha = grow ? ex2_approx(m_run - m_new) : 1.f;
         const float mm = m_new == -INFINITY ? 0.f : m_new;
-        const float2 sc2 = make_float2(factor, factor), nm2 = make_float2(-mm, -mm);
-        float2 ls2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        uint32_t pk[32];
+        const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(-mm, -mm);
+        float2 ls2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        m_run = m_new;
+        // P(k) over S(k), columns 16 half .. + 15: the scores there have been read
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int half = 0; half < 2; ++half) {
+          if constexpr (FP8) scores(sv[0], half);
+          const float(&x)[32] = sv[FP8 ? 0 : half];
+          uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float2 x = __ffma2_rn(make_float2(sv[u][i], sv[u][i + 1]), sc2, nm2);
-            const float2 pp = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-            ls2[(i >> 1) & 3] = __fadd2_rn(ls2[(i >> 1) & 3], pp);
-            pk[u * 16 + i / 2] = pack_bf16x2(pp.x, pp.y);
+            const float2 y = __ffma2_rn(make_float2(x[i], x[i + 1]), sc2, nm2);
+            const float2 pp = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+            ls2[(i >> 1) & 1] = __fadd2_rn(ls2[(i >> 1) & 1], pp);
+            pk[i / 2] = pack_bf16x2(pp.x, pp.y);
           }
-        const float2 ls = __fadd2_rn(__fadd2_rn(ls2[0], ls2[1]), __fadd2_rn(ls2[2], ls2[3]));
+          __syncwarp();
+          tmem_st16u(t_s + 16u * half, pk);
+        }
+        const float2 ls = __fadd2_rn(ls2[0], ls2[1]);
         l_run = l_run * alpha + (ls.x + ls.y);
-        m_run = m_new;
         if (k > k0 && __any_sync(0xffffffffu, alpha != 1.f)) {   // a set's first tile of an item starts its O from zero
           // the set's last P V is done: S(k) was issued after it
 #pragma unroll 1
@@ -698,7 +649,6 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
           }
           tc_wait_st();
         }
-        tmem_st32u(tmem + 64u * set + lane_base, pk);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
