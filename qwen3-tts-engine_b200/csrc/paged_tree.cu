@@ -564,7 +564,7 @@ __device__ __forceinline__ void tree_produce(const TreeParams& p, const TreePlan
       }
       look_up();
     }
-    if (k >= STAGES && !tree_wait(&empty[stage], static_cast<uint32_t>((k / STAGES - 1) & 1))) {
+    if (k >= STAGES && !mbar_wait_sleep(&empty[stage], static_cast<uint32_t>((k / STAGES - 1) & 1))) {
       atomicOr(a.status, kStatusWaitTimeout);
       ok = false;
     }
@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(TreeShape<FP8, STREAMS, WPH, STAGES>::kThreads
     int j = static_cast<int>(P.c0 + k - first);
     for (; k < end; ++k, ++j) {
       const int stage = k % STAGES;
-      if (!tree_wait(&full[stage], static_cast<uint32_t>((k / STAGES) & 1))) {
+      if (!mbar_wait_sleep(&full[stage], static_cast<uint32_t>((k / STAGES) & 1))) {
         atomicOr(a.status, kStatusWaitTimeout);
         ok = false;
       }

@@ -153,6 +153,25 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// The same, sleeping in the barrier up to 20 us at a time instead of polling; false after 2 s.
+__device__ __forceinline__ bool mbar_wait_sleep(uint64_t* bar, uint32_t parity) {
+  auto poll = [&]() -> bool {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    return ok != 0;
+  };
+  if (poll()) return true;
+  const uint64_t t0 = global_timer_ns();
+#pragma unroll 1
+  while (!poll())
+    if (global_timer_ns() - t0 > 2000000000ull) return false;
+  return true;
+}
+
 // 16-byte asynchronous copy global -> shared memory (no register staging; completion by cp_async_wait_all).
 __device__ __forceinline__ void cp_async16(void* smem_dst, const void* gsrc) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(smem_dst)), "l"(gsrc) : "memory");

@@ -146,25 +146,6 @@ __device__ __forceinline__ void e4m3x4_to_half2(uint32_t x, uint32_t& lo, uint32
       : "r"(x));
 }
 
-// Wait for phase `parity` of `bar`, sleeping in the barrier (up to 20 us at a time); false after 2 s.
-__device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity) {
-  auto poll = [&]() -> bool {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_addr(bar)), "r"(parity), "r"(20000u)
-        : "memory");
-    return ok != 0;
-  };
-  if (poll()) return true;
-  const uint64_t t0 = global_timer_ns();
-#pragma unroll 1
-  while (!poll())
-    if (global_timer_ns() - t0 > 2000000000ull) return false;
-  return true;
-}
-
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 __device__ __forceinline__ float tree_exp2(float x) {   // relative error 2^-22, denormal results are zero

@@ -26,14 +26,18 @@ MAX_TREE_TOKENS = 64
 _TORCH_LIB = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libq3torch.so")
 
 
-def _register() -> bool:
-    """Load the bindings and register what tracing needs; False while they are not built (or half built)."""
-    if not (os.path.exists(_TORCH_LIB) and os.path.exists(_lib.LIB_PATH)):
-        return False
-    try:
-        torch.ops.load_library(_TORCH_LIB)
-    except OSError:
-        return False
+_registered = False
+
+
+def _register() -> None:
+    """Load the bindings and register what tracing needs: with the first call of an op, not with the import, so that a
+    process that imports the package to build the libraries does not hold the old ones."""
+    global _registered
+    _lib.load()
+    if not os.path.exists(_TORCH_LIB):
+        raise _lib.Q3Error(f"q3attn PyTorch bindings not built ({_TORCH_LIB} missing): run `python -m q3attn.build` from "
+                           "qwen3-tts-engine_b200/ or __graft_entry__.build()")
+    torch.ops.load_library(_TORCH_LIB)
     fake = torch.library.register_fake
     fake("q3attn::kv_quant_append_slots", lambda *a, **kw: None)
     fake("q3attn::kv_quant_append_paged", lambda *a, **kw: None)
@@ -44,19 +48,13 @@ def _register() -> bool:
     fake("q3attn::token_logprobs", lambda x, ids, top_n=0, temperature=1.0: (
         x.new_empty(ids.shape, dtype=torch.float32), x.new_empty(x.shape[0], dtype=torch.float32),
         x.new_empty(x.shape[0], top_n, dtype=torch.int64), x.new_empty(x.shape[0], top_n, dtype=torch.float32)))
-    return True
-
-
-_registered = _register()
+    _registered = True
 
 
 def _op(name):
-    """The op `q3attn::name`; raises while the library is not built."""
-    global _registered
+    """The op `q3attn::name`."""
     if not _registered:
-        _registered = _register()
-        if not _registered:
-            raise _lib.Q3Error("q3attn libraries not built: run `python -m q3attn.build` from qwen3-tts-engine_b200/")
+        _register()
     return getattr(torch.ops.q3attn, name).default
 
 
