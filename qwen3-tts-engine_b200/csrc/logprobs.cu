@@ -10,7 +10,7 @@
 // preserving bits above the complement of the id, all different.
 //
 // Bound: HBM (the logits are read once). A row is shared by a cluster of 1 to 8 CTAs when there are few rows; every
-// CTA streams its part in tiles of 512 16-byte vectors, the next tile's loads in flight while one is worked on; the
+// CTA streams its part in tiles of 1024 16-byte vectors, the next tile's loads in flight while one is worked on; the
 // arithmetic is packed in pairs, one exponential per logit.
 // Selection needs no pass of its own. m is a thread's largest value; the n-th largest maximum of 128 groups of two
 // threads bounds the top n from below, and only the few threads that reach it (n to 2n of 256) have their vectors
@@ -33,11 +33,11 @@ namespace {
 typedef unsigned long long Key;
 
 constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
-constexpr int kLpVecs = 2;                          // 16-byte vectors per thread and tile
+constexpr int kLpVecs = 4;                          // 16-byte vectors per thread and tile
 constexpr int kLpTileVecs = kLpThreads * kLpVecs;
 constexpr int kLpGroups = kLpThreads / 2;           // two threads a group
 constexpr int kLpMaxElems = 8 * kLpVecs;            // values per thread and tile, 16-bit types
-constexpr int kLpList = 2304;                       // >= kTopMax + kTopMax * 2 * kLpMaxElems
+constexpr int kLpList = 4224;                       // >= kTopMax + kTopMax * 2 * kLpMaxElems
 constexpr int kLpSlack = 64;                        // the list is cut back when it holds n + this many
 constexpr int kLpMaxCluster = 8;
 static_assert(kLpList >= kLogprobMaxTop + kLogprobMaxTop * 2 * kLpMaxElems && kLpGroups >= 2 * kLogprobMaxTop, "list");
@@ -430,10 +430,10 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobAr
   }
 }
 
-// CTAs per row: enough for about four waves of the GPU's 4 CTAs per SM, as long as each keeps two tiles.
+// CTAs per row: enough for at least two waves of the GPU's 4 CTAs per SM, as long as each keeps two tiles.
 int logprob_parts(long long rows, int vocab, int elem_bytes, int num_sms) {
   int parts = 1;
-  while (parts < kLpMaxCluster && rows * parts < 16ll * num_sms &&
+  while (parts < kLpMaxCluster && rows * parts < 8ll * num_sms &&
          static_cast<long long>(vocab) * elem_bytes >= 2ll * 2 * parts * kLpTileVecs * 16)
     parts *= 2;
   return parts;
