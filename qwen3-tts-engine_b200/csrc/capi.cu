@@ -799,7 +799,7 @@ int q3_kv_quant_append_slots(const void* k, const void* v, int64_t row_stride, c
   a.k_rows = static_cast<const __nv_bfloat16*>(k);
   a.v_rows = static_cast<const __nv_bfloat16*>(v);
   a.rows_stride = row_stride;
-  return record(q3::launch_kv_quant_append(a, sm_count(dev), static_cast<cudaStream_t>(stream)));
+  return record(q3::launch_kv_quant_append(a, static_cast<cudaStream_t>(stream)));
 }
 
 int q3_kv_quant_append_paged(const void* k, const void* v, int64_t row_stride, const q3_quant_cache* cache,
@@ -815,7 +815,7 @@ int q3_kv_quant_append_paged(const void* k, const void* v, int64_t row_stride, c
   a.k_rows = static_cast<const __nv_bfloat16*>(k);
   a.v_rows = static_cast<const __nv_bfloat16*>(v);
   a.rows_stride = row_stride;
-  return record(q3::launch_kv_quant_append(a, sm_count(dev), static_cast<cudaStream_t>(stream)));
+  return record(q3::launch_kv_quant_append(a, static_cast<cudaStream_t>(stream)));
 }
 
 int q3_kv_dequant_paged(const q3_quant_cache* cache, int32_t num_kv_heads, int32_t head_dim, const int32_t* positions,
@@ -829,7 +829,7 @@ int q3_kv_dequant_paged(const q3_quant_cache* cache, int32_t num_kv_heads, int32
   if (rc != Q3_OK) return rc;
   if ((rc = quant_common(a, cache, num_kv_heads, head_dim, k_out, v_out, out_row_stride, n_rows, &dev)) != Q3_OK) return rc;
   return record(q3::launch_kv_dequant(a, static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out),
-                                      out_row_stride, sm_count(dev), static_cast<cudaStream_t>(stream)));
+                                      out_row_stride, static_cast<cudaStream_t>(stream)));
 }
 
 size_t q3_paged_tree_workspace_bytes(int32_t batch, int32_t tokens, int32_t quantised) {
@@ -916,7 +916,7 @@ int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_
 int q3_token_logprobs(const q3_logprobs* p, void* stream) {
   if (!p || p->rows < 0 || p->rows > (1ll << 27)) return Q3_ERR_INVALID;
   if (p->vocab < 1 || p->vocab > (1 << 30) || p->given < 0 || p->top_n < 0 || p->top_n > p->vocab ||
-      !(p->temperature > 0.f) || p->logits_dtype < 0 || p->logits_dtype > 2)
+      !(p->temperature >= 1e-30f && p->temperature <= 1e30f) || p->logits_dtype < 0 || p->logits_dtype > 2)
     return Q3_ERR_INVALID;
   if (p->top_n > q3::kLogprobMaxTop) return Q3_ERR_UNSUPPORTED;
   if (p->rows == 0) return Q3_OK;

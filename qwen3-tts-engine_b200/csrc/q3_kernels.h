@@ -94,9 +94,9 @@ struct KvQuantArgs {
   int max_pages;
   uint32_t* status;
 };
-cudaError_t launch_kv_quant_append(const KvQuantArgs& a, int num_sms, cudaStream_t stream);
+cudaError_t launch_kv_quant_append(const KvQuantArgs& a, cudaStream_t stream);
 cudaError_t launch_kv_dequant(const KvQuantArgs& a, __nv_bfloat16* k_out, __nv_bfloat16* v_out, long long out_stride,
-                              int num_sms, cudaStream_t stream);
+                              cudaStream_t stream);
 
 // Attention of up to 64 drafted tokens per seat over the paged cache and each other (paged_tree.cu); decode attention
 // over the 8-bit cache with tokens = 1 and no draft rows.
