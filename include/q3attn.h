@@ -379,7 +379,7 @@ typedef struct q3_logprobs {
   int64_t row_stride;
   int64_t rows;                /* <= 2^27 */
   int32_t vocab;               /* <= 2^30 */
-  float temperature;           /* > 0 */
+  float temperature;           /* 1e-30 to 1e30 */
   const int64_t* ids;          /* [rows, given], rows ids_row_stride apart */
   int64_t ids_row_stride;
   int32_t given;

@@ -174,7 +174,7 @@ Tensor attend(const Tensor& q_, q3_tree_attn& p, const Tensor& kc, const Tensor&
                                                                             static_cast<int32_t>(T), ks.has_value()))},
                         q.options().dtype(ScalarType::Byte));
   p.q = q.data_ptr();
-  p.q_seat_stride = q.stride(0);
+  p.q_seat_stride = B == 1 ? T * kHeads * kDim : q.stride(0);
   p.q_token_stride = T == 1 ? kHeads * kDim : q.stride(1);
   p.k_pool = kc.data_ptr();
   p.v_pool = vc.data_ptr();
@@ -238,7 +238,7 @@ Tensor tree_attn(const Tensor& q, const Tensor& k_, const Tensor& v_, const Tens
   }
   p.k_new = k.data_ptr();
   p.v_new = v.data_ptr();
-  p.kv_new_seat_stride = k.stride(0);
+  p.kv_new_seat_stride = B == 1 ? T * kKvHeads * kDim : k.stride(0);
   p.kv_new_token_stride = T == 1 ? kKvHeads * kDim : k.stride(1);
   p.tree_mask = mask.data_ptr<int64_t>();
   p.tree_mask_stride = mask.dim() == 2 ? mask.stride(0) : 0;
@@ -255,10 +255,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
               "q3attn: logits must be [rows, vocab]");
   const int64_t n = logits.size(0), V = logits.size(1);
   TORCH_CHECK(top_n >= 0 && top_n <= 64 && top_n <= V, "q3attn: top_n must be 0 to 64, and no more than the vocabulary");
-  TORCH_CHECK(temperature > 0, "q3attn: temperature must be positive");
+  TORCH_CHECK(temperature >= 1e-30 && temperature <= 1e30, "q3attn: temperature must be 1e-30 to 1e30");
   on_device(ids_, "ids", logits);
   TORCH_CHECK(ids_.scalar_type() == ScalarType::Long && (ids_.dim() == 1 || ids_.dim() == 2) && ids_.size(0) == n,
               "q3attn: ids must be int64 [rows] or [rows, given]");
+  TORCH_CHECK(n <= (1 << 27) && (ids_.dim() == 1 || ids_.size(1) <= INT32_MAX), "q3attn: too many rows or ids");
   c10::cuda::OptionalCUDAGuard guard(logits.device());
   const Tensor x = (V == 1 || logits.stride(1) == 1) && (n <= 1 || logits.stride(0) >= V) ? logits : logits.contiguous();
   const Tensor ids = ids_.is_contiguous() ? ids_ : ids_.contiguous();
