@@ -11,13 +11,16 @@
 //
 // Bound: HBM (the logits are read once). A row is shared by a cluster of 1 to 8 CTAs when there are few rows; every
 // CTA streams its part in tiles of 1024 16-byte vectors, the next tile's loads in flight while one is worked on; the
-// arithmetic is packed in pairs, one exponential per logit.
+// arithmetic is packed in pairs, one exponential per logit. 1030 bf16 rows of 151000 without alternatives: 64 us, 4.9
+// TB/s (tiles of 512 vectors: 71); with the top 20: 74 us; one row of 151000 with the top 64: 17 us.
 // Selection needs no pass of its own. m is a thread's largest value; the n-th largest maximum of 128 groups of two
 // threads bounds the top n from below, and only the few threads that reach it (n to 2n of 256) have their vectors
-// read again, out of the L2 cache, shared out over all threads. Rows where more than the list holds reach the bound
+// read again, out of the L2 cache, shared out over all threads; a thread keeps the maxima of eight segments of its
+// tiles, and only segments that reach the bound are read (all of them: the top 20 above take 83 us, the top 64 124
+// instead of 88). Rows where more than the list holds reach the bound
 // (massive ties, fewer than n logits above -inf, values in one thread's vectors) take select_tiles, which is bounded for
 // every row: it goes through the tiles with the n-th best key so far, and where nearly all threads have candidates the
-// n-th largest group maximum of the tile is a bound first, so that a tile adds n * 2 threads * 16 values at most.
+// n-th largest group maximum of the tile is a bound first, so that a tile adds n * 2 threads * 32 values at most.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -39,6 +42,7 @@ constexpr int kLpGroups = kLpThreads / 2;           // two threads a group
 constexpr int kLpMaxElems = 8 * kLpVecs;            // values per thread and tile, 16-bit types
 constexpr int kLpList = 4224;                       // >= kTopMax + kTopMax * 2 * kLpMaxElems
 constexpr int kLpSlack = 64;                        // the list is cut back when it holds n + this many
+constexpr int kLpSegs = 8;                          // segments of a CTA's tiles
 constexpr int kLpMaxCluster = 8;
 static_assert(kLpList >= kLogprobMaxTop + kLogprobMaxTop * 2 * kLpMaxElems && kLpGroups >= 2 * kLogprobMaxTop, "list");
 
@@ -132,7 +136,8 @@ struct LpShared {
   Key bound;                      // only keys above it can be among the top n
   uint32_t bound_bits;
   int count, reaching;
-  uint8_t who[kLpThreads];        // the threads whose maximum reaches bound_bits
+  uint32_t seg_bits[kLpSegs][kLpThreads];   // order bits of every thread's maximum in each segment
+  uint16_t who[kLpSegs * kLpThreads];       // (segment, thread) pairs whose maximum reaches bound_bits
 };
 
 // The list cut back to its n largest keys, best first, and the bound raised to the n-th. By all threads; m = the
@@ -278,6 +283,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobAr
   // ---- one pass: the thread's (m, s, t), s and t in two halves
   float m = -INFINITY;
   float2 s2 = make_float2(0.f, 0.f), t2 = s2;
+  const int tiles = (part.v1 - part.v0 + kLpTileVecs - 1) / kLpTileVecs, seg_tiles = (tiles + kLpSegs - 1) / kLpSegs;
+  int seg = 0, left = seg_tiles;
+  float seg_top = -INFINITY;
   uint4 next[kLpVecs];
 #pragma unroll
   for (int j = 0; j < kLpVecs; ++j) next[j] = part.load(part.v0 + j * kLpThreads + tid);
@@ -292,6 +300,12 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobAr
     float top = Vec<T>::top(w[0]);
 #pragma unroll
     for (int j = 1; j < kLpVecs; ++j) top = max_nan(top, Vec<T>::top(w[j]));
+    seg_top = max_nan(seg_top, top);
+    if (--left == 0 || tile + kLpTileVecs >= part.v1) {
+      sh.seg_bits[seg++][tid] = order_bits(seg_top);
+      seg_top = -INFINITY;
+      left = seg_tiles;
+    }
     if (!(top <= m)) {
       const float d = fmaxf((m - top) * c, -1000.f), f = exp2_fast(d);   // nothing yet: s = t = 0
       t2 = make_float2(f * (t2.x + d * s2.x), f * (t2.y + d * s2.y));
@@ -349,12 +363,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobAr
     }
     __syncthreads();
     const uint32_t bound = sh.bound_bits;
-    if (bits >= bound) sh.who[atomicAdd(&sh.reaching, 1)] = static_cast<uint8_t>(tid);
+    if (bits >= bound)
+      for (int k = 0; k < seg; ++k)
+        if (sh.seg_bits[k][tid] >= bound) sh.who[atomicAdd(&sh.reaching, 1)] = static_cast<uint16_t>(k * kLpThreads + tid);
     __syncthreads();
-    const int reaching = sh.reaching;
-    const int items = reaching * ((part.v1 - part.v0 + kLpThreads - 1) / kLpThreads);
+    const int reaching = sh.reaching, items = reaching * seg_tiles * kLpVecs;
     for (int i = tid; i < items; i += kLpThreads) {
-      const int v = part.v0 + i / reaching * kLpThreads + sh.who[i % reaching];
+      const int who = sh.who[i % reaching];
+      const int v = part.v0 + (who / kLpThreads * seg_tiles * kLpVecs + i / reaching) * kLpThreads + who % kLpThreads;
       const uint4 w = part.load(v);
       if (order_bits(Vec<T>::top(w)) < bound) continue;
 #pragma unroll
@@ -404,10 +420,29 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobAr
         sh.total = r;
       }
       if (n > 0) {
-        for (int i = tid; i < parts * n; i += kLpThreads) sh.list[i] = cluster.map_shared_rank(&sh, i / n)->best[i % n];
+        // with j = ceil(n / parts), at least n keys are as large as the least of the parts' j-th (0: a part has fewer)
+        if (warp == 0) {
+          Key k = lane < parts ? cluster.map_shared_rank(&sh, lane)->best[(n + parts - 1) / parts - 1] : ~0ull;
+#pragma unroll
+          for (int o = kLpMaxCluster / 2; o > 0; o >>= 1) {
+            const Key other = __shfl_xor_sync(0xffffffffu, k, o);
+            k = other < k ? other : k;
+          }
+          if (lane == 0) {
+            sh.bound = k;
+            sh.count = 0;
+          }
+        }
         __syncthreads();
-        // empty places (0) of short parts rank last; the row has n values at least
-        cut_list(sh, n, parts * n);
+        const Key bound = sh.bound;
+        for (int i = tid; i < parts * n; i += kLpThreads) {
+          const Key k = cluster.map_shared_rank(&sh, i / n)->best[i % n];
+          if (k >= bound && k != 0ull) sh.list[atomicAdd(&sh.count, 1)] = k;
+        }
+        __syncthreads();
+        const int found = sh.count;
+        __syncthreads();
+        cut_list(sh, n, found);
       }
       __syncthreads();
     }
@@ -430,10 +465,12 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobAr
   }
 }
 
-// CTAs per row: enough for at least two waves of the GPU's 4 CTAs per SM, as long as each keeps two tiles.
+// CTAs per row: as few as fill three quarters of the 4 CTAs that an SM holds (every CTA ends with a selection, which costs
+// more than an uneven last wave), as long as each keeps two tiles. The top 20 of 1030 bf16 rows of 151000: one CTA a row
+// 83 us, two 98; of 250: two 33, four 40.
 int logprob_parts(long long rows, int vocab, int elem_bytes, int num_sms) {
   int parts = 1;
-  while (parts < kLpMaxCluster && rows * parts < 8ll * num_sms &&
+  while (parts < kLpMaxCluster && rows * parts < 3ll * num_sms &&
          static_cast<long long>(vocab) * elem_bytes >= 2ll * 2 * parts * kLpTileVecs * 16)
     parts *= 2;
   return parts;

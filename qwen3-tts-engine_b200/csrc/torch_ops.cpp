@@ -141,10 +141,11 @@ std::tuple<Tensor, Tensor> dequant_paged(const Tensor& kc, const Tensor& vc, con
   return {k, v};
 }
 
-// Fills what both attention ops share and runs: q [B, T, 16, 128].
+// Fills what both attention ops share and runs: q [B, 16, 128] (T = 1) or [B, T, 16, 128].
 Tensor attend(const Tensor& q_, q3_tree_attn& p, const Tensor& kc, const Tensor& vc, const std::optional<Tensor>& ks,
               const std::optional<Tensor>& vs, const Tensor& seqlens, const Tensor& bt, double scale) {
-  const int64_t B = q_.size(0), T = q_.size(1);
+  const bool drafts = q_.dim() == 4;
+  const int64_t B = q_.size(0), T = drafts ? q_.size(1) : 1;
   TORCH_CHECK(q_.scalar_type() == ScalarType::BFloat16, "q3attn: q must be bfloat16");
   TORCH_CHECK(B <= INT32_MAX, "q3attn: too many seats");
   TORCH_CHECK(ks.has_value() == vs.has_value(), "q3attn: k_scale and v_scale go together");
@@ -165,10 +166,9 @@ Tensor attend(const Tensor& q_, q3_tree_attn& p, const Tensor& kc, const Tensor&
   TORCH_CHECK(seqlens.scalar_type() == ScalarType::Int && seqlens.numel() == B && seqlens.is_contiguous(),
               "q3attn: cache_seqlens must be a contiguous int32 tensor [B]");
   c10::cuda::OptionalCUDAGuard guard(q_.device());
-  const bool rows = q_.stride(3) == 1 && q_.stride(2) == kDim && (T == 1 || q_.stride(1) >= kHeads * kDim) &&
-                    q_.stride(0) >= 0;
+  const bool rows = q_.stride(-1) == 1 && q_.stride(-2) == kDim && (T == 1 || q_.stride(1) >= kHeads * kDim);
   const Tensor q = rows ? q_ : q_.contiguous();
-  Tensor out = at::empty({B, T, kHeads, kDim}, q.options());
+  Tensor out = at::empty(q.sizes(), q.options());
   if (B == 0) return out;
   Tensor ws = at::empty({static_cast<int64_t>(q3_paged_tree_workspace_bytes(static_cast<int32_t>(B),
                                                                             static_cast<int32_t>(T), ks.has_value()))},
@@ -204,7 +204,7 @@ Tensor decode_quant(const Tensor& q, const Tensor& kc, const Tensor& vc, const T
   on_device(q, "q", q);
   TORCH_CHECK(q.dim() == 3 && q.size(1) == kHeads && q.size(2) == kDim, "q3attn: q must be [B, 16, 128], got ", q.sizes());
   q3_tree_attn p{};
-  return attend(q.unsqueeze(1), p, kc, vc, ks, vs, seqlens, bt, scale).squeeze(1);
+  return attend(q, p, kc, vc, ks, vs, seqlens, bt, scale);
 }
 
 Tensor tree_attn(const Tensor& q, const Tensor& k_, const Tensor& v_, const Tensor& mask_, const Tensor& kc,
