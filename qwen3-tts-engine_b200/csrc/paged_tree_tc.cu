@@ -15,22 +15,26 @@
 //                 takes a warp longer than the tile's bytes take HBM, so the warps take tiles in turn.
 //   loaders (4/8) turn raw e4m3 tiles into bf16 operands (exact: four significant bits times a power of two); write the
 //                 drafted rows (the last tile of a seat); zero V rows past a seat's last token.
-//   MMA (1)       one thread issues S(t+1) before P(t) V(t), so the tensor core works while the softmax does.
+//   MMA (2)       one issues S(t), up to three tiles ahead of the softmax (three S / P buffers), the other P(t) V(t).
 //   softmax (2 x 4) set t & 1 takes tile t: thread r of a set owns row r: online softmax with a lazy maximum (the set's O is
 //                 rescaled in TMEM when it grows by more than 2^8), P(t) as bf16 into TMEM over S(t). Each set has an O,
 //                 maximum and sum of its own, so that the sets never wait for one another within a seat (one set alone
 //                 took 2000 cycles a tile, most of them latency, where HBM takes 1424); at a seat's end both add the two
-//                 up, half of the dims each, to the output or as a partial to the workspace. They also write Q into TMEM
+//                 up, half of the dims each, to the output or as a partial to the workspace. The set with a seat's last
+//                 tile writes the next seat's Q into TMEM
 //                 (with Q in shared memory an S took 600 cycles: the tensor core reads 6 KB per 16 dims instead of 2).
 //                 Warps without live rows have no part in any of it.
+// Five kinds of warps in one kernel miss the instruction cache: long waits are calls out of line, rows that see part of
+// a tile are masked in TMEM by a small loop of their own, and the e4m3 path is rolled up (96 seats of 1200 to 2400 rows,
+// 32 tokens: bf16 193 -> 149 us, e4m3 282 -> 208).
 // An infinity or NaN in a drafted V row would reach rows that do not see it as 0 * inf: the loaders write zero in its
 // place and raise a flag, and the rows that do see it get it back at the end.
 //
 // Bound: HBM for few tokens; for 64 the exponentials come near it (128 x 64 per tile against 32 KB of K and V: 512 of
-// 1424 cycles of the SM's share of the measured copy rate).
+// 1424 cycles of the SM's share of the measured copy rate). 24 seats x 64 tokens x 1000 to 8000 rows, bf16: 104 us, 4.2
+// TB/s; e4m3 is bound by instruction issue (the conversion to bf16 and the softmax: half of all issue slots).
 #include <cuda.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include <cstring>
 
@@ -45,8 +49,10 @@ namespace {
 constexpr int kTcRows = 64;                     // keys per tile (cached rows, or all drafted rows)
 constexpr int kTcTok = kTreeMaxTokens;          // tokens per item: the whole draft
 constexpr int kTcTmemCols = 512;
-// S(t), P(t) at column 64 (t & 1); O of set s at 128 + 128 s; Q of item i at 384 + 64 (i & 1)
-constexpr uint32_t kTcOCol = 128, kTcQCol = 384;
+constexpr int kTcScores = 3;                    // S / P buffers
+// S(t), P(t) at column 64 (t % 3); Q after them; O of set s at 256 + 128 s
+constexpr uint32_t kTcQCol = 64 * kTcScores, kTcOCol = 256;
+static_assert(kTcQCol + 64 <= kTcOCol && kTcOCol + 256 <= kTcTmemCols, "TMEM columns");
 constexpr int kTcOddSlots = 16;                 // more than the stages: see where it is read
 constexpr int kTcLoaderWarp = 8;                // after the softmax warps 0-7
 
@@ -66,8 +72,8 @@ struct TcSmem {
   static constexpr int kMl = kRaw + kRawSlots * kRawBytes;   // (maximum, sum) of each set's rows, by item & 1
   static constexpr int kBars = kMl + 2 * 2 * 128 * 8;
   static constexpr int kFull = 0, kEmpty = kStages, kCopied = 2 * kStages, kRawFree = kCopied + kCopySlots,
-                       kSFull = kRawFree + kRawSlots, kPFull = kSFull + 2, kPvDone = kPFull + 2, kQFull = kPvDone + 2,
-                       kOFree = kQFull + 2, kSets = kOFree + 1, kFinal = kSets + 4, kNumBars = kFinal + 2;
+                       kSFull = kRawFree + kRawSlots, kPFull = kSFull + kTcScores, kPvDone = kPFull + kTcScores,
+                       kQFull = kPvDone + kTcScores, kOFree = kQFull + 1, kSets = kOFree + 1, kFinal = kSets + 4, kNumBars = kFinal + 2;
   static constexpr int kTmemSlot = kBars + 8 * kNumBars;
   static constexpr int kAbort = kTmemSlot + 4;
   static constexpr int kIssued = kAbort + 4;                 // per copy warp, 1 + its last tile issued (abort path)
@@ -93,24 +99,27 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ bool tc_poll(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(20000u)
+      : "memory");
+  return ok != 0;
+}
 // Wait for phase `parity` of `bar`; false after 2 s or once another role has raised the abort flag. The waits sleep in the
 // barrier (up to 20 us at a time): 14 to 16 warps that poll instead take the issue slots the softmax warps need.
-__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  auto poll = [&]() -> bool {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_addr(bar)), "r"(parity), "r"(20000u)
-        : "memory");
-    return ok != 0;
-  };
-  if (poll()) return true;
+__device__ __noinline__ bool tc_wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   const uint64_t t0 = global_timer_ns();
 #pragma unroll 1
-  while (!poll())
+  while (!tc_poll(bar, parity))
     if (*abort_flag || global_timer_ns() - t0 > 2000000000ull) return false;
   return true;
+}
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  const uint32_t b = smem_addr(bar);
+  return __builtin_expect(tc_poll(b, parity), 1) || tc_wait_on(b, parity, abort_flag);
 }
 
 // 16 consecutive 32-bit columns of this thread's TMEM lane.
@@ -121,6 +130,19 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[1
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
       "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+
+// 8 consecutive 32-bit columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "f"(v[0]), "f"(v[1]),
+               "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
 }
 
 // D += A B with A in TMEM, issued by the lane whose `leader` is not 0. The whole warp runs the code around it, so that
@@ -175,7 +197,7 @@ __device__ __forceinline__ void tc_enter(const TreePlan& P, TcCursor& c) {
 }
 // To tile k >= the present one; true when that is another item.
 __device__ __forceinline__ bool tc_seek(const TreeArgs& a, const TreePlan& P, TcCursor& c, int k) {
-  if (k < c.end) return false;
+  if (__builtin_expect(k < c.end, 1)) return false;
   while (P.c0 + k >= c.first + c.it.n) {
     c.first += c.it.n;
     c.it = tree_item<kTcTok, kTcRows, kTcTok>(a, ++c.w);
@@ -353,25 +375,29 @@ struct TcLoader {
     const int u = tid & 7;
     // dims 16u .. + 15 are units 2u and 2u + 1; the lanes of the second half write the odd unit first (banks)
     const bool swap = u >= 4;
-    uint4 w[kPer];
-    uint32_t s[kPer];
+    static_assert(kPer % 2 == 0, "two pieces at a time");
+#pragma unroll 1
+    for (int x0 = 0; x0 < kPer; x0 += 2) {   // rows 0 .. 63 are K's, 64 .. 127 V's
+      uint4 w[2];
+      uint32_t s[2];
 #pragma unroll
-    for (int x = 0; x < kPer; ++x) {   // rows 0 .. 63 are K's, 64 .. 127 V's
-      const int i = (tid >> 3) + kStep * x;
-      w[x] = *reinterpret_cast<const uint4*>(raw + i * kHeadDim + u * 16);
-      s[x] = raw[2 * kTcRows * kHeadDim + i * kKvHeads + h];
-    }
+      for (int x = 0; x < 2; ++x) {
+        const int i = (tid >> 3) + kStep * (x0 + x);
+        w[x] = *reinterpret_cast<const uint4*>(raw + i * kHeadDim + u * 16);
+        s[x] = raw[2 * kTcRows * kHeadDim + i * kKvHeads + h];
+      }
 #pragma unroll
-    for (int x = 0; x < kPer; ++x) {
-      const int i = (tid >> 3) + kStep * x, r = i % kTcRows;
-      const float sc = e8m0_to_float(s[x]);
-      const float2 f = make_float2(sc, sc);
-      const uint2 p0 = dequant4(w[x].x, f), p1 = dequant4(w[x].y, f), p2 = dequant4(w[x].z, f), p3 = dequant4(w[x].w, f);
-      uint4 lo = make_uint4(p0.x, p0.y, p1.x, p1.y), hi = make_uint4(p2.x, p2.y, p3.x, p3.y);
-      if (r >= real) lo = hi = make_uint4(0, 0, 0, 0);
-      const uint32_t first = dst + i / kTcRows * SM::kTile + tc_unit(r, 2 * u + swap, SM::kHalf);
-      st_shared16(first, swap ? hi : lo);
-      st_shared16(first ^ 16u, swap ? lo : hi);
+      for (int x = 0; x < 2; ++x) {
+        const int i = (tid >> 3) + kStep * (x0 + x), r = i % kTcRows;
+        const float sc = e8m0_to_float(s[x]);
+        const float2 f = make_float2(sc, sc);
+        const uint2 p0 = dequant4(w[x].x, f), p1 = dequant4(w[x].y, f), p2 = dequant4(w[x].z, f), p3 = dequant4(w[x].w, f);
+        uint4 lo = make_uint4(p0.x, p0.y, p1.x, p1.y), hi = make_uint4(p2.x, p2.y, p3.x, p3.y);
+        if (r >= real) lo = hi = make_uint4(0, 0, 0, 0);
+        const uint32_t first = dst + i / kTcRows * SM::kTile + tc_unit(r, 2 * u + swap, SM::kHalf);
+        st_shared16(first, swap ? hi : lo);
+        st_shared16(first ^ 16u, swap ? lo : hi);
+      }
     }
   }
 
@@ -438,12 +464,12 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
     }
     for (int i = 0; i < SM::kCopySlots; ++i) mbar_init(&bars[SM::kCopied + i], FP8 ? 33 : 1);   // + a lane's scales each
     for (int i = 0; i < SM::kRawSlots; ++i) mbar_init(&bars[SM::kRawFree + i], SM::kLoaders);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kTcScores; ++i) {
       mbar_init(&bars[SM::kSFull + i], 1);
       mbar_init(&bars[SM::kPFull + i], live_warps);
       mbar_init(&bars[SM::kPvDone + i], 1);
-      mbar_init(&bars[SM::kQFull + i], live_warps);
     }
+    mbar_init(&bars[SM::kQFull], live_warps);
     mbar_init(&bars[SM::kOFree], 2 * live_warps);
     for (int i = 0; i < 4; ++i) mbar_init(&bars[SM::kSets + i], 2);
     for (int i = 0; i < 2; ++i) mbar_init(&bars[SM::kFinal + i], 1);
@@ -486,25 +512,23 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
     auto wait = [&](int bar, int phase) {
       return __all_sync(0xffffffffu, tc_wait(&bars[bar], static_cast<uint32_t>(phase & 1), abort_flag));
     };
-    int stage = 0, lap = 0;
+    int stage = 0, lap = 0, b = 0, use = 0;   // operand stage and score buffer of tile k, and how often they came round
     for (int k = 0; k < n; ++k) {
       if (scores) {
         const bool starts = tc_seek(a, P, cur, k) || k == 0;
-        ok = (!starts || wait(SM::kQFull + (cur.index & 1), cur.index >> 1)) && wait(SM::kFull + stage, lap) &&
-             (FP8 || wait(SM::kCopied + stage, lap)) &&
-             (k < 2 || wait(SM::kPvDone + (k & 1), (k - 2) >> 1));   // P(k - 2) lay where S(k) goes
+        ok = (!starts || wait(SM::kQFull, cur.index)) && wait(SM::kFull + stage, lap) && (FP8 || wait(SM::kCopied + stage, lap)) &&
+             (use == 0 || wait(SM::kPvDone + b, use - 1));   // P(k - 3) lay where S(k) goes
         if (!ok) break;
         tc_fence_after();
         const uint64_t kk = dk + stage * (2 * SM::kTile >> 4);
-        const uint32_t t_s = tmem + 64u * static_cast<uint32_t>(k & 1), t_q = tmem + kTcQCol + 64u * static_cast<uint32_t>(cur.index & 1);
+        const uint32_t t_s = tmem + 64u * static_cast<uint32_t>(b), t_q = tmem + kTcQCol;
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks)
           tc_mma_tmem_a(leader, t_s, t_q + 8u * ks, kk + ((ks >> 2) * SM::kHalf + (ks & 3) * 32) / 16, kIdescQK, ks > 0);
-        tc_commit(leader, bar0 + 8 * (SM::kSFull + (k & 1)));
+        tc_commit(leader, bar0 + 8 * (SM::kSFull + b));
       } else {
-        const int b = k & 1;
         const bool next = tc_seek(a, P, cur, k);
-        ok = wait(SM::kPFull + b, k >> 1) && (!next || wait(SM::kOFree, cur.index - 1)) &&   // the last item's O has been read
+        ok = wait(SM::kPFull + b, use) && (!next || wait(SM::kOFree, cur.index - 1)) &&   // the last item's O has been read
              wait(SM::kFull + stage, lap) && (FP8 || wait(SM::kCopied + stage, lap));
         if (!ok) break;
         tc_fence_after();
@@ -512,13 +536,17 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
         const uint32_t more = k < cur.begin + 2 ? 0u : 1u;   // 0: a set's first tile of the item
 #pragma unroll
         for (int ks = 0; ks < kTcRows / 16; ++ks)
-          tc_mma_tmem_a(leader, tmem + kTcOCol + 128u * b, tmem + 64u * b + 8u * ks, v + ks * (2048 / 16), kIdescPV, more | ks);
+          tc_mma_tmem_a(leader, tmem + kTcOCol + 128u * static_cast<uint32_t>(k & 1), tmem + 64u * static_cast<uint32_t>(b) + 8u * ks, v + ks * (2048 / 16), kIdescPV, more | ks);
         tc_commit(leader, bar0 + 8 * (SM::kEmpty + stage));
         tc_commit(leader, bar0 + 8 * (SM::kPvDone + b));
       }
       if (++stage == kSt) {
         stage = 0;
         ++lap;
+      }
+      if (++b == kTcScores) {
+        b = 0;
+        ++use;
       }
     }
     if (!ok && lane == 0) tw_fail(a.status, abort_flag);
@@ -531,9 +559,8 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
     auto wait = [&](int bar, int phase) {
       return __all_sync(0xffffffffu, tc_wait(&bars[bar], static_cast<uint32_t>(phase & 1), abort_flag));
     };
-    // Row r of a seat's Q into the TMEM buffer of item `index`. The buffer's last user is two items back: a set gets to write
-    // it when it has read a score of the item between.
-    auto write_q = [&](int seat, int index) {
+    // Row r of a seat's Q into TMEM, by the set that has the last scores of the seat before (so every one has been formed).
+    auto write_q = [&](int seat) {
       const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<long long>(seat) * a.q_seat + static_cast<long long>(tok) * a.q_tok +
                                                        (2 * h + (r & 1)) * kHeadDim);
       const bool mine = r < 2 * a.tokens;
@@ -547,19 +574,18 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
           w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
         }
         __syncwarp();
-        tmem_st32u(tmem + kTcQCol + 64u * static_cast<uint32_t>(index & 1) + 32u * half + lane_base, w);
+        tmem_st32u(tmem + kTcQCol + 32u * half + lane_base, w);
       }
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[SM::kQFull + (index & 1)]);
+      if (lane == 0) mbar_arrive(&bars[SM::kQFull]);
     };
     TcCursor nxt = cur;
-    if (set == 0) write_q(cur.it.seat, 0);
+    if (set == 0) write_q(cur.it.seat);
     while (k < n && ok) {
       tc_seek(a, P, cur, k);
       const int begin = cur.begin, end = cur.end;
-      const int q_at = max(begin, end - 2);   // the tile at which its set writes the next seat's Q
       unsigned long long see = 0;
       if (tok < cur.it.drafts)
         see = static_cast<unsigned long long>(a.mask[static_cast<long long>(cur.it.seat) * a.mask_seat + tok]) &
@@ -567,29 +593,34 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
       float m_run = -INFINITY, l_run = 0.f;
       const int k0 = begin + ((begin ^ set) & 1);                  // the set's first tile
       for (k = k0; k < end && ok; k += 2) {
-        const int j = tc_chunk(cur, k);
-        if (k == q_at && end < n) {
-          tc_seek(a, P, nxt, end);
-          write_q(nxt.it.seat, nxt.index);
-        }
-        ok = wait(SM::kSFull + set, k >> 1);
+        const int j = tc_chunk(cur, k), b = k % kTcScores, use = k / kTcScores;
+        ok = wait(SM::kSFull + b, use);
         if (!ok) break;
         tc_fence_after();
+        if (k == end - 1 && end < n) {
+          tc_seek(a, P, nxt, end);
+          write_q(nxt.it.seat);
+        }
         const bool draft = j >= cur.it.nc;
         const int real = draft ? kTcRows : cur.it.len - j * kTcRows;
-        const uint32_t t_s = tmem + 64u * set + lane_base;
-        // 32 products, -inf where the row does not see the key
+        const bool masked = draft || real < kTcRows;
+        const unsigned long long keep = draft ? see : real < kTcRows ? (1ull << real) - 1 : ~0ull;   // real >= 1
+        const uint32_t t_s = tmem + 64u * static_cast<uint32_t>(b) + lane_base;
+        if (__builtin_expect(masked, 0)) {   // -inf where the row does not see the key
+#pragma unroll 1
+          for (int c = 0; c < kTcRows; c += 8) {
+            float x[8];
+            tmem_ld8(t_s + c, x);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = ((keep >> c >> i) & 1ull) ? x[i] : -INFINITY;
+            tmem_st8(t_s + c, x);
+          }
+          tc_wait_st();
+        }
         auto scores = [&](float (&x)[32], int half) {
           tmem_ld32(t_s + 32u * half, x);
           tc_wait_ld();
-          if (draft) {
-            const uint32_t bits = static_cast<uint32_t>(see >> (32 * half));
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = ((bits >> i) & 1u) ? x[i] : -INFINITY;
-          } else if (real < kTcRows) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = half * 32 + i < real ? x[i] : -INFINITY;
-          }
         };
         auto largest = [](const float (&x)[32]) {
           float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -601,10 +632,12 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
         float sv[FP8 ? 1 : 2][32];
         float cmax;
         if constexpr (FP8) {
-          scores(sv[0], 0);
-          cmax = largest(sv[0]);
-          scores(sv[0], 1);
-          cmax = fmaxf(cmax, largest(sv[0]));
+          cmax = -INFINITY;
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            scores(sv[0], half);
+            cmax = fmaxf(cmax, largest(sv[0]));
+          }
         } else {
           scores(sv[0], 0);
           scores(sv[1], 1);
@@ -619,7 +652,7 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
         float2 ls2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         m_run = m_new;
         // P(k) over S(k), columns 16 half .. + 15: the scores there have been read
-#pragma unroll
+#pragma unroll(FP8 ? 1 : 2)
         for (int half = 0; half < 2; ++half) {
           if constexpr (FP8) scores(sv[0], half);
           const float(&x)[32] = sv[FP8 ? 0 : half];
@@ -636,8 +669,10 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
         }
         const float2 ls = __fadd2_rn(ls2[0], ls2[1]);
         l_run = l_run * alpha + (ls.x + ls.y);
-        if (k > k0 && __any_sync(0xffffffffu, alpha != 1.f)) {   // a set's first tile of an item starts its O from zero
-          // the set's last P V is done: S(k) was issued after it
+        if (__builtin_expect(k > k0 && __any_sync(0xffffffffu, alpha != 1.f), 0)) {   // a set's first tile of an item starts its O from zero
+          ok = wait(SM::kPvDone + (k - 2) % kTcScores, (k - 2) / kTcScores);   // the set's last P V
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             float ov[32];
@@ -652,7 +687,7 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[SM::kPFull + set]);
+        if (lane == 0) mbar_arrive(&bars[SM::kPFull + b]);
       }
       k = end;
       if (!ok) break;
@@ -660,8 +695,8 @@ __global__ void __launch_bounds__(TcSmem<FP8>::kThreads, 1) paged_tree_tc_kernel
       set_ml[((cur.index & 1) * 2 + set) * 128 + r] = make_float2(m_run, l_run);
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[SM::kSets + (warp & 3)]);
-      ok = wait(SM::kSets + (warp & 3), cur.index) && wait(SM::kPvDone + ((end - 1) & 1), (end - 1) >> 1) &&
-           (end - begin < 2 || wait(SM::kPvDone + (end & 1), (end - 2) >> 1));
+      ok = wait(SM::kSets + (warp & 3), cur.index) && wait(SM::kPvDone + (end - 1) % kTcScores, (end - 1) / kTcScores) &&
+           (end - begin < 2 || wait(SM::kPvDone + (end - 2) % kTcScores, (end - 2) / kTcScores));
       if (!ok) break;
       tc_fence_after();
       const float2 other = set_ml[((cur.index & 1) * 2 + (set ^ 1)) * 128 + r];
