@@ -25,8 +25,8 @@
 //                 (with Q in shared memory an S took 600 cycles: the tensor core reads 6 KB per 16 dims instead of 2).
 //                 Warps without live rows have no part in any of it.
 // Five kinds of warps in one kernel miss the instruction cache: long waits are calls out of line, rows that see part of
-// a tile are masked in TMEM by a small loop of their own, and the e4m3 path is rolled up (96 seats of 1200 to 2400 rows,
-// 32 tokens: bf16 193 -> 149 us, e4m3 282 -> 208).
+// a tile are masked in TMEM by a small loop of their own, drafted rows come in by a function, and the e4m3 path is rolled
+// up (96 seats of 1200 to 2400 rows, 32 tokens: bf16 193 -> 149 us, e4m3 282 -> 200).
 // An infinity or NaN in a drafted V row would reach rows that do not see it as 0 * inf: the loaders write zero in its
 // place and raise a flag, and the rows that do see it get it back at the end.
 //
@@ -168,6 +168,15 @@ __device__ __forceinline__ uint32_t tc_elect() {
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
+  return v;
+}
+// 16 bytes of shared memory from `bytes` (16 or 0) bytes at src and zeros.
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -325,10 +334,37 @@ __device__ __forceinline__ void tc_copies(const TcParams& p, const TreePlan& P, 
 }
 
 // ------------------------------------------------------------------ the loader warps
+// A seat's drafted rows (one head of each, kv_tok elements apart) as one operand tile at dst, by 128 threads; true when a V
+// value was an infinity or NaN (zero is written in its place). Out of line, like all that runs once per seat.
+__device__ __noinline__ bool tc_load_draft(const __nv_bfloat16* k, const __nv_bfloat16* v, long long kv_tok, int drafts, uint32_t dst,
+                                           int v_off, int half, int tid) {
+  const int u = tid & 15;
+#pragma unroll 1
+  for (int r = tid >> 4; r < kTcRows; r += 8) {
+    const uint32_t at = dst + tc_unit(r, u, half), bytes = r < drafts ? 16u : 0u;   // 0: zeros
+    const long long off = min(r, drafts - 1) * kv_tok + 8 * u;
+    cp_async16_zfill(at, k + off, bytes);
+    cp_async16_zfill(at + v_off, v + off, bytes);
+  }
+  cp_async_wait_all();
+  bool odd = false;
+#pragma unroll 1
+  for (int r = tid >> 4; r < drafts; r += 8) {   // the thread's own pieces
+    const uint32_t at = dst + v_off + tc_unit(r, u, half);
+    const uint4 x = ld_shared16(at);
+    const uint4 f = make_uint4(finite_or_zero(x.x), finite_or_zero(x.y), finite_or_zero(x.z), finite_or_zero(x.w));
+    if (f.x != x.x || f.y != x.y || f.z != x.z || f.w != x.w) {
+      odd = true;
+      st_shared16(at, f);
+    }
+  }
+  return odd;
+}
+
 template <bool FP8>
 struct TcLoader {
   using SM = TcSmem<FP8>;
-  static constexpr int kThreads = 128, kRowStep = kThreads / 16;   // the first four warps: 16 threads per row of 256 bytes
+  static constexpr int kThreads = 128;   // of a drafted tile: the first four warps
   const TreeArgs& a;
   const TreePlan& P;
   uint32_t sbase;
@@ -360,7 +396,8 @@ struct TcLoader {
       wrote = true;
     }
     if (j >= c.it.nc && tid < kThreads) {
-      if (load_draft(c.it, dst)) odd[c.index % kTcOddSlots] = c.index + 1;
+      const long long off = static_cast<long long>(c.it.seat) * a.kv_seat + h * kHeadDim;
+      if (tc_load_draft(a.k_new + off, a.v_new + off, a.kv_tok, c.it.drafts, dst, SM::kTile, SM::kHalf, tid)) odd[c.index % kTcOddSlots] = c.index + 1;
       wrote = true;
     }
     if (wrote) fence_proxy_async_smem();   // this thread's writes before the tensor core reads
@@ -405,34 +442,6 @@ struct TcLoader {
     if (__all_sync(0xffffffffu, tc_wait(&bars[bar], parity, abort_flag))) return true;
     tw_fail(a.status, abort_flag);
     return false;
-  }
-  // The drafted rows as one tile; true when a V value was an infinity or NaN.
-  __device__ __forceinline__ bool load_draft(const TreeItem& it, uint32_t dst) {
-    const int u = tid & 15;
-    bool odd = false;
-#pragma unroll
-    for (int x0 = 0; x0 < kTcRows / kRowStep; x0 += 4) {
-      uint4 k[4], v[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int r = (tid >> 4) + kRowStep * (x0 + x);
-        k[x] = v[x] = make_uint4(0, 0, 0, 0);
-        if (r < it.drafts) {
-          const long long off = static_cast<long long>(it.seat) * a.kv_seat + static_cast<long long>(r) * a.kv_tok + h * kHeadDim;
-          k[x] = __ldg(reinterpret_cast<const uint4*>(a.k_new + off) + u);
-          v[x] = __ldg(reinterpret_cast<const uint4*>(a.v_new + off) + u);
-        }
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const uint32_t at = tc_unit((tid >> 4) + kRowStep * (x0 + x), u, SM::kHalf);
-        const uint4 f = make_uint4(finite_or_zero(v[x].x), finite_or_zero(v[x].y), finite_or_zero(v[x].z), finite_or_zero(v[x].w));
-        odd |= f.x != v[x].x || f.y != v[x].y || f.z != v[x].z || f.w != v[x].w;
-        st_shared16(dst + at, k[x]);
-        st_shared16(dst + SM::kTile + at, f);
-      }
-    }
-    return odd;
   }
 };
 

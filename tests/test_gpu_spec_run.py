@@ -9,7 +9,7 @@ import torch
 
 from helpers import bits_equal
 from oracle import spec as OSP
-from test_gpu_spec import BF, DEV, SCALE, check_attention, dev, expect_cache, gen, pools, rows, table_for, tree_case
+from test_gpu_spec import BF, DEV, SCALE, check_attention, dev, expect_cache, gen, pools, ref_tree, rows, run_tree, table_for, tree_case
 
 pytestmark = pytest.mark.gpu
 
@@ -263,6 +263,17 @@ def test_refusals(q3):
         with pytest.raises(RuntimeError, match="q3"):
             bad()
     torch.cuda.synchronize()
+    assert q3._lib.read_status() == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("T", [9, 33, 64])
+@pytest.mark.parametrize("lens", [[0] * 300, [0, 64, 0, 0, 65, 0, 0, 0, 64, 1] * 40, [128 if i % 7 == 0 else 0 for i in range(200)]])
+def test_short_seats_of_many_tokens(q3, fp8, T, lens):
+    """Many seats per CTA of one tile (the drafted rows) or a few."""
+    c = tree_case(len(lens), T, lens, 64, 71, fp8, drafts=[1 + (5 * i) % T for i in range(len(lens))])
+    got = run_tree(q3, c)
+    check_attention(got, ref_tree(c), [n + T for n in lens], fp8, True)
     assert q3._lib.read_status() == 0
 
 
