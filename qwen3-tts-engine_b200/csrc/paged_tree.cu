@@ -22,6 +22,9 @@
 // size, so a box never leaves its page), laid out [head or half head][R rows][128 bytes] with the 128-byte swizzle, which
 // makes the fragment loads of the matrix instructions free of bank conflicts. (One bulk copy per row and lane into padded
 // rows cost the producer 66 cycles each, 32 a chunk: 189 us on 576 seats, e4m3.) Eight consumer warps take one KV head each.
+// One token over e4m3, 576 seats of 200 to 1200 rows: 156 us, 5.4 TB/s, 83% of a copy's rate; 288 seats x 7 tokens, bf16: 148
+// us, 5.5 TB/s, 85%. Five to eight tokens over e4m3 reach half of it: the conversions to fp16 and the softmax, latency more
+// than issue slots (40% of them are used).
 // Scores S^T = K.Q^T and outputs O^T = V^T.P^T use mma.sync m16n8k16 with the 16 keys (dims) as the rows of A and the
 // 2 heads x 4 tokens as the 8 columns of B: with so few query columns the legacy tensor path is far below its limit.
 #include <cuda.h>
@@ -459,14 +462,13 @@ __device__ __forceinline__ void tree_tile_bf16(TreeState<FP8, NT>& st, const uin
 }
 
 // End of an item's chunks in this CTA. slot < 0: the item is complete and its rows are written; else its partial goes
-// to that workspace slot: outputs [8 heads][cols][128] fp32 and (maximum, sum) pairs, the warp's columns from col0 on.
+// to that workspace slot: outputs [8 heads][8 NT][128] fp32 and (maximum, sum) pairs.
 template <bool FP8, int NT>
-__device__ __forceinline__ void tree_finish(const TreeArgs& a, const TreeItem& it, int tok0, int cols, int col0, int h, int lane,
-                                            TreeState<FP8, NT>& st, int slot) {
+__device__ __forceinline__ void tree_finish(const TreeArgs& a, const TreeItem& it, int h, int lane, TreeState<FP8, NT>& st, int slot) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int tok = tok0 + 4 * nt + t;
+    const int tok = it.tok0 + 4 * nt + t;
     const bool padded = a.draft_lens != nullptr && tok >= it.drafts;
     float r[2], mx[2], l[2];
 #pragma unroll
@@ -499,7 +501,7 @@ __device__ __forceinline__ void tree_finish(const TreeArgs& a, const TreeItem& i
     } else {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const long long col = (static_cast<long long>(slot) * kKvHeads + h) * cols + col0 + 8 * nt + 2 * t + k;
+        const long long col = (static_cast<long long>(slot) * kKvHeads + h) * (8 * NT) + 8 * nt + 2 * t + k;
         float* dst = a.ws_o + col * kHeadDim;
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt)
@@ -595,16 +597,18 @@ __device__ __forceinline__ void tree_produce(const TreeParams& p, const TreePlan
 }
 
 // One CTA per SM: STREAMS shares of the chunk list, each with a ring of STAGES stages, a producer warp (of warpgroup 0, the
-// others of which leave) and 8 WPH consumer warps; the WPH warps of a head take four tokens each of a group of 4 WPH. With
-// 16 consumer warps (640 threads at 96 registers) warpgroup 0 goes down to 32 registers and the consumers up to 112:
-// 128 x 32 + 512 x 112 = 640 x 96.
-template <bool FP8, int STREAMS, int WPH, int STAGES>
+// others of which leave) and a consumer warp per KV head, which takes all 4 NT tokens of a group: K and V are converted
+// once, and eight tokens in one warp beat four in each of two (registers permitting: 288 seats x 7 tokens, e4m3: 147 -> 132
+// us, bf16: 153 -> 148). Few tokens leave a warp waiting, so e4m3, where a chunk takes longest, has two streams then.
+// Registers move from warpgroup 0 (down to 32) to the consumers: with 16 of them (640 threads at 96) up to 112, with eight
+// and NT = 2 (384 threads at 168) up to 232.
+template <bool FP8, int STREAMS, int NT, int STAGES>
 struct TreeShape {
-  static constexpr int kConsumers = kKvHeads * WPH * STREAMS, kThreads = 128 + 32 * kConsumers;
-  static constexpr bool kMoveRegs = kConsumers == 16;
-  static constexpr int kLaunchRegs = 96, kProducerRegs = 32, kConsumerRegs = 112;
-  static_assert(kConsumers == 8 || 128 * kProducerRegs + 512 * kConsumerRegs == 640 * kLaunchRegs, "the register split");
-  static constexpr int kTok = 4 * WPH;
+  static constexpr int kConsumers = kKvHeads * STREAMS, kThreads = 128 + 32 * kConsumers;
+  static constexpr bool kMoveRegs = kConsumers == 16 || NT > 1;
+  static constexpr int kLaunchRegs = kConsumers == 16 ? 96 : 168, kProducerRegs = 32, kConsumerRegs = kConsumers == 16 ? 112 : 232;
+  static_assert(128 * kProducerRegs + 32 * kConsumers * kConsumerRegs <= kThreads * kLaunchRegs, "the register split");
+  static constexpr int kTok = 4 * NT;
   static constexpr int kStream = STAGES * TreeStage<FP8>::kBytes;
   static constexpr int kBars = STREAMS * kStream;            // per stream: full[STAGES], empty[STAGES]
   static constexpr int kBytes = kBars + STREAMS * 2 * STAGES * 8;
@@ -612,11 +616,11 @@ struct TreeShape {
   static_assert(kAlloc + 1024 <= 232448, "shared memory");
 };
 
-template <bool FP8, bool DRAFTS, int STREAMS, int WPH, int STAGES>
-__global__ void __launch_bounds__(TreeShape<FP8, STREAMS, WPH, STAGES>::kThreads, 1)
+template <bool FP8, bool DRAFTS, int STREAMS, int NT, int STAGES>
+__global__ void __launch_bounds__(TreeShape<FP8, STREAMS, NT, STAGES>::kThreads, 1)
     paged_tree_kernel(const __grid_constant__ TreeParams p) {
   using SL = TreeStage<FP8>;
-  using SH = TreeShape<FP8, STREAMS, WPH, STAGES>;
+  using SH = TreeShape<FP8, STREAMS, NT, STAGES>;
   const TreeArgs& a = p.a;
   extern __shared__ __align__(1024) uint8_t tree_raw[];
   uint8_t* smem = tree_raw + ((1024u - (smem_addr(tree_raw) & 1023u)) & 1023u);
@@ -625,14 +629,14 @@ __global__ void __launch_bounds__(TreeShape<FP8, STREAMS, WPH, STAGES>::kThreads
     prefetch_map(&p.k);
     prefetch_map(&p.v);
   }
-  const int mine = warp < 4 ? min(warp, STREAMS - 1) : (warp - 4) / (kKvHeads * WPH);   // the warp's stream
+  const int mine = warp < 4 ? min(warp, STREAMS - 1) : (warp - 4) / kKvHeads;   // the warp's stream
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be scheduled; it waits for this grid
   if (tid == 0) {
     for (int s = 0; s < STREAMS; ++s) {
       uint64_t* b = reinterpret_cast<uint64_t*>(smem + SH::kBars) + 2 * STAGES * s;
       for (int i = 0; i < STAGES; ++i) {
         mbar_init(&b[i], FP8 && p.box_rows == 1 ? 33 : 1);   // + each lane's scales when they come row by row
-        mbar_init(&b[STAGES + i], kKvHeads * WPH);
+        mbar_init(&b[STAGES + i], kKvHeads);
       }
       tree_no_span(a, STREAMS * blockIdx.x + s);
     }
@@ -653,8 +657,8 @@ __global__ void __launch_bounds__(TreeShape<FP8, STREAMS, WPH, STAGES>::kThreads
     return;
   }
   if constexpr (SH::kMoveRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::kConsumerRegs));
-  const int h = (warp - 4) % kKvHeads, sub = (warp - 4) / kKvHeads % WPH, t = lane & 3, c = STREAMS * static_cast<int>(blockIdx.x) + mine;
-  TreeState<FP8, 1> st;
+  const int h = (warp - 4) % kKvHeads, t = lane & 3, c = STREAMS * static_cast<int>(blockIdx.x) + mine;
+  TreeState<FP8, NT> st;
   TreeLane<FP8> at;
   at.init(p.box_rows, h, lane >> 2, t);
   int w = P.w, k = 0;
@@ -666,8 +670,7 @@ __global__ void __launch_bounds__(TreeShape<FP8, STREAMS, WPH, STAGES>::kThreads
       first += it.n;
       it = tree_item<SH::kTok, kTreeRows, SL::kDraftRows>(a, ++w);
     }
-    const int tok0 = it.tok0 + 4 * sub;   // this warp's four tokens
-    tree_begin<FP8, 1>(a, it.seat, tok0, h, lane, st);
+    tree_begin<FP8, NT>(a, it.seat, it.tok0, h, lane, st);
     const int end = static_cast<int>(min(first + it.n, P.c1) - P.c0);
     int j = static_cast<int>(P.c0 + k - first);
     for (; k < end; ++k, ++j) {
@@ -678,22 +681,24 @@ __global__ void __launch_bounds__(TreeShape<FP8, STREAMS, WPH, STAGES>::kThreads
       }
       if (__any_sync(0xffffffffu, !ok)) break;
       const uint8_t* base = stages + stage * SL::kBytes;
-      uint32_t see[1] = {0};
+      uint32_t see[NT] = {};
       if (!DRAFTS || j < it.nc) {
         const int rows = it.len - j * kTreeRows;
         if constexpr (FP8) {
-          if (rows >= kTreeRows) tree_tile_e4m3<1, false>(st, base, at, h, lane, kTreeRows);
-          else tree_tile_e4m3<1, true>(st, base, at, h, lane, rows);
+          if (rows >= kTreeRows) tree_tile_e4m3<NT, false>(st, base, at, h, lane, kTreeRows);
+          else tree_tile_e4m3<NT, true>(st, base, at, h, lane, rows);
         } else {
-          if (rows >= kTreeRows) tree_tile_bf16<false, 1, false, false>(st, base, at, h, lane, kTreeRows, see);
-          else tree_tile_bf16<false, 1, true, false>(st, base, at, h, lane, rows, see);
+          if (rows >= kTreeRows) tree_tile_bf16<false, NT, false, false>(st, base, at, h, lane, kTreeRows, see);
+          else tree_tile_bf16<false, NT, true, false>(st, base, at, h, lane, rows, see);
         }
       } else if constexpr (DRAFTS) {
         const int r0 = (j - it.nc) * SL::kDraftRows;
-        if (tok0 + t < it.drafts)
-          see[0] = static_cast<uint32_t>(
-              static_cast<unsigned long long>(a.mask[static_cast<long long>(it.seat) * a.mask_seat + tok0 + t]) >> r0);
-        tree_tile_bf16<FP8, 1, false, true>(st, base, at, h, lane, min(SL::kDraftRows, it.drafts - r0), see);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          if (it.tok0 + 4 * nt + t < it.drafts)
+            see[nt] = static_cast<uint32_t>(
+                static_cast<unsigned long long>(a.mask[static_cast<long long>(it.seat) * a.mask_seat + it.tok0 + 4 * nt + t]) >> r0);
+        tree_tile_bf16<FP8, NT, false, true>(st, base, at, h, lane, min(SL::kDraftRows, it.drafts - r0), see);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[stage]);
@@ -701,8 +706,8 @@ __global__ void __launch_bounds__(TreeShape<FP8, STREAMS, WPH, STAGES>::kThreads
     if (k < end) break;   // a wait gave up
     // slot 2c + 1 holds the item that starts here and goes on, 2c the one that came in from the share before
     const bool from_before = first < P.c0, goes_on = first + it.n > P.c1;
-    tree_finish<FP8, 1>(a, it, tok0, 8 * WPH, 8 * sub, h, lane, st, from_before ? 2 * c : (goes_on ? 2 * c + 1 : -1));
-    if (!from_before && h == 0 && sub == 0 && lane == 0)
+    tree_finish<FP8, NT>(a, it, h, lane, st, from_before ? 2 * c : (goes_on ? 2 * c + 1 : -1));
+    if (!from_before && h == 0 && lane == 0)
       tree_span(a, w, c, goes_on ? tree_last_share(P, first + it.n - 1) : c);
   }
   if (k < n && lane == 0)
@@ -794,10 +799,11 @@ struct TreeConfig {
   int tok, shares;       // tokens per group; shares of the chunk list
 };
 
-// Few tokens: the kernel above, in groups of 4 (one warp per head) or 8 (two) that each read the cache. More: the tcgen05
-// kernel, whose time hardly grows with the tokens, one share per 8 SMs (a CTA per KV head). 96 seats of 1200 to 2400 rows:
-// bf16, 8 tokens 130 us here, 9 tokens 204 here and 181 there; e4m3, 16 tokens 224 here and 250 there, 17 tokens 319 and
-// 254. The tcgen05 kernel takes the row maximum before it scales, so a scale that is not positive runs here too.
+// Few tokens: the kernel above, in groups of 4 or 8 that each read the cache. More: the tcgen05 kernel, whose time hardly
+// grows with the tokens, one share per 8 SMs (a CTA per KV head). 96 seats of 1200 to 2400 rows: bf16, 8 tokens 124 us here,
+// 9 tokens about 180 here and 141 there; e4m3, 16 tokens 193 here and 203 there (288 seats of 200 to 1200 rows: 248 and 310),
+// 17 tokens about 270 and 196. The tcgen05 kernel takes the row maximum before it scales, so a scale that is not positive
+// runs here too.
 TreeConfig tree_config(bool fp8, int tokens, float scale, int num_sms) {
   if (tokens > (fp8 ? 16 : 8) && scale > 0.f) return {true, tokens, max(1, num_sms / kKvHeads)};
   const int tok = tokens <= 4 ? 4 : 8;
@@ -821,10 +827,10 @@ bool make_pool_map(CUtensorMap* m, const void* base, long long rows, int box_row
 
 // With the moved registers the launch is refused unless the kernel was built at exactly kLaunchRegs: a setmaxnreg.inc that
 // cannot be met would wait forever.
-template <bool FP8, bool DRAFTS, int STREAMS, int WPH, int STAGES>
+template <bool FP8, bool DRAFTS, int STREAMS, int NT, int STAGES>
 cudaError_t launch_tree_main(const TreeArgs& a, int shares, cudaStream_t stream) {
-  using SH = TreeShape<FP8, STREAMS, WPH, STAGES>;
-  auto kern = paged_tree_kernel<FP8, DRAFTS, STREAMS, WPH, STAGES>;
+  using SH = TreeShape<FP8, STREAMS, NT, STAGES>;
+  auto kern = paged_tree_kernel<FP8, DRAFTS, STREAMS, NT, STAGES>;
   static thread_local int configured_device = -1;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
