@@ -7,7 +7,7 @@
 //   O += P V       M = 128, N = 128 dims:      A = P (bf16) from TMEM, B = V from shared memory
 // The 8 CTAs of a share walk the same keys at the same time, one head each, so the 256 (128) contiguous bytes a CTA
 // takes of a token row join the other heads' in the DRAM page. Warps:
-//   copies (3/1)  bring the head's part of 64 token rows by TMA tensor copies of 128 bytes x R rows, R the largest
+//   copies (2)    bring the head's part of 64 token rows by TMA tensor copies of 128 bytes x R rows, R the largest
 //                 power of two up to 64 that divides the page size (a box never leaves its page), with the table
 //                 entries looked up a tile ahead. bf16 rows land swizzled, as operands. e4m3 rows (and their scales)
 //                 land in a ring of raw tiles. (Four-row gathers serve any page the same way but took 66 cycles each,

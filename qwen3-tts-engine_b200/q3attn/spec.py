@@ -14,6 +14,7 @@ several streams, or in several captured graphs, never share one. The ops themsel
 are in csrc/torch_ops.cpp: they are short, and through Python and ctypes a call would cost more host time than GPU time.
 """
 import os
+import threading
 from typing import NamedTuple, Optional
 
 import torch
@@ -26,7 +27,7 @@ MAX_TREE_TOKENS = 64
 _TORCH_LIB = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libq3torch.so")
 
 
-_registered = False
+_registered, _lock = False, threading.Lock()
 
 
 def _register() -> None:
@@ -51,10 +52,19 @@ def _register() -> None:
     _registered = True
 
 
+@torch.compiler.assume_constant_result   # a compiled function may be an op's first caller: registering is not traced
+def _ready() -> bool:
+    if not _registered:
+        with _lock:
+            if not _registered:
+                _register()
+    return True
+
+
 def _op(name):
     """The op `q3attn::name`."""
     if not _registered:
-        _register()
+        _ready()
     return getattr(torch.ops.q3attn, name).default
 
 

@@ -183,6 +183,27 @@ def test_graph_of_a_step_with_growing_lengths(q3):
         assert torch.equal(sc.top_ids, top)
 
 
+def test_compiled_step(q3):
+    """append + tree attention + scores under torch.compile (one graph, functionalised) give what eager calls give."""
+    c = tree_case(3, 5, [20, 0, 33], 16, 39, True)
+    seq, bt = torch.tensor(c["lens"], dtype=torch.int32, device=DEV), c["bt"].to(DEV)
+    q, k, v, m = dev(c["q"], c["k"], c["v"], c["mask"])
+    w = (torch.randn(2048, 300, generator=gen(3)) / 45).to(DEV, BF)
+    ids = torch.arange(15, device=DEV)
+
+    def step(kc, vc, ks, vs):
+        o = q3.paged_tree_attn(q, k, v, m, kc, vc, seq, bt, SCALE, k_scale=ks, v_scale=vs)
+        q3.kv_quant_append_paged(k[:, 0], v[:, 0], kc, vc, ks, vs, seq, bt)
+        o1 = q3.paged_decode_quant(q[:, 0], kc, vc, ks, vs, seq + 1, bt, SCALE)
+        return (o, o1, *q3.token_logprobs(o.view(15, 2048) @ w, ids, 4))
+
+    a, b = dev(*c["cache"]), dev(*c["cache"])
+    want = step(*a)
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(*b)
+    assert all(bits_equal(x, y) for x, y in zip(got, want))
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+
+
 # ------------------------------------------------------------------------------------------------ arguments
 @pytest.mark.parametrize("fp8,T", [(True, 3), (True, 12), (True, 30), (False, 3), (False, 30)])
 @pytest.mark.parametrize("scale", [0.0, -0.05])

@@ -3,6 +3,9 @@ their ops have shape rules, refuse CPU tensors and trace as single nodes; visibi
 their formulas say."""
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -165,6 +168,18 @@ def test_ops_trace_as_single_nodes():
     for op in ("paged_tree_attn", "kv_quant_append_paged", "token_logprobs"):
         assert targets.count(f"q3attn.{op}.default") == 1, targets
     assert not any("softmax" in t or "matmul" in t for t in targets)
+
+
+def test_first_call_from_a_compiled_function():
+    """In a process of its own: torch.compile traces the op's very first call as one graph (the CPU tensors are refused
+    when it runs)."""
+    src = ("import sys; sys.path.insert(0, sys.argv[1])\nimport torch, q3attn\n"
+           "f = torch.compile(lambda x, i: q3attn.token_logprobs(x * 2, i, 3, 0.9).logprobs + 1, fullgraph=True, backend='eager')\n"
+           "try:\n    f(torch.randn(4, 50), torch.zeros(4, dtype=torch.int64))\n"
+           "except RuntimeError as e:\n    print('refused' if 'must be a CUDA tensor' in str(e) else repr(e))\n")
+    pkg = os.path.dirname(os.path.dirname(os.path.abspath(_lib.__file__)))
+    r = subprocess.run([sys.executable, "-c", src, pkg], capture_output=True, text=True, timeout=300)
+    assert r.stdout.strip() == "refused", r.stdout + r.stderr[-2000:]
 
 
 # ------------------------------------------------------------------------------------------------ visibility words
