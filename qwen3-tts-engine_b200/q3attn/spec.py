@@ -140,5 +140,7 @@ def token_logprobs(logits, ids, top_n: int = 0, temperature: float = 1.0) -> Tok
     alternatives, e.g. to accept or reject drafted tokens. logits [rows, vocab] bf16, fp16 or fp32; ids int64 [rows] or
     [rows, given] (an id outside the vocabulary, such as -1 for padding, scores -inf). top_n <= min(64, vocab), ordered
     by (logit descending, id ascending), NaN first. Logits of -inf have probability 0; a row with NaN or +inf, or of
-    -inf alone, gives NaN. temperature 1e-30 to 1e30. One launch."""
+    -inf alone, gives NaN. temperature 1e-30 to 1e30. One launch.
+    Statistics are fp32: an entropy, or a log probability near zero, is good to about 1e-7 absolutely (a row that one token
+    all but owns has an entropy of few significant digits)."""
     return TokenLogprobs(*_op("token_logprobs")(logits, ids, top_n, temperature))
