@@ -45,6 +45,8 @@ constexpr int kLpSlack = 64;                        // the list is cut back when
 constexpr int kLpSegs = 8;                          // segments of a CTA's tiles
 constexpr int kLpMaxCluster = 8;
 static_assert(kLpList >= kLogprobMaxTop + kLogprobMaxTop * 2 * kLpMaxElems && kLpGroups >= 2 * kLogprobMaxTop, "list");
+// select_tiles: what is listed before a tile and the candidates of a tile that adds them as they are
+static_assert(kLpList >= kLogprobMaxTop + kLpSlack + kLpThreads / 2 * kLpMaxElems, "list of a tile without a bound of its own");
 
 __device__ __forceinline__ uint32_t order_bits(float x) {
   if (x != x) return 0xffffffffu;
@@ -212,10 +214,13 @@ __device__ __noinline__ void select_tiles(LpShared& sh, const Part<T> part, int 
     const bool some = order_bits(top) > static_cast<uint32_t>(sh.bound >> 32);
     const int threads = __syncthreads_count(some);
     if (threads == 0) continue;
-    const int m = sh.count;
     Key bound = sh.bound;
-    if (m + threads * kLpVecs * N > kLpList || threads > kLpThreads / 2) {
+    // The branch holds barriers, so it is taken on the barrier's own result: sh.count may not be looked at here, since
+    // other warps may be listing keys already. At most n + kLpSlack keys are listed before a tile, and half of the threads
+    // add kLpMaxElems each at most: the list holds them.
+    if (threads > kLpThreads / 2) {
       // many: the n-th largest group maximum bounds the tile's part of the top n from below
+      const int m = sh.count;   // no warp lists before this branch's barriers
       Key mine = 0ull;
 #pragma unroll
       for (int j = 0; j < kLpVecs; ++j)

@@ -120,6 +120,28 @@ def test_values_in_one_place(q3, n):
         check(q3, x, torch.full((n,), at.start), 40)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v", [(3, 30000), (200, 30000), (1, 130000)])
+@pytest.mark.parametrize("threads", [40, 66, 100, 125])
+def test_ties_with_candidates_of_some_threads(q3, dtype, n, v, threads):
+    """Massive ties (fewer than 64 of 128 groups of two threads above them) leave the row to the selection by tiles; its
+    later tiles then have candidates of `threads` of 256 threads, in all four of a thread's vectors, which are listed as
+    they are."""
+    vec = 16 // dtype.itemsize
+    x = torch.ones(n, v, dtype=dtype)
+    i = torch.arange(v)
+    for tile, up in ((1, 1), (2, 1), (3, 2)):
+        x[:, (i // (1024 * vec) == tile) & (i // vec % 256 < threads)] += up
+    x[n // 2, -40:] = 9.0
+    ids = torch.arange(n) * 7 % v
+    check(q3, x, ids, 64)
+    d, first = x.to(DEV), None
+    for _ in range(10):
+        top = q3.token_logprobs(d, ids.to(DEV), 64).top_ids
+        first = top if first is None else first
+        assert torch.equal(top, first)
+
+
 def test_graph_replay(q3):
     x = logits(12, 30000, 10, torch.bfloat16).to(DEV)
     ids = torch.arange(12, device=DEV)
