@@ -365,6 +365,9 @@ typedef struct q3_tree_attn {
 } q3_tree_attn;
 size_t q3_paged_tree_workspace_bytes(int32_t batch, int32_t tokens, int32_t quantised);
 int q3_paged_tree_attn(const q3_tree_attn* args, void* workspace, size_t workspace_bytes, void* stream);
+/* Self-test: the call's second kernel alone, over whatever the workspace holds. Where no partial is recorded for an item
+ * (as where a wait gave up) nothing is read or written for it. */
+int q3_selftest_tree_merge(const q3_tree_attn* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Log probabilities of given tokens, with the entropy of each row and its top alternatives: the scores that accept or
  * reject drafted tokens. For row r, p = softmax(logits[r] / temperature):

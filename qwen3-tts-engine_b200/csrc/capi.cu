@@ -841,7 +841,8 @@ size_t q3_paged_tree_workspace_bytes(int32_t batch, int32_t tokens, int32_t quan
   return x > y ? x : y;
 }
 
-int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_bytes, void* stream) {
+// Checks of q3_paged_tree_attn and the kernels' arguments; a.B == 0: nothing to do.
+static int tree_args(const q3_tree_attn* p, void* workspace, size_t workspace_bytes, q3::TreeArgs& a, q3::TreeWorkspace& w) {
   if (!p) return Q3_ERR_INVALID;
   int rc = check_family(p->num_heads, p->num_kv_heads, p->head_dim);
   if (rc != Q3_OK) return rc;
@@ -869,9 +870,8 @@ int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_
     return Q3_ERR_ALIGNMENT;
   int dev = 0;
   if ((rc = current_device(&dev)) != Q3_OK) return rc;
-  const q3::TreeWorkspace w = q3::tree_workspace(p->k_scale != nullptr, p->batch, p->tokens, p->softmax_scale, sm_count(dev));
+  w = q3::tree_workspace(p->k_scale != nullptr, p->batch, p->tokens, p->softmax_scale, sm_count(dev));
   if (!workspace || workspace_bytes < w.bytes || !aligned(workspace, 256)) return Q3_ERR_WORKSPACE;
-  q3::TreeArgs a{};
   if ((rc = status_ptr(dev, &a.status)) != Q3_OK) return rc;
   a.q = static_cast<const __nv_bfloat16*>(p->q);
   a.q_seat = p->q_seat_stride;
@@ -910,7 +910,23 @@ int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_
   a.span_by_item = w.span_by_item;
   a.ws_ml = reinterpret_cast<float*>(ws + w.ml);
   a.ws_o = reinterpret_cast<float*>(ws + w.o);
+  return Q3_OK;
+}
+
+int q3_paged_tree_attn(const q3_tree_attn* p, void* workspace, size_t workspace_bytes, void* stream) {
+  q3::TreeArgs a{};
+  q3::TreeWorkspace w;
+  const int rc = tree_args(p, workspace, workspace_bytes, a, w);
+  if (rc != Q3_OK || a.B == 0) return rc;
   return record(q3::launch_paged_tree(a, w, static_cast<cudaStream_t>(stream)));
+}
+
+int q3_selftest_tree_merge(const q3_tree_attn* p, void* workspace, size_t workspace_bytes, void* stream) {
+  q3::TreeArgs a{};
+  q3::TreeWorkspace w;
+  const int rc = tree_args(p, workspace, workspace_bytes, a, w);
+  if (rc != Q3_OK || a.B == 0) return rc;
+  return record(q3::launch_paged_tree_merge(a, w, static_cast<cudaStream_t>(stream)));
 }
 
 int q3_token_logprobs(const q3_logprobs* p, void* stream) {

@@ -734,14 +734,19 @@ struct MergeState {
 };
 
 template <bool WIDE>
-__global__ void __launch_bounds__(kMergeWarps * 32) paged_tree_merge_kernel(const TreeArgs a, int tok_per_group) {
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_tree_merge_kernel(const TreeArgs a, int tok_per_group, int shares) {
   constexpr int kCols = WIDE ? 1 : 4, kBatch = 8 / kCols;   // columns per warp; partials asked for at a time
   __shared__ float4 part_o[WIDE ? kMergeWarps : 1][32];
   __shared__ float2 part_ml[WIDE ? kMergeWarps : 1];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int4 span = __ldcg(&a.ws_span[blockIdx.x]);
-  if (span.x < 0) return;
+  // x < 0: nothing to add. A share that gave up a wait leaves the records of its items as the workspace came, and these
+  // words say where this kernel reads and writes: what is not an item's own record within bounds is passed over. (Cleared
+  // beforehand, in the plan or by an idle warp, they cost the first kernel 2 to 15% by its registers.)
+  if (span.x < 0 || span.x >= a.B * a.groups || span.y < 0 || span.y >= span.z || span.z >= shares ||
+      static_cast<int>(blockIdx.x) != (a.span_by_item ? span.x : span.y))
+    return;
   const int seat = span.x / a.groups, tok0 = (span.x - seat * a.groups) * tok_per_group, c = span.y, parts = span.z - c + 1;
   const int live = 2 * min(tok_per_group, a.tokens - tok0), cols = 2 * tok_per_group, pairs = kKvHeads * live;
   const int pair0 = WIDE ? blockIdx.y : (blockIdx.y * kMergeWarps + warp) * kCols;
@@ -881,7 +886,10 @@ cudaError_t launch_paged_tree(const TreeArgs& a, const TreeWorkspace& w, cudaStr
   else if (fp8) e = launch_tree_main<true, true, 1, 2, 6>(a, w.shares, stream);
   else if (w.tok == 4) e = launch_tree_main<false, true, 1, 1, 3>(a, w.shares, stream);
   else e = launch_tree_main<false, true, 1, 2, 3>(a, w.shares, stream);
-  if (e != cudaSuccess) return e;
+  return e != cudaSuccess ? e : launch_paged_tree_merge(a, w, stream);
+}
+
+cudaError_t launch_paged_tree_merge(const TreeArgs& a, const TreeWorkspace& w, cudaStream_t stream) {
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
@@ -894,8 +902,8 @@ cudaError_t launch_paged_tree(const TreeArgs& a, const TreeWorkspace& w, cudaStr
   lc.stream = stream;
   lc.attrs = &at;
   lc.numAttrs = 1;
-  return wide ? cudaLaunchKernelEx(&lc, paged_tree_merge_kernel<true>, a, w.tok)
-              : cudaLaunchKernelEx(&lc, paged_tree_merge_kernel<false>, a, w.tok);
+  return wide ? cudaLaunchKernelEx(&lc, paged_tree_merge_kernel<true>, a, w.tok, w.shares)
+              : cudaLaunchKernelEx(&lc, paged_tree_merge_kernel<false>, a, w.tok, w.shares);
 }
 
 }  // namespace q3

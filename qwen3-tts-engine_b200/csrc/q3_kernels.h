@@ -138,6 +138,7 @@ struct TreeWorkspace {
 };
 TreeWorkspace tree_workspace(bool fp8, int batch, int tokens, float scale, int num_sms);
 cudaError_t launch_paged_tree(const TreeArgs& a, const TreeWorkspace& w, cudaStream_t stream);
+cudaError_t launch_paged_tree_merge(const TreeArgs& a, const TreeWorkspace& w, cudaStream_t stream);   // its second kernel
 cudaError_t launch_paged_tree_tc(const TreeArgs& a, int shares, cudaStream_t stream);
 
 struct PrefixCopyArgs {

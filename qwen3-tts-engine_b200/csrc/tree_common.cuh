@@ -124,7 +124,8 @@ __device__ __forceinline__ bool tree_plan(const TreeArgs& a, TreePlan& P, int c,
   return true;
 }
 
-// Nothing starts in share c and goes on, so far (records per share; records per item are all written as items end).
+// Nothing starts in share c and goes on, so far (records per share; records per item are written as items end, unless a
+// wait gave up: the merge checks them).
 __device__ __forceinline__ void tree_no_span(const TreeArgs& a, int c) {
   if (!a.span_by_item) a.ws_span[c] = make_int4(-1, 0, 0, 0);
 }

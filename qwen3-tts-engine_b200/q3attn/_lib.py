@@ -101,6 +101,7 @@ SIGNATURES = {
     "q3_kv_dequant_paged": (ctypes.c_int, [_QC, _I32, _I32, _P, _P, _P, _I64, _I32, _I32, _P, _P, _I64, _I32, _P]),
     "q3_paged_tree_workspace_bytes": (_SZ, [_I32, _I32, _I32]),
     "q3_paged_tree_attn": (ctypes.c_int, [ctypes.POINTER(TreeAttn), _P, _SZ, _P]),
+    "q3_selftest_tree_merge": (ctypes.c_int, [ctypes.POINTER(TreeAttn), _P, _SZ, _P]),
     "q3_token_logprobs": (ctypes.c_int, [ctypes.POINTER(Logprobs), _P]),
     "q3_cp_step_qkv": (ctypes.c_int, [_P, _I64, _NR, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _I32,
                                       _I32, _F32, _P, _I64, _P]),

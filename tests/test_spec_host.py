@@ -251,3 +251,16 @@ def test_oracle_logprobs_are_log_softmax():
     assert (ent - torch.special.entr(ref.exp()).sum(-1)).abs().max() < 1e-12
     assert torch.equal(tl, ref.topk(4).values) or (tl - ref.topk(4).values).abs().max() < 1e-12
     assert torch.equal(ids, x.topk(4).indices)
+
+
+def test_the_merge_alone_refuses_what_the_call_refuses():
+    lib = _lib.load()
+    call = lambda p, ws=A, n=1 << 40: lib.q3_selftest_tree_merge(p, ws, n, None)  # noqa: E731
+    one = lambda **kw: ctypes.byref(_lib.TreeAttn(**{**dict(  # noqa: E731
+        q=A, q_seat_stride=2048, q_token_stride=2048, k_pool=A, v_pool=A, num_pages=1, page_size=16, cache_seqlens=A, block_table=A,
+        block_table_stride=1, max_pages_per_seat=1, batch=1, tokens=1, num_heads=16, num_kv_heads=8, head_dim=128,
+        softmax_scale=0.1, out=A, out_seat_stride=2048, out_token_stride=2048), **kw}))
+    assert call(None) == call(one(q=None)) == call(one(tokens=0)) == call(one(block_table_stride=0)) == INVALID
+    assert call(one(tokens=65)) == call(one(head_dim=64)) == UNSUPPORTED
+    assert call(one(out=A + 8)) == ALIGN
+    assert call(one(batch=0, q=None)) == OK
