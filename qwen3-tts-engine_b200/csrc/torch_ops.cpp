@@ -2,6 +2,7 @@
 // argument checks, outputs and the call, in C++. These ops run in a few microseconds, so their host side must not take
 // longer than they do: through Python and ctypes a call costs 25 to 40 us of host time. Shapes for tracing are in
 // q3attn/spec.py, which also documents each op.
+#include <ATen/ops/clamp.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -60,13 +61,15 @@ void check_table(const Tensor& bt, const Tensor& first) {
 // A table of one column may have any inner stride; its row stride is at least its width.
 int64_t table_stride(const Tensor& bt) { return bt.size(0) <= 1 && bt.stride(0) < bt.size(1) ? bt.size(1) : bt.stride(0); }
 
-// Index vectors are taken as they are, or converted (int64 positions, strided slices).
+// Index vectors are taken as they are, or converted (int64 positions, strided slices). Narrowing saturates, so that what
+// lies outside int32 stays out of range: -1 is no row, and neither is INT32_MAX (row_addresses).
 Tensor index_of(const Tensor& t, const char* name, ScalarType type, int64_t n, const Tensor& first) {
   on_device(t, name, first);
   TORCH_CHECK(t.numel() == n, "q3attn: ", name, " must have one entry per row");
   TORCH_CHECK(t.scalar_type() == ScalarType::Int || t.scalar_type() == ScalarType::Long, "q3attn: ", name,
               " must be int32 or int64");
-  return t.scalar_type() == type && t.is_contiguous() ? t : t.to(type).contiguous();
+  if (t.scalar_type() == type) return t.is_contiguous() ? t : t.contiguous();
+  return (type == ScalarType::Int ? at::clamp(t, -1, INT32_MAX) : t).to(type).contiguous();
 }
 
 // k and v rows [n, 8, 128] with one shared row stride (as the kernels take them), copied when theirs differ.
@@ -104,6 +107,8 @@ struct Rows {
 Rows row_addresses(int64_t n, const Tensor& positions, const Tensor& bt, const std::optional<Tensor>& seat_of_row,
                    const Tensor& first) {
   check_table(bt, first);
+  TORCH_CHECK(positions.scalar_type() == ScalarType::Int || bt.size(1) * first.size(1) <= INT32_MAX,
+              "q3attn: int64 positions with a block_table of 2^31 tokens a seat and more");
   Rows r{index_of(positions, "positions", ScalarType::Int, n, first), std::nullopt};
   if (seat_of_row.has_value()) r.seat = index_of(*seat_of_row, "seat_of_row", ScalarType::Int, n, first);
   else TORCH_CHECK(n <= bt.size(0), "q3attn: without seat_of_row row i is seat i's: block_table has too few rows");

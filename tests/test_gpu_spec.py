@@ -442,3 +442,41 @@ def test_deterministic(q3):
     first = run_tree(q3, c)
     for _ in range(5):
         assert bits_equal(first, run_tree(q3, c))
+
+
+@pytest.mark.parametrize("far", [1 << 31, 1 << 32, (1 << 32) + 5, (1 << 40) + 5, -(1 << 31) - 1, -(1 << 32), -(1 << 40) + 3, (1 << 63) - 1, -(1 << 63)])
+def test_int64_positions_and_seats_do_not_wrap(q3, far):
+    """What lies outside int32 is out of range like any other: skipped with its status bit, read back as zeros."""
+    cache = q3.empty_quant_cache(4, 16, DEV)
+    bt = torch.arange(4, dtype=torch.int32, device=DEV).view(2, 2)
+    k = rows(64, 1).to(DEV)
+    q3.kv_quant_append_slots(k, k, *cache, torch.arange(64, device=DEV))
+    before = [bits(c) for c in cache]
+    seat = torch.tensor([0, far, 1, 0], device=DEV)
+    pos = torch.tensor([far, 3, far, 7], device=DEV)
+    assert q3._lib.read_status() == 0
+    new = rows(4, 2)
+    q3.kv_quant_append_paged(new.to(DEV), new.to(DEV), *cache, pos, bt, seat)
+    assert q3._lib.read_status() == q3._lib.STATUS_BAD_LENGTH
+    rest = torch.arange(64) != 7
+    for c, b in zip(cache, before):
+        now = bits(c)
+        assert torch.equal(now.reshape(64, -1)[rest], b.reshape(64, -1)[rest])
+    y, e = expect_cache(new[3:])
+    assert torch.equal(cache[0].cpu().view(-1, 8, 128)[7].float().double(), y[0]) and torch.equal(bits(cache[2]).view(-1, 8)[7], e[0])
+    kb, vb = q3.kv_dequant_paged(*cache, pos, bt, seat)
+    assert q3._lib.read_status() == q3._lib.STATUS_BAD_LENGTH
+    assert not kb.cpu()[:3].float().abs().any() and not vb.cpu()[:3].float().abs().any() and kb.cpu()[3].float().abs().any()
+
+
+def test_int64_positions_of_tables_past_int32_are_refused(q3):
+    """A table of 2^31 tokens a seat and more: an int64 position cannot be narrowed, an int32 one is taken."""
+    cache = q3.empty_quant_cache(1, 1 << 16, DEV)
+    bt = torch.zeros(1, 1 << 15, dtype=torch.int32, device=DEV)
+    k, seat = rows(1, 3).to(DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError, match="int64 positions"):
+        q3.kv_quant_append_paged(k, k, *cache, seat.long(), bt, seat)
+    with pytest.raises(RuntimeError, match="int64 positions"):
+        q3.kv_dequant_paged(*cache, seat.long(), bt, seat)
+    q3.kv_quant_append_paged(k, k, *cache, seat, bt, seat.long())
+    assert q3._lib.read_status() == 0 and bits(cache[2]).any()
