@@ -224,7 +224,8 @@ def kv_append_slots(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
 def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                     positions: torch.Tensor, block_table: torch.Tensor,
                     seat_of_row: Optional[torch.Tensor] = None) -> None:
-    """Row i -> token positions[i] of seat seat_of_row[i] (default: seat i) through the block table."""
+    """Row i -> token positions[i] of seat seat_of_row[i] (default: seat i) through the block table. Positions outside
+    the table are skipped and raise a status bit; seats must be rows of the table."""
     lib = _lib.load()
     k, v = _paired_rows(_rows("k", k), _rows("v", v))
     _check_cuda_bf16("k_cache", k_cache)
@@ -232,9 +233,12 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     _need(k_cache.dim() == 4 and k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.shape == v_cache.shape,
           "caches must be contiguous [num_pages, page_size, 8, 128]")
     _need(v.shape == k.shape and v.stride(0) == k.stride(0), "k and v must have the same shape and row stride")
-    pos = positions.to(device=k.device, dtype=torch.int32).contiguous()
     _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1,
           "block_table must be int32 [seats, max_pages]")
+    if positions.dtype == torch.int64:      # saturated, not wrapped: what lies outside int32 is no position of the table
+        _need(block_table.shape[1] * k_cache.shape[1] < 1 << 31, "int64 positions with a table of 2^31 tokens a seat")
+        positions = positions.clamp(-1, (1 << 31) - 1)
+    pos = positions.to(device=k.device, dtype=torch.int32).contiguous()
     sor = None if seat_of_row is None else seat_of_row.to(device=k.device, dtype=torch.int32).contiguous()
     with torch.cuda.device(k.device):
         rc = lib.q3_kv_append_paged(k.data_ptr(), v.data_ptr(), k.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),

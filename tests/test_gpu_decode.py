@@ -259,6 +259,23 @@ def test_kv_append_paged_bit_exact_and_identity_table_flat(q3):
         assert bits_equal(gk, rk) and bits_equal(gv, rv)
 
 
+@pytest.mark.parametrize("far", [1 << 31, 1 << 32, (1 << 40) + 5, -(1 << 32), -(1 << 63)])
+def test_kv_append_paged_int64_positions_do_not_wrap(q3, far):
+    """A position outside int32 is skipped and raises its status bit; the others of the call land."""
+    g = synth.cpu_gen(11)
+    k = synth.randn((3, 8, 128), g, 1.0, torch.bfloat16)
+    bt = torch.arange(6, dtype=torch.int32).view(3, 2)
+    pools = [torch.zeros(6, 16, 8, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    pos = torch.tensor([far, 17, far])
+    q3._lib.read_status(clear=True)
+    q3.kv_append_paged(k.to(DEV), k.to(DEV), *pools, pos.to(DEV), bt.to(DEV))
+    assert q3._lib.read_status(clear=True) == q3._lib.STATUS_BAD_LENGTH
+    for p in pools:
+        want = torch.zeros(96, 8, 128, dtype=torch.bfloat16)
+        want[3 * 16 + 1] = k[1]
+        assert bits_equal(p.view(96, 8, 128), want)
+
+
 def test_bad_block_table_entry_reports_status(q3):
     """An out-of-range page id is caught by the kernel's own bounds check (clamped, status bit raised)."""
     lay = _layout(2, [20, 20], 16, 2, seed=4)
