@@ -335,11 +335,12 @@ int q3_kv_dequant_paged(const q3_quant_cache* cache, int32_t num_kv_heads, int32
  * Token i < draft_lens[b] (NULL: tokens) of seat b attends over the seat's cache_seqlens[b] cached rows and over the
  * drafted rows j < draft_lens[b] with bit j of tree_mask[b, i] set (a token that sees itself has its own bit set). The
  * drafted rows are read where they are and not written to the cache: after verification the accepted ones are appended.
- * A token with nothing to see, and one at or past draft_lens[b], gets a zero row. Values that a token does not see do
- * not reach its output, whatever they are. k_new == NULL: no drafted rows (tree_mask and draft_lens are not read).
- * The cache is bf16 (k_scale == v_scale == NULL) or the 8-bit format above. Sums and softmax statistics are fp32.
- * 1 <= tokens <= 64; the workspace (q3_paged_tree_workspace_bytes, 256-byte aligned) needs no initialisation and may
- * not be shared by calls that overlap. Entries of the block table outside the pool read page 0 and raise a status bit. */
+ * A token with nothing to see, one at or past draft_lens[b], and one whose scores are all -inf get zero rows (a key that
+ * scores -inf has no weight). Values that a token does not see do not reach its output, whatever they are. k_new == NULL:
+ * no drafted rows (tree_mask and draft_lens are not read). The cache is bf16 (k_scale == v_scale == NULL) or the 8-bit
+ * format above. Sums and softmax statistics are fp32. 1 <= tokens <= 64; the workspace (q3_paged_tree_workspace_bytes,
+ * 256-byte aligned) needs no initialisation and may not be shared by calls that overlap. Entries of the block table
+ * outside the pool read page 0 and raise a status bit. */
 typedef struct q3_tree_attn {
   const void* q;               /* bf16 [batch, tokens, 16, 128], heads contiguous; strides in elements */
   int64_t q_seat_stride, q_token_stride;

@@ -122,6 +122,9 @@ __device__ __forceinline__ uint32_t word4(const uint4& w, int e) {
   return e == 0 ? w.x : (e == 1 ? w.y : (e == 2 ? w.z : w.w));
 }
 
+// Minus the maximum of no scores: finite, so that a first score of -inf has probability 0 and is not -inf + inf = NaN.
+constexpr float kNoMax = 3.402823466e38f;
+
 // What a consumer warp keeps of an item: lane 4g + t owns columns 2t and 2t + 1 (both heads of token 4 nt + t of the
 // group) of every 8-column tile nt, and of the outputs the dims row_dim(mt) (accumulators 0, 1) and row_dim(mt) + 1
 // (2, 3).
@@ -130,7 +133,7 @@ struct TreeState {
   uint32_t q[NT][8][2];    // B fragments of Q^T: for k-step s the four dims key_dim(t, s) .. + 3 of column g
   float cf[NT][2];         // score factor of the lane's columns
   float o[NT][8][4];
-  float nm[NT][2];         // minus the maximum that the outputs are relative to (FP8: of s + ev; else of s); +inf: none
+  float nm[NT][2];         // minus the maximum that the outputs are relative to (FP8: of s + ev; else of s); kNoMax: none
   float ns[NT][2];         // FP8: minus the maximum of s that l is relative to
   float l[NT][2];          // this lane's part of the sum
 };
@@ -182,7 +185,7 @@ __device__ __forceinline__ void tree_begin(const TreeArgs& a, int seat, int tok0
     st.cf[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      st.nm[nt][k] = st.ns[nt][k] = INFINITY;
+      st.nm[nt][k] = st.ns[nt][k] = kNoMax;
       st.l[nt][k] = 0.f;
     }
 #pragma unroll
@@ -195,8 +198,7 @@ __device__ __forceinline__ void tree_begin(const TreeArgs& a, int seat, int tok0
 // The fp32 products of one tile (acc: keys g and g + 8 of columns 2t, 2t + 1) into the running state; returns the P^T
 // fragments and the probabilities. k0, k1: score factors of the two keys; ev0, ev1: their V exponents (FP8 cache rows; 1
 // and 0 for others). MASKED: hide[nt] bit 0 / 1 set: the lane's token does not see key g / g + 8.
-// The maxima are lazy: they move when some score passes one by more than 2^8 (or comes first: +inf - the initial
-// maximum), which is voted on and rare, so a tile has no exchange between lanes and no rescaling.
+// The maxima are lazy: they move when some score passes one by more than 2^8 (or comes first: the initial one is -kNoMax), which is voted on and rare, so a tile has no exchange between lanes and no rescaling.
 template <bool FP8, int NT, bool HALF_P, bool MASKED>
 __device__ __forceinline__ void tree_softmax(TreeState<FP8, NT>& st, const float (&acc)[NT][4], float k0, float k1,
                                              float ev0, float ev1, const uint32_t (&hide)[NT], uint32_t (&pf)[NT][2],
@@ -241,7 +243,6 @@ __device__ __forceinline__ void tree_softmax(TreeState<FP8, NT>& st, const float
           }
           if (!FP8) st.l[nt][c] *= alpha;
         }
-        if (ref == INFINITY) ref = 0.f;               // nothing seen yet
         p[nt][c] = w0 + ref;
         p[nt][2 + c] = w1 + ref;
         if (FP8) {
@@ -251,7 +252,6 @@ __device__ __forceinline__ void tree_softmax(TreeState<FP8, NT>& st, const float
             st.l[nt][c] *= tree_exp2(-rs - ms);
             rs = st.ns[nt][c] = -ms;
           }
-          if (rs == INFINITY) rs = 0.f;
           x[nt][c] = s[0] + rs;
           x[nt][2 + c] = s[1] + rs;
         }
@@ -476,7 +476,7 @@ __device__ __forceinline__ void tree_finish(const TreeArgs& a, const TreeItem& i
       l[k] = sum_over_rows(st.l[nt][k]);
       mx[k] = FP8 ? -st.ns[nt][k] : -st.nm[nt][k];
       // outputs relative to the maximum that l is relative to
-      r[k] = FP8 && st.nm[nt][k] != INFINITY && st.ns[nt][k] != INFINITY ? exp2f(st.ns[nt][k] - st.nm[nt][k]) : 1.f;
+      r[k] = FP8 && st.nm[nt][k] != kNoMax && st.ns[nt][k] != kNoMax ? exp2f(st.ns[nt][k] - st.nm[nt][k]) : 1.f;
       if (slot < 0) r[k] = (padded || l[k] == 0.f) ? 0.f : r[k] / l[k];
     }
     if (tok >= a.tokens) continue;

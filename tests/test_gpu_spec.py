@@ -8,6 +8,8 @@ max_j p_j max_d |v_jd| (a row's largest e4m3 value is at least 224, half of 448)
 products and sums is off by 2^-24 of sum |q k| at most; with |q| |k| scale <= 64 here that is under 2^-11 in log units
 for unit-sized data, twice (numerator and sum): 2^-10 A.
 """
+import math
+
 import pytest
 import torch
 
@@ -480,3 +482,41 @@ def test_int64_positions_of_tables_past_int32_are_refused(q3):
         q3.kv_dequant_paged(*cache, seat.long(), bt, seat)
     q3.kv_quant_append_paged(k, k, *cache, seat, bt, seat.long())
     assert q3._lib.read_status() == 0 and bits(cache[2]).any()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("T", [1, 3, 4, 7, 8, 12, 20, 64])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_keys_that_score_minus_infinity_come_first(q3, fp8, T, infinite):
+    """A seat's first keys score -inf (a product past fp32's range, or K of -inf) for every head and token, the later ones
+    zero: the first have no weight. A seat of such keys alone, without visible drafts, has zero rows."""
+    if infinite and fp8:
+        return                                                  # an 8-bit cache holds no infinities
+    lens, page = [40, 16, 17, 5], 16
+    bt, pages = table_for(lens, page, 1)
+    x = torch.zeros(pages * page, 8, 128)
+    for b, n in enumerate(lens):
+        x.view(pages, page, 8, 128)[bt[b, 0].item()] = -math.inf if infinite else 4.0
+    v = rows(pages * page, 3, -1, 1)
+    (kq, ks), (vq, vs) = ((lambda y, e: (y.float().to(torch.float8_e4m3fn), (e + 127).to(torch.uint8).view(torch.float8_e8m0fnu)))(*OSP.quantise(z))
+                          for z in (x.to(BF).nan_to_num(neginf=0), v))
+    kp, vp = (kq, vq) if fp8 else (x.to(BF), v)
+    shape = lambda z, *s: z.view(pages, page, 8, *s)  # noqa: E731
+    vals = (shape(OSP.values(kq, ks), 128), shape(OSP.values(vq, vs), 128)) if fp8 else (shape(kp, 128), shape(vp, 128))
+    q = torch.full((4, T, 16, 128), 1.0 if infinite else -2e38).to(BF)
+    k, dv = torch.zeros(4, T, 8, 128, dtype=BF), rows(4 * T, 4, -1, 1).view(4, T, 8, 128)
+    mask = torch.zeros(4, T, dtype=torch.int64)
+    mask[:3] = torch.tensor([1 << i if i < 63 else -(1 << 63) for i in range(T)])
+    sc = dict(k_scale=shape(ks).to(DEV), v_scale=shape(vs).to(DEV)) if fp8 else {}
+    got = q3.paged_tree_attn(*dev(q, k, dv, mask), *dev(shape(kp, 128), shape(vp, 128)), torch.tensor(lens, dtype=torch.int32, device=DEV),
+                             bt.to(DEV), SCALE, **sc)
+    ref = OSP.tree_attention(q, k, dv, mask, *vals, lens, bt, SCALE)
+    assert not got.cpu()[3].float().abs().any()
+    check_attention(got[:3], [r[:3] for r in ref], lens[:3], fp8, True)
+    if T == 1 and fp8:
+        got = q3.paged_decode_quant(q[:, 0].to(DEV), *dev(shape(kq, 128), shape(vq, 128)), sc["k_scale"], sc["v_scale"],
+                                    torch.tensor(lens, dtype=torch.int32, device=DEV), bt.to(DEV), SCALE)
+        assert not got.cpu()[[1, 3]].float().abs().any()
+        ref = OSP.tree_attention(q, None, None, None, *vals, lens, bt, SCALE)
+        check_attention(got.cpu()[[0, 2], None], [r[[0, 2]] for r in ref], [40, 17], True, False)
+    assert q3._lib.read_status() == 0
