@@ -4,8 +4,10 @@
 //   log p(v) = (x_v - m) / T - ln s          entropy = ln s - ln 2 * t / s
 // Each thread keeps (m, s, t) of what it has seen; a larger m moves them by d = (m_old - m_new) log2(e) / T:
 // s <- 2^d s, t <- 2^d (t + d s) (with the old s). x - m is formed before it is scaled, so logits of any size, the
-// lowest finite value included, neither overflow nor lose digits. Logits of -inf add nothing; a NaN or +inf makes the
-// row's numbers NaN, and so does a row of -inf alone.
+// lowest finite value included, neither overflow nor lose digits. A tile's 16 (fp32: 8) terms are summed from zero before
+// they join s and t: next to a term of 1, single terms below 2^-24 would be lost one by one (a row of 151000 with 150999
+// tokens at e^-16.75: log probabilities off by 1.6e-5 so, by 1 to 2e-6 here, in the same time). Logits of -inf add
+// nothing; a NaN or +inf makes the row's numbers NaN, and so does a row of -inf alone.
 // The top n are ordered by (value descending, id ascending), NaN above everything: 64-bit keys, the value's order-
 // preserving bits above the complement of the id, all different.
 //
@@ -319,15 +321,18 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobAr
     }
     const float ref = m == -INFINITY ? 0.f : m;
     const float2 nref = make_float2(-ref, -ref), cc = make_float2(c, c);
+    float2 ts = make_float2(0.f, 0.f), tt = ts;   // the tile's s and t
 #pragma unroll
     for (int j = 0; j < kLpVecs; ++j)
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) {
         const float2 z = __fmul2_rn(__fadd2_rn(Vec<T>::pair(w[j], i), nref), cc);
         const float2 p = make_float2(exp2_fast(z.x), exp2_fast(z.y));
-        s2 = __fadd2_rn(s2, p);
-        t2 = __ffma2_rn(p, make_float2(fmaxf(z.x, -1000.f), fmaxf(z.y, -1000.f)), t2);   // 0 * -inf would be NaN
+        ts = __fadd2_rn(ts, p);
+        tt = __ffma2_rn(p, make_float2(fmaxf(z.x, -1000.f), fmaxf(z.y, -1000.f)), tt);   // 0 * -inf would be NaN
       }
+    s2 = __fadd2_rn(s2, ts);
+    t2 = __fadd2_rn(t2, tt);
   }
   float s = s2.x + s2.y, t = t2.x + t2.y;
 

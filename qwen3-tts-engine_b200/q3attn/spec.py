@@ -141,6 +141,7 @@ def token_logprobs(logits, ids, top_n: int = 0, temperature: float = 1.0) -> Tok
     [rows, given] (an id outside the vocabulary, such as -1 for padding, scores -inf). top_n <= min(64, vocab), ordered
     by (logit descending, id ascending), NaN first. Logits of -inf have probability 0; a row with NaN or +inf, or of
     -inf alone, gives NaN. temperature 1e-30 to 1e30. One launch.
-    Statistics are fp32: an entropy, or a log probability near zero, is good to about 1e-7 absolutely (a row that one token
-    all but owns has an entropy of few significant digits)."""
+    Statistics are fp32 and summed tile by tile: a log probability is good to (vocab / 8192 + 80) 2^-24 absolutely (fp32
+    logits: vocab / 4096), next to 2^-22 of its own size: 6e-6 at a vocabulary of 151000, 2e-6 as measured. The entropy
+    is good to that times 2 + ln(vocab) + entropy, so a row that one token all but owns has one of few significant digits."""
     return TokenLogprobs(*_op("token_logprobs")(logits, ids, top_n, temperature))

@@ -161,3 +161,27 @@ def test_graph_replay(q3):
 def test_no_rows(q3):
     got = q3.token_logprobs(torch.empty(0, 100, device=DEV), torch.empty(0, dtype=torch.int64, device=DEV), 3)
     assert got.logprobs.shape == (0,) and got.top_ids.shape == (0, 3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v", [(500, 151000), (2, 151000), (460, 40007), (1, 2000003)])
+def test_many_small_probabilities_next_to_a_certain_token(q3, dtype, n, v):
+    """One token at 1, all others at e^-16.75 = 0.89 * 2^-24 of it: none of them may be lost in a sum that holds the one.
+    ln p and the entropy in closed form. Tolerance: V / 8192 tile sums (fp32: 4096) of 16 terms to a thread's half, and 61
+    roundings of exponentials, shuffles, warps and CTAs, 2^-24 of s = 1 + V e^-16.75 < 1.11 each; t / s = ln V + H times
+    that at most."""
+    d = 16.75
+    x = torch.zeros(n, v, dtype=dtype, device=DEV)
+    ids = torch.arange(n) * 997 % v
+    x[torch.arange(n), ids] = d
+    got = q3.token_logprobs(x, torch.stack([ids, (ids + 1) % v], 1).to(DEV), 1)
+    rest = (v - 1) * math.exp(-d)
+    lp, h = -math.log1p(rest), math.log1p(rest) + rest / (1 + rest) * d
+    base = 1.11 * (v / (8192 if dtype != torch.float32 else 4096) + 16 + 61) * 2.0 ** -24
+    assert torch.equal(got.top_ids[:, 0].cpu(), ids)
+    err = lambda a, b: float((a.cpu().double() - b).abs().max())  # noqa: E731
+    assert err(got.logprobs[:, 0], lp) <= base and err(got.top_logprobs[:, 0], lp) <= base
+    assert err(got.logprobs[:, 1], lp - d) <= base + d * 2.0 ** -22
+    assert err(got.entropy, h) <= base * (2 + math.log(v) + h)
+    if n > 400:
+        assert err(got.entropy, h) <= 2 * base        # the part of t that each token has is d e^-d: no cancellation
