@@ -69,6 +69,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// (x - m) / T. x - m may lie outside fp32's range where the quotient does not: halves first then, which
+// is exact.
+__device__ __forceinline__ float scaled_below(float x, float m, float inv_temp) {
+  const float d = x - m;
+  return d == -INFINITY ? (0.5f * x - 0.5f * m) * (2.f * inv_temp) : d * inv_temp;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {   // 2 ulp; results below 2^-126 are zero
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -465,13 +472,13 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobAr
   for (int i = tid; i < a.given; i += kLpThreads) {
     const long long id = a.ids[row * a.ids_stride + i];
     float lp = -INFINITY;                              // an id outside the vocabulary has no probability
-    if (id >= 0 && id < a.vocab) lp = (to_float(part.x[id]) - r.m) * a.inv_temp - log_s;
+    if (id >= 0 && id < a.vocab) lp = scaled_below(to_float(part.x[id]), r.m, a.inv_temp) - log_s;
     a.logprobs[row * a.given + i] = lp;
   }
   if (tid < n) {
     const Key k = sh.best[tid];
     a.top_ids[row * n + tid] = static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(k));
-    a.top_logprobs[row * n + tid] = (order_value(static_cast<uint32_t>(k >> 32)) - r.m) * a.inv_temp - log_s;
+    a.top_logprobs[row * n + tid] = scaled_below(order_value(static_cast<uint32_t>(k >> 32)), r.m, a.inv_temp) - log_s;
   }
 }
 

@@ -185,3 +185,15 @@ def test_many_small_probabilities_next_to_a_certain_token(q3, dtype, n, v):
     assert err(got.entropy, h) <= base * (2 + math.log(v) + h)
     if n > 400:
         assert err(got.entropy, h) <= 2 * base        # the part of t that each token has is d e^-d: no cancellation
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [1.5, 4.0, 1000.0])
+def test_logits_further_apart_than_fp32_reaches(q3, dtype, T):
+    """x - m = -2 * 3.4e38 leaves fp32, (x - m) / T need not."""
+    x = logits(4, 3001, 21, dtype)
+    x[0] = torch.finfo(dtype).min
+    x[0, 77] = torch.finfo(dtype).max
+    x[1, ::2], x[1, 5] = torch.finfo(dtype).min, torch.finfo(dtype).max / 2
+    x[2, 9], x[2, 10], x[2, 11:] = torch.finfo(dtype).max, torch.finfo(dtype).min, -math.inf
+    check(q3, x, torch.tensor([[3, 77], [4, 5], [10, 2000], [1, 2]]), 40, T)
