@@ -6,7 +6,7 @@ Every .cu under qwen3-tts-engine_b200/csrc is compiled separately (in parallel) 
 qwen3-tts-engine_b200/q3attn/libq3attn.so next to this file, where q3attn._lib loads it; csrc/torch_ops.cpp (PyTorch
 bindings written in C++) becomes libq3torch.so beside it, linked against libq3attn.so and torch's own libraries. Objects go
 to qwen3-tts-engine_b200/_build/. The library is rebuilt unless the SHA-256 of every source, header and this script (and
-the nvcc flags) equals the digest stamped beside it when it was last built, so a copied tree never runs a library that
+the nvcc flags and torch's version) equals the digest stamped beside it when it was last built, so a copied tree never runs a library that
 was built from other sources, whatever the files' modification times say.
 """
 import concurrent.futures as cf
@@ -49,8 +49,10 @@ def _deps():
 
 
 def source_digest() -> str:
-    """SHA-256 over the build inputs: each dependency's name and bytes, in name order, plus the nvcc flags."""
-    h = hashlib.sha256(" ".join(NVCC_FLAGS).encode())
+    """SHA-256 over the build inputs: each dependency's name and bytes, in name order, plus the nvcc flags and the torch
+    that the bindings are compiled against (its C++ interface differs from version to version)."""
+    import torch
+    h = hashlib.sha256(" ".join(NVCC_FLAGS + [torch.__version__, str(torch._C._GLIBCXX_USE_CXX11_ABI)]).encode())
     for d in sorted(set(_deps())):
         h.update(os.path.basename(d).encode() + b"\0")
         with open(d, "rb") as f:
