@@ -831,7 +831,7 @@ bool make_pool_map(CUtensorMap* m, const void* base, long long rows, int box_row
 }
 
 // With the moved registers the launch is refused unless the kernel was built at exactly kLaunchRegs: a setmaxnreg.inc that
-// cannot be met would wait forever.
+// cannot be met would wait forever. (build.py looks at the count when it compiles this file.)
 template <bool FP8, bool DRAFTS, int STREAMS, int NT, int STAGES>
 cudaError_t launch_tree_main(const TreeArgs& a, int shares, cudaStream_t stream) {
   using SH = TreeShape<FP8, STREAMS, NT, STAGES>;

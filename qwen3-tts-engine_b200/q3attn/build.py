@@ -13,6 +13,7 @@ import concurrent.futures as cf
 import glob
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -81,19 +82,38 @@ def torch_flags():
     return compile_, link
 
 
+def check_registers(ptxas_log: str) -> None:
+    """paged_tree.cu moves registers between its warps, from the count that a kernel is launched with: built at another
+    count its launches are refused (they could wait for ever). Raises when the compiler settled on one, so that the build
+    says it and not the first call."""
+    with open(os.path.join(CSRC, "paged_tree.cu")) as f:
+        two_streams, eight_tokens = map(int, re.search(r"kLaunchRegs = kConsumers == 16 \? (\d+) : (\d+)", f.read()).groups())
+    found = re.findall(r"Compiling entry function '\S*paged_tree_kernelILb\dELb\dELi(\d)ELi(\d)ELi\dE\S*'.*?Used (\d+) registers",
+                       ptxas_log, re.S)
+    if not found:
+        raise RuntimeError("paged_tree.cu: the compiler's output names no kernel's registers")
+    for streams, nt, used in found:
+        want = two_streams if streams == "2" else eight_tokens if nt == "2" else int(used)
+        if int(used) != want:
+            raise RuntimeError(f"paged_tree.cu ({streams} streams, {4 * int(nt)} tokens): compiled with {used} registers, its register "
+                               f"split starts from {want} (kLaunchRegs): build with CUDA 12.9, or fit the split to this compiler")
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
     if not force and not ptxas_info and up_to_date():
         return LIB
     os.makedirs(BUILD_DIR, exist_ok=True)
     cc = nvcc()
-    extra = ["-Xptxas", "-v"] if ptxas_info else []
 
     def compile_one(src):
         obj = os.path.join(BUILD_DIR, os.path.basename(src)[:-3] + ".o")
-        cmd = [cc, "-c", src, "-o", obj] + NVCC_FLAGS + extra
+        counted = os.path.basename(src) == "paged_tree.cu"
+        cmd = [cc, "-c", src, "-o", obj] + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info or counted else [])
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"nvcc failed on {os.path.basename(src)}:\n{r.stderr}")
+        if counted:
+            check_registers(r.stderr)
         return obj, r.stderr
 
     cflags, lflags = torch_flags()
