@@ -336,12 +336,6 @@ __device__ __forceinline__ void tree_tile_e4m3(TreeState<true, NT>& st, const ui
   }
 }
 
-__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {   // infinities and NaN replaced by zero
-  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
-  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
-  return w;
-}
-
 // A tile of bf16 rows: 16 cached ones (TAIL: the first `rows` real, what follows them stale), or drafted ones (DRAFT: 16,
 // or 8 in the e4m3 kernel's stages, the first `rows` real; see[nt]: bit j set when the lane's token of tile nt sees row j).
 template <bool FP8, int NT, bool TAIL, bool DRAFT>

@@ -226,12 +226,6 @@ __device__ __forceinline__ uint2 dequant4(uint32_t w, float2 f) {
   return make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(y.x, y.y));
 }
 
-__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
-  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
-  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
-  return w;
-}
-
 // ------------------------------------------------------------------ the copy warps: warp cw, tiles cw, cw + kCopyWarps, ..
 // Lane l looks after rows 4 (l & 15) .. + 3 of a tile, of K (l < 16) or V, and copies the boxes that start there. With
 // boxes of four rows or more those rows are neighbours in the pool: one table entry, one box at most. All of a tile's
@@ -352,7 +346,7 @@ __device__ __noinline__ bool tc_load_draft(const __nv_bfloat16* k, const __nv_bf
   for (int r = tid >> 4; r < drafts; r += 8) {   // the thread's own pieces
     const uint32_t at = dst + v_off + tc_unit(r, u, half);
     const uint4 x = ld_shared16(at);
-    const uint4 f = make_uint4(finite_or_zero(x.x), finite_or_zero(x.y), finite_or_zero(x.z), finite_or_zero(x.w));
+    const uint4 f = make_uint4(finite_bf16x2(x.x), finite_bf16x2(x.y), finite_bf16x2(x.z), finite_bf16x2(x.w));
     if (f.x != x.x || f.y != x.y || f.z != x.z || f.w != x.w) {
       odd = true;
       st_shared16(at, f);

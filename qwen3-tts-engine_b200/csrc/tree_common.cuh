@@ -147,6 +147,12 @@ __device__ __forceinline__ void e4m3x4_to_half2(uint32_t x, uint32_t& lo, uint32
       : "r"(x));
 }
 
+__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {   // infinities and NaN replaced by zero
+  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
+  return w;
+}
+
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 __device__ __forceinline__ float tree_exp2(float x) {   // relative error 2^-22, denormal results are zero
@@ -168,19 +174,9 @@ __device__ __forceinline__ int tree_page(const TreeArgs& a, int tok) {
   return a.page_shift >= 0 ? tok >> a.page_shift : tok / a.page_size;
 }
 
-// Pool row of token `tok` of `seat`; an entry outside the pool reads page 0 and raises its status bit.
-__device__ __forceinline__ long long tree_pool_row(const TreeArgs& a, int seat, int tok) {
-  const int pidx = tree_page(a, tok);
-  int pg = a.block_table[static_cast<long long>(seat) * a.bt_stride + pidx];
-  if (pg < 0 || pg >= a.num_pages) {
-    atomicOr(a.status, kStatusBadPage);
-    pg = 0;
-  }
-  return static_cast<long long>(pg) * a.page_size + (tok - pidx * a.page_size);
-}
-
-// The same for N tokens tok0, tok0 + STEP, ..., in two steps so that the table entries travel while other work is done:
-// tree_pages asks for them (tokens at or past `len`: none), tree_row turns one into a pool row (-1: no token).
+// Pool rows of N tokens tok0, tok0 + STEP, ... of a seat, in two steps so that the table entries travel while other work is
+// done: tree_pages asks for them (tokens at or past `len`: none), tree_row turns one into a pool row (-1: no token; an
+// entry outside the pool reads page 0 and raises its status bit).
 template <int N, int STEP>
 __device__ __forceinline__ void tree_pages(const TreeArgs& a, int seat, int tok0, int len, int (&page)[N]) {
   const int32_t* table = a.block_table + static_cast<long long>(seat) * a.bt_stride;
