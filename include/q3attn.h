@@ -317,7 +317,8 @@ typedef struct q3_quant_cache {
 /* q3_kv_append_slots / q3_kv_append_paged for an 8-bit cache: row i of k/v (bf16 [8, 128], row_stride elements apart)
  * is quantised into pool row slots[i], or into token positions[i] of seat seat_of_row[i] (NULL: seat i) of the
  * num_seats block-table rows. A row whose slot, seat, position or page is out of range is skipped and raises its
- * status bit. The destinations of one call must differ; which row's bytes a repeated one ends up with is unspecified. */
+ * status bit. The destinations of one call must differ: a repeated one ends up with any mix of its rows' bytes and scales
+ * (finite ones from finite rows), so it serves for rows that nothing reads, such as padding. */
 int q3_kv_quant_append_slots(const void* k, const void* v, int64_t row_stride, const q3_quant_cache* cache,
                              int32_t num_kv_heads, int32_t head_dim, const int64_t* slots, int32_t n_rows, void* stream);
 int q3_kv_quant_append_paged(const void* k, const void* v, int64_t row_stride, const q3_quant_cache* cache,
@@ -338,7 +339,10 @@ int q3_kv_dequant_paged(const q3_quant_cache* cache, int32_t num_kv_heads, int32
  * A token with nothing to see, one at or past draft_lens[b], and one whose scores are all -inf get zero rows (a key that
  * scores -inf has no weight). Values that a token does not see do not reach its output, whatever they are. k_new == NULL:
  * no drafted rows (tree_mask and draft_lens are not read). The cache is bf16 (k_scale == v_scale == NULL) or the 8-bit
- * format above. Sums and softmax statistics are fp32. 1 <= tokens <= 64; the workspace (q3_paged_tree_workspace_bytes,
+ * format above. Sums and softmax statistics are fp32. Probabilities meet V rounded, which q3_paged_decode's do not: to bf16
+ * over a bf16 cache, for drafted rows, and from 17 tokens on (2^-8 of each at most); to fp16 over the 8-bit cache's rows up
+ * to 16 tokens (2^-11 of each, and those below 2^-25 of the largest count as 0; q, too, is fp16 there, scaled by a power of
+ * two per token and head, exact but for elements 2^-28 and less of the largest). 1 <= tokens <= 64; the workspace (q3_paged_tree_workspace_bytes,
  * 256-byte aligned) needs no initialisation and may not be shared by calls that overlap. Entries of the block table
  * outside the pool read page 0 and raise a status bit. */
 typedef struct q3_tree_attn {

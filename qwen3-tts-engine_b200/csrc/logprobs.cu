@@ -14,15 +14,16 @@
 // Bound: HBM (the logits are read once). A row is shared by a cluster of 1 to 8 CTAs when there are few rows; every
 // CTA streams its part in tiles of 1024 16-byte vectors, the next tile's loads in flight while one is worked on; the
 // arithmetic is packed in pairs, one exponential per logit. 1030 bf16 rows of 151000 without alternatives: 64 us, 4.9
-// TB/s (tiles of 512 vectors: 71); with the top 20: 74 us; one row of 151000 with the top 64: 17 us.
+// TB/s (tiles of 512 vectors: 71); with the top 20: 74 to 78 us on four B200s; one row of 151000 with the top 64: 17 us.
 // Selection needs no pass of its own. m is a thread's largest value; the n-th largest maximum of 128 groups of two
 // threads bounds the top n from below, and only the few threads that reach it (n to 2n of 256) have their vectors
 // read again, out of the L2 cache, shared out over all threads; a thread keeps the maxima of eight segments of its
 // tiles, and only segments that reach the bound are read (all of them: the top 20 above take 83 us, the top 64 124
-// instead of 88). Rows where more than the list holds reach the bound
-// (massive ties, fewer than n logits above -inf, values in one thread's vectors) take select_tiles, which is bounded for
-// every row: it goes through the tiles with the n-th best key so far, and where nearly all threads have candidates the
-// n-th largest group maximum of the tile is a bound first, so that a tile adds n * 2 threads * 32 values at most.
+// instead of 88). Parts of rows where more than the list holds reach the bound (massive ties, fewer than n logits above
+// -inf, values in one thread's vectors) take select_tiles, which is bounded for every row: it goes through the tiles with
+// the n-th best key so far, and where more than half of the threads have candidates the n-th largest group maximum of the
+// tile is a bound first, so that a tile adds n * 2 threads * 32 values at most. (The row of 151000 with the top 64 takes 92
+// us instead of 17 when its last eighth, a CTA's whole part, is -inf.)
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 

@@ -22,11 +22,16 @@
 // size, so a box never leaves its page), laid out [head or half head][R rows][128 bytes] with the 128-byte swizzle, which
 // makes the fragment loads of the matrix instructions free of bank conflicts. (One bulk copy per row and lane into padded
 // rows cost the producer 66 cycles each, 32 a chunk: 189 us on 576 seats, e4m3.) Eight consumer warps take one KV head each.
-// One token over e4m3, 576 seats of 200 to 1200 rows: 156 us, 5.4 TB/s, 83% of a copy's rate; 288 seats x 7 tokens, bf16: 148
-// us, 5.5 TB/s, 85%. Five to eight tokens over e4m3 reach half of it: the conversions to fp16 and the softmax, latency more
-// than issue slots (40% of them are used).
+// One token over e4m3, 576 seats of 200 to 1200 rows: 155 to 163 us on four B200s, 5.2 to 5.4 TB/s, 80 to 83% of a copy's
+// rate; 288 seats x 7 tokens, bf16: 146 to 150 us, 5.5 TB/s, 84 to 86%. Four and seven tokens over e4m3 reach half of it (119
+// and 131 us): the conversions to fp16 and the softmax, latency more than issue slots (28% of them are used).
 // Scores S^T = K.Q^T and outputs O^T = V^T.P^T use mma.sync m16n8k16 with the 16 keys (dims) as the rows of A and the
 // 2 heads x 4 tokens as the 8 columns of B: with so few query columns the legacy tensor path is far below its limit.
+//
+// Roundings. P meets V in V's type, since both operands of an MMA have one: bf16 rows (cached or drafted) take it in bf16
+// (half a step is 2^-8 of it), e4m3 rows in fp16 (2^-11 of it, or 2^-25 of the largest weight: a smaller one has none), while
+// the sums of P stay fp32 and unrounded. That is at most 2^-8 (2^-11) of sum_j p_j |v_j| next to the output's own 2^-8 of
+// itself: 0.0022 instead of 0.0017 in the 2-norm over bf16, 0.0017 over e4m3. Two bf16 pieces of P would double the MMAs of P.V.
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -198,7 +203,8 @@ __device__ __forceinline__ void tree_begin(const TreeArgs& a, int seat, int tok0
 // The fp32 products of one tile (acc: keys g and g + 8 of columns 2t, 2t + 1) into the running state; returns the P^T
 // fragments and the probabilities. k0, k1: score factors of the two keys; ev0, ev1: their V exponents (FP8 cache rows; 1
 // and 0 for others). MASKED: hide[nt] bit 0 / 1 set: the lane's token does not see key g / g + 8.
-// The maxima are lazy: they move when some score passes one by more than 2^8 (or comes first: the initial one is -kNoMax), which is voted on and rare, so a tile has no exchange between lanes and no rescaling.
+// The maxima are lazy: they move when some score passes one by more than 2^8 (or comes first: the initial one is
+// -kNoMax), which is voted on and rare, so a tile has no exchange between lanes and no rescaling.
 template <bool FP8, int NT, bool HALF_P, bool MASKED>
 __device__ __forceinline__ void tree_softmax(TreeState<FP8, NT>& st, const float (&acc)[NT][4], float k0, float k1,
                                              float ev0, float ev1, const uint32_t (&hide)[NT], uint32_t (&pf)[NT][2],
@@ -595,7 +601,9 @@ __device__ __forceinline__ void tree_produce(const TreeParams& p, const TreePlan
 // once, and eight tokens in one warp beat four in each of two (registers permitting: 288 seats x 7 tokens, e4m3: 147 -> 132
 // us, bf16: 153 -> 148). Few tokens leave a warp waiting, so e4m3, where a chunk takes longest, has two streams then.
 // Registers move from warpgroup 0 (down to 32) to the consumers: with 16 of them (640 threads at 96) up to 112, with eight
-// and NT = 2 (384 threads at 168) up to 232.
+// and NT = 2 (384 threads at 168) up to 232. At these counts the compiler still spills 136 bytes a thread (stores) in the
+// two-stream decode form, 264 with drafts, 44 to 48 with NT = 2: 1.7% of the instructions executed over 576 seats in decode,
+// 0.3% over 288 seats x 7 tokens.
 template <bool FP8, int STREAMS, int NT, int STAGES>
 struct TreeShape {
   static constexpr int kConsumers = kKvHeads * STREAMS, kThreads = 128 + 32 * kConsumers;
@@ -799,9 +807,10 @@ struct TreeConfig {
 };
 
 // Few tokens: the kernel above, in groups of 4 or 8 that each read the cache. More: the tcgen05 kernel, whose time hardly
-// grows with the tokens, one share per 8 SMs (a CTA per KV head). 96 seats of 1200 to 2400 rows: bf16, 8 tokens 124 us here,
-// 9 tokens about 180 here and 141 there; e4m3, 16 tokens 193 here and 203 there (288 seats of 200 to 1200 rows: 248 and 310),
-// 17 tokens about 270 and 196. The tcgen05 kernel takes the row maximum before it scales, so a scale that is not positive
+// grows with the tokens, one share per 8 SMs (a CTA per KV head). The number of groups decides, over long and short seats
+// alike. 96 seats of 1200 to 2400 rows (288 of 200 to 1200), us, here and there: bf16, 8 tokens 132 and 163 (154 and 219), 9
+// tokens 217 and 165 (276 and 222); e4m3, 8 tokens 112 and 196 (133 and 275), 16 tokens 200 and 201 (247 and 289), 17 tokens
+// 286 and 203 (354 and 293). The tcgen05 kernel takes the row maximum before it scales, so a scale that is not positive
 // runs here too.
 TreeConfig tree_config(bool fp8, int tokens, float scale, int num_sms) {
   if (tokens > (fp8 ? 16 : 8) && scale > 0.f) return {true, tokens, max(1, num_sms / kKvHeads)};

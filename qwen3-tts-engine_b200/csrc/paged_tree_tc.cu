@@ -31,8 +31,13 @@
 // place and raise a flag, and the rows that do see it get it back at the end.
 //
 // Bound: HBM for few tokens; for 64 the exponentials come near it (128 x 64 per tile against 32 KB of K and V: 512 of
-// 1424 cycles of the SM's share of the measured copy rate). 24 seats x 64 tokens x 1000 to 8000 rows, bf16: 104 us, 4.2
-// TB/s; e4m3 is bound by instruction issue (the conversion to bf16 and the softmax: half of all issue slots).
+// 1424 cycles of the SM's share of the measured copy rate). 24 seats x 64 tokens x 1000 to 8000 rows, bf16: 104 to 117 us on
+// four B200s, 3.8 to 4.2 TB/s (28% of all issue slots, the tensor pipe active 26% of the time); over e4m3 132 us. e4m3 is
+// bound by instruction issue (the conversion to bf16 and the softmax: 51% of all issue slots over 96 seats x 64 tokens, 232
+// us; 0.8% of the instructions there are the 84 bytes a thread that the compiler spills at 96 registers).
+//
+// Roundings. P is bf16 (half a step is 2^-8 of it) over either cache, since e4m3 rows are bf16 operands here; its sums stay
+// fp32 and unrounded. K, V and Q are exact.
 #include <cuda.h>
 #include <cuda_fp16.h>
 

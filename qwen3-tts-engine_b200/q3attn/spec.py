@@ -10,7 +10,10 @@
 The cache: k_cache / v_cache [num_pages, page_size, 8, 128] float8_e4m3fn and k_scale / v_scale [num_pages, page_size, 8]
 float8_e8m0fnu (one power of two per token and head), from empty_quant_cache. Every op launches on the current stream of
 its tensors' device and never synchronises. Workspaces come from the caching allocator with each call, so calls on
-several streams, or in several captured graphs, never share one. The ops themselves (schemas, argument checks, calls)
+several streams, or in several captured graphs, never share one. Tensors start on 16-byte boundaries, and the strides of
+their rows, tokens and seats are multiples of 8 elements (block tables, lengths, masks and logits: their own type's
+alignment): other views are refused, while rows that are not contiguous within a token, and k / v of different strides,
+are copied first. The ops themselves (schemas, argument checks, calls)
 are in csrc/torch_ops.cpp: they are short, and through Python and ctypes a call would cost more host time than GPU time.
 """
 import os
@@ -78,7 +81,8 @@ def empty_quant_cache(num_pages: int, page_size: int, device):
 def kv_quant_append_slots(k, v, k_cache, v_cache, k_scale, v_scale, slots) -> None:
     """kv_append_slots for an 8-bit cache: row i of k/v [n, 8, 128] bf16 is quantised into flat pool row slots[i]. Each
     head's 128 values share the least power-of-two scale that brings the largest to 448 or less; one rounding to e4m3.
-    The slots of a call must differ. Out-of-range ones are skipped and raise a status bit."""
+    The slots of a call must differ (a repeated one ends up with a mix of its rows). Out-of-range ones are skipped and raise
+    a status bit."""
     _op("kv_quant_append_slots")(k, v, k_cache, v_cache, k_scale, v_scale, slots)
 
 
@@ -97,7 +101,8 @@ def kv_dequant_paged(k_cache, v_cache, k_scale, v_scale, positions, block_table,
 
 def paged_decode_quant(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, softmax_scale: float):
     """paged_decode over an 8-bit cache: q [B, 16, 128] over cache_seqlens[b] tokens of seat b's pages -> [B, 16, 128]
-    bf16; a seat without tokens gets zeros. Append the step's rows first (kv_quant_append_paged)."""
+    bf16; a seat without tokens gets zeros. Append the step's rows first (kv_quant_append_paged). Sums and softmax
+    statistics are fp32; q and the probabilities are rounded to fp16 (include/q3attn.h)."""
     return _op("paged_decode_quant")(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_table, float(softmax_scale))
 
 
@@ -108,7 +113,11 @@ def paged_tree_attn(q, k, v, tree_mask, k_cache, v_cache, cache_seqlens, block_t
     [B, T], or [T] for one tree in every seat; `tree_mask(parents)` builds it). q [B, T, 16, 128] and the drafted rows
     k / v [B, T, 8, 128], bf16, after RoPE at the tokens' own positions. The cache is bf16, or 8-bit with
     k_scale / v_scale, and is only read: append the accepted rows afterwards (kv_append_paged, kv_quant_append_paged).
-    draft_lens int32 [B]: seats with fewer than T drafts; their padded tokens get zero rows. -> [B, T, 16, 128] bf16."""
+    draft_lens int32 [B]: seats with fewer than T drafts; their padded tokens get zero rows. -> [B, T, 16, 128] bf16.
+    Sums and softmax statistics are fp32, but the probabilities that meet V are rounded, which paged_decode's are not: to
+    bf16 over a bf16 cache, for drafted rows and from 17 tokens on; to fp16 over an 8-bit cache's rows up to 16 tokens. So a
+    draft's output is not bit for bit what single steps give: its error against 64 bits is 0.0022 in the 2-norm over bf16
+    where unrounded probabilities leave 0.0017, the bf16 output's own."""
     return _op("paged_tree_attn")(q, k, v, tree_mask, k_cache, v_cache, cache_seqlens, block_table, float(softmax_scale),
                                   k_scale, v_scale, draft_lens)
 

@@ -520,3 +520,17 @@ def test_keys_that_score_minus_infinity_come_first(q3, fp8, T, infinite):
         ref = OSP.tree_attention(q, None, None, None, *vals, lens, bt, SCALE)
         check_attention(got.cpu()[[0, 2], None], [r[[0, 2]] for r in ref], [40, 17], True, False)
     assert q3._lib.read_status() == 0
+
+
+@pytest.mark.parametrize("n", [2, 300])
+def test_rows_that_padding_shares_stay_finite_and_the_others_exact(q3, n):
+    """Padded rows of a batch all go to one row that nothing reads: the others land as ever."""
+    cache = q3.empty_quant_cache(2 * n, 16, DEV)
+    k, v = rows(2 * n, 1), rows(2 * n, 2)
+    slots = torch.cat([torch.arange(n) * 16 + 3, torch.zeros(n, dtype=torch.int64)])
+    q3.kv_quant_append_slots(k.to(DEV), v.to(DEV), *cache, slots.to(DEV))
+    y, e = expect_cache(k[:n])
+    got = cache[0].cpu().view(-1, 8, 128)[slots[:n]].float().double()
+    assert torch.equal(got, y) and torch.equal(bits(cache[2]).view(-1, 8)[slots[:n]], e)
+    kb, vb = q3.kv_dequant_paged(*cache, torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV))
+    assert torch.isfinite(kb).all() and torch.isfinite(vb).all() and q3._lib.read_status() == 0
