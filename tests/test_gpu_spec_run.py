@@ -316,3 +316,41 @@ def test_many_seats(q3):
     ref = OSP.tree_attention(q, k, v, mask, *vals, lens, bt, SCALE, drafts)
     check_attention(got, ref, [n + T for n in lens], True, True)
     assert q3._lib.read_status() == 0
+
+
+def test_a_chunk_of_a_prompt_over_an_8_bit_prefix(q3):
+    """A prompt in two chunks over the 8-bit cache: the first chunk's rows are appended, read back as bf16 ahead of the
+    second chunk's own rows, and `prefill` attends over both (causal, aligned to the end)."""
+    first, second, page = [40, 0, 17, 130], [5, 33, 1, 70], 16
+    B = len(first)
+    bt, pages = table_for([a + b for a, b in zip(first, second)], page, 5)
+    cache, table = q3.empty_quant_cache(pages, page, DEV), bt.to(DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    k1, v1 = rows(sum(first), 1, -1, 1), rows(sum(first), 2, -3, 2)
+    pos = i32([p for n in first for p in range(n)])
+    seat = i32([b for b, n in enumerate(first) for _ in range(n)])
+    q3.kv_quant_append_paged(k1.to(DEV), v1.to(DEV), *cache, pos, table, seat)
+    kp, vp = q3.kv_dequant_paged(*cache, pos, table, seat)
+    k2, v2 = rows(sum(second), 3, -1, 1), rows(sum(second), 4, -3, 2)
+    q = torch.randn(sum(second), 16, 128, generator=gen(6)).to(BF)
+    split = lambda x, n: torch.split(x, n)  # noqa: E731
+    join = lambda a, b: torch.cat([x for p in zip(split(a, first), split(b, second)) for x in p])  # noqa: E731
+    cu = lambda n: torch.nn.functional.pad(torch.cumsum(torch.tensor(n), 0), (1, 0)).to(DEV, torch.int32)  # noqa: E731
+    out = q3.prefill(q.to(DEV), join(kp, k2.to(DEV)), join(vp, v2.to(DEV)), cu(second), cu([a + b for a, b in zip(first, second)]),
+                     max(second), SCALE).cpu()
+    for b, (got, q_) in enumerate(zip(split(out, second), split(q, second))):
+        n, m = first[b], second[b]
+        keys = torch.cat([split(kp.cpu(), first)[b], split(k2, second)[b]]).double()
+        vals = torch.cat([split(vp.cpu(), first)[b], split(v2, second)[b]]).double()
+        see = torch.arange(n + m)[None] <= n + torch.arange(m)[:, None]
+        ref = [r[None] for r in OSP.attend(q_, keys, vals, see, SCALE)]
+        check_attention(got[None], ref, [n + m], False, True)
+    # the second chunk's rows follow the first's, and the next token attends over all of them
+    q3.kv_quant_append_paged(k2.to(DEV), v2.to(DEV), *cache, i32([n + p for n, m in zip(first, second) for p in range(m)]), table,
+                             i32([b for b, m in enumerate(second) for _ in range(m)]))
+    vals = tuple(OSP.values(c.cpu(), s.cpu()) for c, s in zip(cache[:2], cache[2:]))
+    lens = [a + b for a, b in zip(first, second)]
+    q1 = torch.randn(B, 16, 128, generator=gen(7)).to(BF)
+    one = q3.paged_decode_quant(q1.to(DEV), *cache, i32(lens), table, SCALE)
+    check_attention(one[:, None], OSP.tree_attention(q1[:, None], None, None, None, *vals, lens, bt, SCALE), lens, True, False)
+    assert q3._lib.read_status() == 0
